@@ -126,6 +126,13 @@ extern "C" {
     pub fn rtb_relu_mask_f64(ctx: *mut rtb_ctx, x: *mut f64, mask: *mut f64, n: usize) -> c_int;
     pub fn rtb_sgd_update_f64(ctx: *mut rtb_ctx, p: *mut f64, g: *const f64, lr: f64, n: usize) -> c_int;
     pub fn rtb_u8_to_f32_div(ctx: *mut rtb_ctx, src: *const u8, dst: *mut f32, divisor: f32, n: usize) -> c_int;
+    pub fn rtb_gated_scan(ctx: *mut rtb_ctx, dtype: c_int, flags: c_int, gate: *const c_void, stride_g: *const isize, off_g: usize, x: *const c_void, stride_x: *const isize, off_x: usize, h0: *const c_void, h: *mut c_void, rank: usize, shape: *const usize, axis: usize) -> c_int;
+    pub fn rtb_gated_scan_backward(ctx: *mut rtb_ctx, dtype: c_int, flags: c_int, up: *const c_void, stride_u: *const isize, off_u: usize, gate: *const c_void, stride_g: *const isize, off_g: usize, x: *const c_void, stride_x: *const isize, off_x: usize, h: *const c_void, codes: *const i8, mags: *const c_void, h0: *const c_void, d_x: *mut c_void, d_gate: *mut c_void, d_h0: *mut c_void, rank: usize, shape: *const usize, axis: usize) -> c_int;
+    pub fn rtb_gated_step(ctx: *mut rtb_ctx, dtype: c_int, flags: c_int, state: *mut c_void, stride_s: *const isize, off_s: usize, gate: *const c_void, stride_g: *const isize, off_g: usize, x: *const c_void, stride_x: *const isize, off_x: usize, rank: usize, shape: *const usize) -> c_int;
+    pub fn rtb_ckpt8_store(ctx: *mut rtb_ctx, dtype: c_int, src: *const c_void, n: usize, codes: *mut i8, mags: *mut c_void) -> c_int;
+    pub fn rtb_ckpt8_restore(ctx: *mut rtb_ctx, dtype: c_int, codes: *const i8, mags: *const c_void, n: usize, dst: *mut c_void) -> c_int;
+    pub fn rtb_ckpt8_grad(ctx: *mut rtb_ctx, dtype: c_int, kind: c_int, codes: *const i8, mags: *const c_void, up: *const c_void, n: usize, dst: *mut c_void) -> c_int;
+    pub fn rtb_cross_entropy(ctx: *mut rtb_ctx, dtype: c_int, logits: *const c_void, rows: usize, classes: usize, pitch: isize, targets: *const i64, reduction: c_int, loss: *mut c_void, grad_map: *mut c_void) -> c_int;
     pub fn rtb_convert(ctx: *mut rtb_ctx, src_dtype: c_int, dst_dtype: c_int, src: *const c_void, dst: *mut c_void, n: usize) -> c_int;
     pub fn rtb_shard_range(extent: usize, parts: usize, part: usize, begin: *mut usize, end: *mut usize);
     pub fn rtb_shard_pick_dim(rank: usize, shape: *const usize, parts: usize) -> c_int;

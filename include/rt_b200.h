@@ -408,6 +408,61 @@ int rtb_u8_to_f32_div(rtb_ctx *ctx, const uint8_t *src, float *dst, float diviso
  * is alloc + this call. */
 int rtb_convert(rtb_ctx *ctx, int src_dtype, int dst_dtype, const void *src, void *dst, size_t n);
 
+/* ---- gated linear recurrence along an axis (NO COUNTERPART IN THE REFERENCE, whose only operators along an axis
+ *      are the reductions).  In processing order s along `axis` (ascending, or descending with RTB_SCAN_REVERSE):
+ *        h_s = a_s h_{s-1} + x_s              a = gate, h_{-1} = h0 (NULL: 0)
+ *        h_s = a_s h_{s-1} + (1 - a_s) x_s    with RTB_SCAN_COUPLED
+ *      gate and x are views of `shape`; stride 0 broadcasts.  h, h0 and every gradient are dense row-major: h, d_x over
+ *      `shape`, h0 and d_h0 over `shape` with dim `axis` as 1, d_gate over `shape` with the dims along which the
+ *      gate has stride 0 as 1 (summed over them, as rtb_reduce_to_shape does).  No output may overlap an input.
+ *      f32 / f64; states are held in the tensors' type, a step is one fused multiply-add.
+ *
+ *      rtb_gated_scan_backward: `up` is the gradient of every h_s; `h` the states of the forward pass, or NULL with `codes`
+ *      and `mags`, their checkpoint (rtb_ckpt8_store of the dense h).  d_x, d_gate and d_h0 may be NULL: without d_gate
+ *      neither the states nor x are read; x is read for d_gate of the coupled form only.
+ *
+ *      rtb_gated_step: one step in place, state = gate state + x (or (1 - gate) x) over views of one shape; state must not
+ *      be broadcast, and may overlap gate or x only where it is the same view.
+ *
+ *      Long axes are cut into chunks that run in parallel (results do not depend on timing); chunked calls use the
+ *      context workspace.  A carry whose wait runs out (seconds) turns the rest of its sequence to NaN instead
+ *      of hanging.  Gates in [-1, 1] behave as the formula; where a PRODUCT of gates within some thousand steps
+ *      leaves the type's range, the result may be inf or NaN though every step's is finite. -------------------- */
+enum { RTB_SCAN_REVERSE = 1, RTB_SCAN_COUPLED = 2 };
+int rtb_gated_scan(rtb_ctx *ctx, int dtype, int flags, const void *gate, const ptrdiff_t *stride_g, size_t off_g, const void *x,
+                   const ptrdiff_t *stride_x, size_t off_x, const void *h0, void *h, size_t rank, const size_t *shape, size_t axis);
+int rtb_gated_scan_backward(rtb_ctx *ctx, int dtype, int flags, const void *up, const ptrdiff_t *stride_u, size_t off_u, const void *gate,
+                            const ptrdiff_t *stride_g, size_t off_g, const void *x, const ptrdiff_t *stride_x, size_t off_x,
+                            const void *h, const int8_t *codes, const void *mags, const void *h0, void *d_x, void *d_gate,
+                            void *d_h0, size_t rank, const size_t *shape, size_t axis);
+int rtb_gated_step(rtb_ctx *ctx, int dtype, int flags, void *state, const ptrdiff_t *stride_s, size_t off_s, const void *gate,
+                   const ptrdiff_t *stride_g, size_t off_g, const void *x, const ptrdiff_t *stride_x, size_t off_x, size_t rank,
+                   const size_t *shape);
+
+/* ---- 8-bit activation checkpoints (no counterpart in the reference, whose tape keeps every saved tensor in full).
+ *      A contiguous tensor of n elements becomes n codes and ceil(n / RTB_CKPT8_BLOCK) magnitudes of its own type: a block
+ *      of 128 consecutive elements has m = max |x| and codes round(127 x / m), rounded to nearest in real
+ *      arithmetic, ties to even; a code c stands for c m / 127, at most m / 254 from x.  m, -m, 0 and masks of zeros and
+ *      ones are exact.  A block with an infinity or a NaN stands for NaN as a whole.  f32 / f64.
+ *      rtb_ckpt8_grad: dst = f'(r) up for the restored r, never written out: MUL r up, SIGMOID r (1 - r) up and TANH
+ *      (1 - r r) up (r the op's RESULT), SQUARE 2 r up (r its input).  dst may be up.  codes: 4-byte aligned. ---- */
+#define RTB_CKPT8_BLOCK 128
+enum { RTB_CKPT8_MUL = 0, RTB_CKPT8_SIGMOID = 1, RTB_CKPT8_TANH = 2, RTB_CKPT8_SQUARE = 3 };
+int rtb_ckpt8_store(rtb_ctx *ctx, int dtype, const void *src, size_t n, int8_t *codes, void *mags);
+int rtb_ckpt8_restore(rtb_ctx *ctx, int dtype, const int8_t *codes, const void *mags, size_t n, void *dst);
+int rtb_ckpt8_grad(rtb_ctx *ctx, int dtype, int kind, const int8_t *codes, const void *mags, const void *up, size_t n, void *dst);
+
+/* ---- softmax cross-entropy of (rows, classes) logits against one class per row, with its gradient map (no counterpart
+ *      in the reference, whose only loss is L1; the contract is rtb_l1_loss's).  Row r starts at logits + r * pitch.
+ *        loss = sum_r (logsumexp(x_r) - x_r[t_r])            divided by the number of counted rows for reduction 0 (mean)
+ *        grad_map (dense, may be NULL) = softmax(x_r) - [j = t_r], divided likewise
+ *      A row with t_r < 0 does not count and gets a zero map (padding); t_r >= classes makes its map and the loss NaN.
+ *      The mean of no row is NaN, the sum 0.  An entry of -inf takes no part; a row of -inf only, of +inf or
+ *      with a NaN gives NaN.  f32 / f64; the rows' losses are added in 64 bits in a fixed order.  grad_map may be the
+ *      logits' own buffer when pitch == classes. ---------------------------------------------------------------- */
+int rtb_cross_entropy(rtb_ctx *ctx, int dtype, const void *logits, size_t rows, size_t classes, ptrdiff_t pitch, const int64_t *targets,
+                      int reduction, void *loss, void *grad_map);
+
 /* ---- multi-GPU (new; the reference is single-device: `Cuda::new()` -> device 0 with
  *      `// TODO multiple devices`, src/backend/cuda.rs:155-162, 815-818).  One rank per GPU, one
  *      communicator per context.  The path shards by slabs with no data-path collective for

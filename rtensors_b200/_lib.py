@@ -19,6 +19,9 @@ OK = 0
 
 
 MASK_RELU, MASK_ABS, MASK_LEAKY_RELU, MASK_RECIPROCAL = 1, 2, 3, 4   # rtb_grad_mask kinds
+SCAN_REVERSE, SCAN_COUPLED = 1, 2                                     # rtb_gated_scan flags
+CKPT8_MUL, CKPT8_SIGMOID, CKPT8_TANH, CKPT8_SQUARE = 0, 1, 2, 3       # rtb_ckpt8_grad kinds
+CKPT8_BLOCK = 128
 # rtb_status codes used by host-side checks (include/rt_b200.h)
 ERR_INVALID, ERR_DTYPE, ERR_BROADCAST, ERR_BOUNDS, ERR_DIM, ERR_SHAPE, ERR_NONCONTIG = -1, -2, -3, -4, -5, -6, -7
 
@@ -63,6 +66,16 @@ def lib() -> C.CDLL:
         l.rtb_meta_contiguous_strides.restype = None
         l.rtb_shard_range.restype = None
         l.rtb_ctx_destroy.restype = None
+        # declared, so that calls pass plain ints: a tiny call costs the host less
+        i, n, p = C.c_int, C.c_size_t, C.c_void_p
+        view = [p, p, n]
+        l.rtb_gated_scan.argtypes = [p, i, i, *view, *view, p, p, n, p, n]
+        l.rtb_gated_scan_backward.argtypes = [p, i, i, *view, *view, *view, p, p, p, p, p, p, p, n, p, n]
+        l.rtb_gated_step.argtypes = [p, i, i, *view, *view, *view, n, p]
+        l.rtb_ckpt8_store.argtypes = [p, i, p, n, p, p]
+        l.rtb_ckpt8_restore.argtypes = [p, i, p, p, n, p]
+        l.rtb_ckpt8_grad.argtypes = [p, i, i, p, p, p, n, p]
+        l.rtb_cross_entropy.argtypes = [p, i, p, n, n, C.c_ssize_t, p, i, p, p]
         _lib = l
     return _lib
 

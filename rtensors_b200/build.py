@@ -26,7 +26,7 @@ COMMON = ["-std=c++17", "-O3", "-lineinfo", "--fmad=false", "--prec-div=true", "
 
 EW_DTYPES = list(range(13))
 PLAIN = ["rtb_planner.cpp", "rtb_context.cpp", "rtb_api.cpp", "rtb_host.cpp", "rtb_abi_v1.cpp", "rtb_reduce.cu", "rtb_reduce_ext.cu", "rtb_noalloc.cu", "rtb_mg.cu",
-         "rtb_convert.cu"]
+         "rtb_convert.cu", "rtb_scan.cu", "rtb_ckpt8.cu", "rtb_xent.cu"]
 
 
 def _units():

@@ -1,0 +1,260 @@
+// 8-bit activation checkpoints (format: rtb_ckpt8.cuh): store, restore, and the backward maps of the tape's nodes
+// fed from codes, so that the restored tensor never exists in memory.  All HBM-bound: f32 moves 5 bytes per
+// element to store or restore, 9 to apply a map.
+#include "rtb_internal.h"
+#include "rtb_ckpt8.cuh"
+
+namespace rtb {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kUnroll = 4;                                  // blocks of a warp, loads of all in flight at once
+constexpr int kTileBlocks = kWarps * kUnroll;
+
+template <typename T> struct alignas(16) Vec {
+    static constexpr int N = 16 / sizeof(T);
+    T e[N];
+};
+
+template <typename T> struct Bits;
+template <> struct Bits<float> {
+    using U = uint32_t;
+    static constexpr U inf = 0x7f800000u;
+    static __device__ __forceinline__ U abs(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+    static __device__ __forceinline__ float value(U u) { return __uint_as_float(u); }
+    static __device__ __forceinline__ U warp_max(U u) { return __reduce_max_sync(0xffffffffu, u); }
+};
+template <> struct Bits<double> {
+    using U = unsigned long long;
+    static constexpr U inf = 0x7ff0000000000000ull;
+    static __device__ __forceinline__ U abs(double x) { return (U)__double_as_longlong(x) & 0x7fffffffffffffffull; }
+    static __device__ __forceinline__ double value(U u) { return __longlong_as_double((long long)u); }
+    static __device__ __forceinline__ U warp_max(U u) {
+#pragma unroll
+        for (int d = 16; d; d >>= 1) {
+            const U v = __shfl_xor_sync(0xffffffffu, u, d);
+            u = v > u ? v : u;
+        }
+        return u;
+    }
+};
+
+// round(127 x / m), ties to even, exactly.  f32: the quotient in 64 bits decides every case (127 x is exact there, and
+// a quotient that is no tie is at least 2^-33 of itself away from one); the product with the rounded
+// reciprocal is off by less than 2e-5 and decides all but the values that near to a tie.
+struct Quantise32 {
+    float m, inv;
+    bool wide;
+    __device__ __forceinline__ explicit Quantise32(float mag) : m(mag), inv(127.0f / mag), wide(mag < 1e-30f) {}
+    __device__ __forceinline__ int code(float x) const {
+        const float t = x * inv;
+        float q = rintf(t);
+        if (wide || fabsf(t - q) > 0.4999f) q = m > 0.0f ? (float)rint(127.0 * (double)x / (double)m) : 0.0f;
+        return (int)q;
+    }
+};
+struct Quantise64 {
+    double m, down;
+    __device__ __forceinline__ explicit Quantise64(double mag) : m(mag), down(1.0) {
+        if (mag > 1e300) m = mag * 0x1p-20, down = 0x1p-20;   // 127 x stays finite
+    }
+    __device__ __forceinline__ int code(double x) const { return m > 0.0 ? (int)rint(127.0 * (x * down) / m) : 0; }
+};
+template <typename T> struct QuantiseOf;
+template <> struct QuantiseOf<float> { using type = Quantise32; };
+template <> struct QuantiseOf<double> { using type = Quantise64; };
+
+// lane l holds elements 4 l .. 4 l + 3 of its block
+template <typename T, bool VEC> __device__ __forceinline__ void load4(const T *p, size_t i, size_t n, T v[4]) {
+    if (VEC && i + 4 <= n) {
+        constexpr int N = Vec<T>::N;
+#pragma unroll
+        for (int k = 0; k < 4; k += N) {
+            const Vec<T> q = *reinterpret_cast<const Vec<T> *>(p + i + k);
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[k + j] = q.e[j];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = i + k < n ? p[i + k] : (T)0;
+    }
+}
+template <typename T, bool VEC> __device__ __forceinline__ void store4(T *p, size_t i, size_t n, const T v[4]) {
+    if (VEC && i + 4 <= n) {
+        constexpr int N = Vec<T>::N;
+#pragma unroll
+        for (int k = 0; k < 4; k += N) {
+            Vec<T> q;
+#pragma unroll
+            for (int j = 0; j < N; ++j) q.e[j] = v[k + j];
+            *reinterpret_cast<Vec<T> *>(p + i + k) = q;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k < n) p[i + k] = v[k];
+    }
+}
+
+__device__ __forceinline__ char4 load_codes(const int8_t *p, size_t i, size_t n) {
+    if (i + 4 <= n) return *reinterpret_cast<const char4 *>(p + i);
+    char4 c = make_char4(0, 0, 0, 0);
+    if (i < n) c.x = p[i];
+    if (i + 1 < n) c.y = p[i + 1];
+    if (i + 2 < n) c.z = p[i + 2];
+    return c;
+}
+__device__ __forceinline__ void store_codes(int8_t *p, size_t i, size_t n, char4 c) {
+    if (i + 4 <= n) {
+        *reinterpret_cast<char4 *>(p + i) = c;
+        return;
+    }
+    if (i < n) p[i] = c.x;
+    if (i + 1 < n) p[i + 1] = c.y;
+    if (i + 2 < n) p[i + 2] = c.z;
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) ckpt8_store_kernel(const T *src, size_t n, int8_t *codes, T *mags) {
+    const int lane = threadIdx.x & 31;
+    const size_t block0 = ((size_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * kUnroll;
+    grid_dep_sync();
+    T v[kUnroll][4];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) load4<T, VEC>(src, (block0 + u) * kCkpt8Block + lane * 4, n, v[u]);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        using B = Bits<T>;
+        const size_t i = (block0 + u) * kCkpt8Block + lane * 4;
+        typename B::U top = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = max(top, B::abs(v[u][k]));
+        top = B::warp_max(top);
+        if ((block0 + u) * kCkpt8Block >= n) continue;   // the same in the whole warp
+        char4 c = make_char4(0, 0, 0, 0);
+        T m = B::value(top);
+        if (top >= B::inf) {
+            m = B::value(B::inf | 1u);   // some NaN
+        } else {
+            const typename QuantiseOf<T>::type q(m);
+            c = make_char4(q.code(v[u][0]), q.code(v[u][1]), q.code(v[u][2]), q.code(v[u][3]));
+        }
+        store_codes(codes, i, n, c);
+        if (lane == 0) mags[block0 + u] = m;
+    }
+}
+
+// KIND < 0: restore only
+template <typename T, int KIND> __device__ __forceinline__ T map(T r, T up) {
+    if constexpr (KIND == RTB_CKPT8_MUL) return r * up;
+    if constexpr (KIND == RTB_CKPT8_SIGMOID) return r * ((T)1 - r) * up;
+    if constexpr (KIND == RTB_CKPT8_TANH) return ((T)1 - r * r) * up;
+    if constexpr (KIND == RTB_CKPT8_SQUARE) return (T)2 * r * up;
+    return r;
+}
+
+template <typename T, int KIND, bool VEC>
+__global__ void __launch_bounds__(kThreads) ckpt8_read_kernel(const int8_t *codes, const T *mags, const T *up, size_t n, T *dst) {
+    const int lane = threadIdx.x & 31;
+    const size_t block0 = ((size_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * kUnroll;
+    grid_dep_sync();
+    char4 c[kUnroll];
+    T w[kUnroll][4], m[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const size_t i = (block0 + u) * kCkpt8Block + lane * 4;
+        c[u] = load_codes(codes, i, n);
+        if (KIND >= 0) load4<T, VEC>(up, i, n, w[u]);
+        m[u] = (block0 + u) * kCkpt8Block < n ? mags[block0 + u] : (T)0;
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const size_t i = (block0 + u) * kCkpt8Block + lane * 4;
+        const Ckpt8Scale<T> scale(m[u]);
+        const int8_t code[4] = {(int8_t)c[u].x, (int8_t)c[u].y, (int8_t)c[u].z, (int8_t)c[u].w};
+        T out[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) out[k] = map<T, KIND>(scale.restore(code[k]), KIND >= 0 ? w[u][k] : (T)0);
+        store4<T, VEC>(dst, i, n, out);
+    }
+}
+
+int tiles(size_t n, unsigned *grid) {
+    const size_t blocks = (n + kCkpt8Block - 1) / kCkpt8Block, g = (blocks + kTileBlocks - 1) / kTileBlocks;
+    if (g > 0x7fffffffu) return fail(RTB_ERR_TOO_LARGE, "checkpoint of %zu elements is beyond one launch", n);
+    *grid = (unsigned)g;
+    return RTB_OK;
+}
+
+template <typename T> bool aligned16(const T *p) { return ((uintptr_t)p & 15u) == 0; }
+
+template <typename T> int store_typed(Ctx *ctx, const T *src, size_t n, int8_t *codes, T *mags) {
+    unsigned grid = 0;
+    if (int rc = tiles(n, &grid)) return rc;
+    if (aligned16(src)) launch_dep(ctx, grid, kThreads, ckpt8_store_kernel<T, true>, src, n, codes, mags);
+    else launch_dep(ctx, grid, kThreads, ckpt8_store_kernel<T, false>, src, n, codes, mags);
+    return check_launch(ctx, "ckpt8_store_kernel");
+}
+
+template <typename T, int KIND> int read_typed(Ctx *ctx, const int8_t *codes, const T *mags, const T *up, size_t n, T *dst) {
+    unsigned grid = 0;
+    if (int rc = tiles(n, &grid)) return rc;
+    if (aligned16(up) && aligned16(dst)) launch_dep(ctx, grid, kThreads, ckpt8_read_kernel<T, KIND, true>, codes, mags, up, n, dst);
+    else launch_dep(ctx, grid, kThreads, ckpt8_read_kernel<T, KIND, false>, codes, mags, up, n, dst);
+    return check_launch(ctx, "ckpt8_read_kernel");
+}
+
+template <typename T> int read_kind(Ctx *ctx, int kind, const int8_t *codes, const T *mags, const T *up, size_t n, T *dst) {
+    switch (kind) {
+        case -1: return read_typed<T, -1>(ctx, codes, mags, up, n, dst);
+        case RTB_CKPT8_MUL: return read_typed<T, RTB_CKPT8_MUL>(ctx, codes, mags, up, n, dst);
+        case RTB_CKPT8_SIGMOID: return read_typed<T, RTB_CKPT8_SIGMOID>(ctx, codes, mags, up, n, dst);
+        case RTB_CKPT8_TANH: return read_typed<T, RTB_CKPT8_TANH>(ctx, codes, mags, up, n, dst);
+        case RTB_CKPT8_SQUARE: return read_typed<T, RTB_CKPT8_SQUARE>(ctx, codes, mags, up, n, dst);
+    }
+    return fail(RTB_ERR_INVALID, "unknown checkpoint map %d", kind);
+}
+
+int check_ckpt(rtb_ctx *c, int dtype) {
+    if (!c) return fail(RTB_ERR_INVALID, "null ctx");
+    if (dtype != RTB_F32 && dtype != RTB_F64) return fail(RTB_ERR_DTYPE, "checkpoints are defined for f32 and f64 only");
+    return RTB_OK;
+}
+
+int read_any(rtb_ctx *c, int dtype, int kind, const int8_t *codes, const void *mags, const void *up, size_t n, void *dst) {
+    if (n == 0) return RTB_OK;
+    if (!codes || !mags || !dst || (kind >= 0 && !up)) return fail(RTB_ERR_INVALID, "null argument");
+    if ((uintptr_t)codes & 3u) return fail(RTB_ERR_INVALID, "the codes must be 4-byte aligned");
+    Ctx *ctx = reinterpret_cast<Ctx *>(c);
+    if (int rc = use_device(ctx)) return rc;
+    return dtype == RTB_F32 ? read_kind<float>(ctx, kind, codes, (const float *)mags, (const float *)up, n, (float *)dst)
+                            : read_kind<double>(ctx, kind, codes, (const double *)mags, (const double *)up, n, (double *)dst);
+}
+
+}  // namespace
+}  // namespace rtb
+
+using namespace rtb;
+
+RTB_API int rtb_ckpt8_store(rtb_ctx *c, int dtype, const void *src, size_t n, int8_t *codes, void *mags) {
+    if (int rc = check_ckpt(c, dtype)) return rc;
+    if (n == 0) return RTB_OK;
+    if (!src || !codes || !mags) return fail(RTB_ERR_INVALID, "null argument");
+    if ((uintptr_t)codes & 3u) return fail(RTB_ERR_INVALID, "the codes must be 4-byte aligned");
+    Ctx *ctx = reinterpret_cast<Ctx *>(c);
+    if (int rc = use_device(ctx)) return rc;
+    return dtype == RTB_F32 ? store_typed<float>(ctx, (const float *)src, n, codes, (float *)mags)
+                            : store_typed<double>(ctx, (const double *)src, n, codes, (double *)mags);
+}
+
+RTB_API int rtb_ckpt8_restore(rtb_ctx *c, int dtype, const int8_t *codes, const void *mags, size_t n, void *dst) {
+    if (int rc = check_ckpt(c, dtype)) return rc;
+    return read_any(c, dtype, -1, codes, mags, nullptr, n, dst);
+}
+
+RTB_API int rtb_ckpt8_grad(rtb_ctx *c, int dtype, int kind, const int8_t *codes, const void *mags, const void *up, size_t n, void *dst) {
+    if (int rc = check_ckpt(c, dtype)) return rc;
+    if (kind < RTB_CKPT8_MUL || kind > RTB_CKPT8_SQUARE) return fail(RTB_ERR_INVALID, "unknown checkpoint map %d", kind);
+    return read_any(c, dtype, kind, codes, mags, up, n, dst);
+}

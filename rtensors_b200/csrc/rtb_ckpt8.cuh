@@ -1,0 +1,42 @@
+// 8-bit activation checkpoints: the format, shared by the kernels that write and read it.
+//
+// kCkpt8Block consecutive elements share one magnitude m = max |x| (in the tensor's own type); an element is
+// the code c = round(127 x / m), the quotient rounded to nearest in real arithmetic, ties to even.  It stands for
+// c m / 127, half a step (m / 254) from x at most; +-m, 0 and therefore a mask of zeros and ones are exact.
+// A block that holds an infinity or a NaN has magnitude NaN and stands for NaN as a whole.
+#pragma once
+#include <cstdint>
+
+namespace rtb {
+
+constexpr int kCkpt8Shift = 7;
+constexpr int kCkpt8Block = 1 << kCkpt8Shift;   // one warp, four elements per lane
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float ckpt8_fma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double ckpt8_fma(double a, double b, double c) { return fma(a, b, c); }
+
+// m / 127 as an unevaluated sum hi + lo: c hi + c lo rounds to c m / 127 to within half an ulp and a little (a
+// single rounded m / 127 would put up to 127 / 2 ulp on m itself).  Tiny magnitudes are scaled up and
+// the result scaled back, so that hi and lo are no subnormals.
+template <typename T> struct Ckpt8Scale {
+    T hi, lo, post;
+    __device__ __forceinline__ explicit Ckpt8Scale(T m) {
+        const T tiny = sizeof(T) == 4 ? (T)1e-30f : (T)1e-280;
+        const T up = sizeof(T) == 4 ? (T)18446744073709551616.0 : (T)1.3407807929942597e154;      // 2^64, 2^512
+        const T down = sizeof(T) == 4 ? (T)5.421010862427522e-20 : (T)7.458340731200207e-155;      // 2^-64, 2^-512
+        const bool small = m < tiny;
+        m = small ? m * up : m;
+        post = small ? down : (T)1;
+        const T r127 = (T)(1.0 / 127.0);
+        hi = m * r127;
+        lo = ckpt8_fma((T)-127, hi, m) * r127;   // the residual itself is exact
+    }
+    __device__ __forceinline__ T restore(int8_t code) const {
+        const T c = (T)code;
+        return ckpt8_fma(c, hi, c * lo) * post;
+    }
+};
+#endif
+
+}  // namespace rtb

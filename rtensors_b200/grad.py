@@ -11,6 +11,13 @@ slab of the upstream, because `inverse_broadcast_gradient` keeps only the meta o
 (src/grad/backwards.rs:527).  `ref_quirks=False` is what that code means to do: seed 1 and a true
 sum over the broadcast dims.
 
+`checkpoint8=True` keeps the activations that the backward pass reads in 8 bits an element (Checkpoint8 in
+rtensors_b200.tensor) instead of in full.  Kept so: operands of `*` and of `matmul` that a tracked op produced, the maps of
+relu and abs (exact: their values are 0 and +-1), the results of sigmoid, tanh and exp, the input of square, the states of
+gated_scan_at (and x of its coupled form).  Kept in full: leaves and untracked inputs (they live anyway), the gate of a
+recurrence (its errors would add up along the axis), and what other nodes divide by or take a pole of.
+The backward kernels read the codes; only `matmul` restores its operand.
+
     with grad.enabled(ref_quirks=False) as ctx:
         w.param(); b.param()
         loss = mean_l1_loss((x.matmul(w) + b).relu(), target)
@@ -58,13 +65,13 @@ class no_grad:
 class enabled:
     """grad::with: runs the block with a thread-local GradContext (created on first use)."""
 
-    def __init__(self, ref_quirks: bool = False):
-        self.ref_quirks = ref_quirks
+    def __init__(self, ref_quirks: bool = False, checkpoint8: bool = False):
+        self.ref_quirks, self.checkpoint8 = ref_quirks, checkpoint8
 
     def __enter__(self) -> "GradContext":
         self.prev = getattr(_state, "ctx", None)
         if self.prev is None:
-            _state.ctx = GradContext(self.ref_quirks)
+            _state.ctx = GradContext(self.ref_quirks, self.checkpoint8)
         return _state.ctx
 
     def __exit__(self, *exc):
@@ -91,8 +98,8 @@ class GradHolder:
 
 
 class GradContext:
-    def __init__(self, ref_quirks: bool = False):
-        self.ref_quirks = ref_quirks
+    def __init__(self, ref_quirks: bool = False, checkpoint8: bool = False):
+        self.ref_quirks, self.checkpoint8 = ref_quirks, checkpoint8
         self.nodes: Dict[int, GradNode] = {}
         self.none_node = self._insert(GradNode("None"))
 
@@ -112,6 +119,19 @@ class GradContext:
     def _resolve(self, key: Optional[int]) -> int:
         # a key from an earlier context names nothing here: the tensor counts as an untracked input
         return key if key is not None and key in self.nodes else self.none_node
+
+    def tracked(self, tensor) -> bool:
+        return tensor.op is not None and tensor.op in self.nodes and tensor.op != self.none_node
+
+    def keep(self, tensor, activation: bool):
+        """What the tape saves of a tensor: an 8-bit checkpoint of an activation under checkpoint8, else the tensor itself."""
+        if self.checkpoint8 and activation and tensor.size and tensor.buf.dtype.is_floating_point:
+            return tensor.checkpoint8()
+        return tensor
+
+    def keep_operand(self, tensor):
+        """An operand: an activation if a tracked op other than a leaf produced it."""
+        return self.keep(tensor, self.tracked(tensor) and not self.nodes[tensor.op].is_leaf())
 
     def graph_toposort(self, root) -> List[int]:
         """Iterative depth-first post-order with cycle detection (src/grad/mod.rs:319-360)."""
@@ -216,10 +236,24 @@ def _backwards_sub(ctx, node, upstream):
             _inverse_broadcast_gradient(ctx, upstream.neg(), sv["rhs_strides"], sv["rhs_shape"])]
 
 
+def _full(saved):
+    """A saved tensor, restored if it is kept in 8 bits."""
+    from .tensor import Checkpoint8
+    return saved.restore() if isinstance(saved, Checkpoint8) else saved
+
+
+def _times(saved, upstream):
+    """saved * upstream; from the codes where no broadcast is in between."""
+    from .tensor import Checkpoint8
+    if isinstance(saved, Checkpoint8):
+        return saved.grad("mul", upstream) if saved.shape == upstream.shape else saved.restore() * upstream
+    return saved * upstream
+
+
 def _backwards_mul(ctx, node, upstream):
     sv = node.saved
-    return [_inverse_broadcast_gradient(ctx, sv["rhs"] * upstream, sv["lhs_strides"], sv["lhs_shape"]),
-            _inverse_broadcast_gradient(ctx, sv["lhs"] * upstream, sv["rhs_strides"], sv["rhs_shape"])]
+    return [_inverse_broadcast_gradient(ctx, _times(sv["rhs"], upstream), sv["lhs_strides"], sv["lhs_shape"]),
+            _inverse_broadcast_gradient(ctx, _times(sv["lhs"], upstream), sv["rhs_strides"], sv["rhs_shape"])]
 
 
 def _backwards_l1(ctx, node, upstream):
@@ -228,12 +262,24 @@ def _backwards_l1(ctx, node, upstream):
 
 
 def _backwards_relu(ctx, node, upstream):
-    return [node.saved["grad_map"] * upstream]         # :229-239
+    return [_times(node.saved["grad_map"], upstream)]  # :229-239
 
 
 def _backwards_matmul(ctx, node, upstream):
-    left, right = node.saved["left_input"], node.saved["right_input"]   # :493-510
+    left, right = _full(node.saved["left_input"]), _full(node.saved["right_input"])   # :493-510
     return [upstream.matmul(right.transpose()), left.transpose().matmul(upstream)]
+
+
+def _backwards_scan(ctx, node, upstream):
+    from .tensor import gated_scan_backward
+    sv = node.saved
+    want = tuple(p is not None for p in node.parents)
+    x = _full(sv["x"]) if want[1] and sv["coupled"] else None
+    return list(gated_scan_backward(upstream, sv["axis"], sv["gate"], sv["h"], x, sv["h0"], sv["reverse"], sv["coupled"], want))
+
+
+def _backwards_cross_entropy(ctx, node, upstream):
+    return [node.saved["grad_map"] * upstream]         # upstream is the rank-0 seed
 
 
 def _backwards_add_scalar(ctx, node, upstream):
@@ -297,11 +343,18 @@ _UNARY_BACKWARD = {
 }
 
 
+# the unary nodes whose saved tensor may be kept in 8 bits, and the map their backward applies to the codes
+_CKPT8_UNARY = {"ReLU": "mul", "Abs": "mul", "Sigmoid": "sigmoid", "Tanh": "tanh", "Exp": "mul", "Square": "square"}
+
+
 def _unary_backward(kind):
     key, dfdx = _UNARY_BACKWARD[kind]
 
     def run(ctx, node, upstream):
+        from .tensor import Checkpoint8
         t = node.saved[key]
+        if isinstance(t, Checkpoint8):
+            return [t.grad(_CKPT8_UNARY[kind], upstream)]
         if kind == "Sqrt":
             return [upstream / (t * 2.0)]
         return [dfdx(t) * upstream]
@@ -312,6 +365,7 @@ _BACKWARD = {
     "Leaf": _accumulate_grad, "None": lambda ctx, node, up: [],
     "BroadcastAdd": _backwards_add, "BroadcastSub": _backwards_sub, "BroadcastMul": _backwards_mul,
     "BroadcastDiv": _backwards_div,
+    "GatedScan": _backwards_scan, "CrossEntropy": _backwards_cross_entropy,
     "L1": _backwards_l1, "ReLU": _backwards_relu, "MatMul": _backwards_matmul,
     "AddScalar": _backwards_add_scalar, "MulScalar": _backwards_mul_scalar, "DivScalar": _backwards_div_scalar,
     "Negate": _backwards_negate, "Permute": _backwards_permute, "Unsqueeze": _backwards_unsqueeze,
@@ -328,7 +382,8 @@ def attach_broadcast(kind: str, out, a, b) -> None:
     shape, sa, sb = broadcast_params(a.meta, b.meta)
     saved = {"lhs_strides": tuple(sa), "rhs_strides": tuple(sb), "lhs_shape": tuple(a.shape), "rhs_shape": tuple(b.shape)}
     if kind == "BroadcastMul":
-        saved["lhs"], saved["rhs"] = a, b            # read in place; the reference copies both operands
+        if ctx.tracked(a) or ctx.tracked(b):
+            saved["lhs"], saved["rhs"] = ctx.keep_operand(a), ctx.keep_operand(b)   # read in place; the reference copies both
     if kind == "BroadcastDiv":
         with no_grad():                               # the reciprocal map in one kernel (reference: a get / set loop)
             saved["lhs"], saved["rhs_reciprocal"] = a, b.reciprocal_map()
@@ -338,13 +393,32 @@ def attach_broadcast(kind: str, out, a, b) -> None:
 def attach_unary(kind: str, out, src, **saved) -> None:
     ctx = _ctx()
     if ctx is not None:
+        if kind in _CKPT8_UNARY and ctx.tracked(src):
+            # an input is an activation if a tracked op produced it; a result or a map always is
+            saved = {k: ctx.keep_operand(v) if k == "input" else ctx.keep(v, True) for k, v in saved.items()}
         ctx.attach(out, GradNode(kind, [src.op], dict(saved)))
 
 
 def attach_matmul(out, a, b) -> None:
     ctx = _ctx()
     if ctx is not None:
-        ctx.attach(out, GradNode("MatMul", [a.op, b.op], {"left_input": a, "right_input": b}))
+        if ctx.tracked(a) or ctx.tracked(b):
+            a_kept, b_kept = ctx.keep_operand(a), ctx.keep_operand(b)
+            ctx.attach(out, GradNode("MatMul", [a.op, b.op], {"left_input": a_kept, "right_input": b_kept}))
+
+
+def attach_scan(out, x, gate, h0, axis, reverse, coupled) -> None:
+    ctx = _ctx()
+    if ctx is not None and any(t is not None and ctx.tracked(t) for t in (x, gate, h0)):
+        saved = {"gate": gate, "x": ctx.keep_operand(x) if coupled else None, "h0": h0, "axis": axis, "reverse": reverse, "coupled": coupled}
+        saved["h"] = ctx.keep(out, True) if ctx.tracked(gate) else None    # only the gate's gradient reads the states
+        ctx.attach(out, GradNode("GatedScan", [x.op, gate.op, None if h0 is None else h0.op], saved))
+
+
+def attach_cross_entropy(loss, logits, grad_map) -> None:
+    ctx = _ctx()
+    if ctx is not None:
+        ctx.attach(loss, GradNode("CrossEntropy", [logits.op], {"grad_map": grad_map, "loss": loss}))
 
 
 def attach_l1(loss, a, b, grad_map) -> None:

@@ -15,7 +15,7 @@ import torch
 from . import _lib as L
 from . import grad as _grad
 from .backend import CODE_TO_NP, CudaB200, dtype_code
-from .meta import Meta
+from .meta import Meta, broadcast_params
 
 _NP_TO_TORCH = {np.dtype(np.float32): torch.float32, np.dtype(np.float64): torch.float64,
                 np.dtype(np.int8): torch.int8, np.dtype(np.int16): torch.int16, np.dtype(np.int32): torch.int32,
@@ -305,6 +305,166 @@ class Tensor:
     def logsumexp(self): return self.logsumexp_at(None)
     def argmax(self): return self.argmax_at(None)
     def argmin(self): return self.argmin_at(None)
+
+    # ---- gated linear recurrence --------------------------------------------------------------
+    def _spread(self, meta: Meta, what: str) -> Meta:
+        """`meta` broadcast to this tensor's shape."""
+        if meta.shape == self.meta.shape:
+            return meta
+        shape, _, strides = broadcast_params(self.meta, meta)
+        if shape != tuple(self.shape):
+            raise L.RtbError(L.ERR_BROADCAST, f"{what} of shape {meta.shape} does not broadcast to {self.shape}")
+        return Meta(shape, strides, meta.offset)
+
+    def gated_scan_at(self, axis: int, gate: "Tensor", h0: Optional["Tensor"] = None, reverse: bool = False,
+                      coupled: bool = False) -> "Tensor":
+        """The gated linear recurrence h_s = gate_s h_{s-1} + x_s along `axis`, x being this tensor: descending with
+        `reverse`, h_s = gate_s h_{s-1} + (1 - gate_s) x_s with `coupled`.  gate broadcasts to x's shape; h0 is the state
+        in front of the first step, x's shape with `axis` as 1 (zero without it).  -> every state."""
+        gate, gm, h0 = _scan_operands(self, axis, gate, h0)
+        out = Tensor(self.backend, self.backend.gated_scan(self.buf, self.meta, gate.buf, gm, axis, None if h0 is None else h0.buf,
+                                                           reverse, coupled), Meta.contiguous(self.shape))
+        if _grad.is_enabled():
+            _grad.attach_scan(out, self, gate, h0, axis, reverse, coupled)
+        return out
+
+    def gated_step_inplace(self, gate: "Tensor", x: "Tensor", coupled: bool = False) -> "Tensor":
+        """One step of the recurrence with this tensor as the state: h = gate h + x (or gate h + (1 - gate) x) in place."""
+        self.backend.gated_step(self.buf, self.meta, gate.buf, self._spread(gate.meta, "the gate"), x.buf, self._spread(x.meta, "x"), coupled)
+        return self
+
+    # ---- 8-bit checkpoints --------------------------------------------------------------------
+    def checkpoint8(self) -> "Checkpoint8":
+        """The tensor in 8 bits an element (see Checkpoint8), in row-major order of its shape."""
+        c = _dense(self)
+        codes, mags = self.backend.ckpt8_store(c.buf, c.size, c.offset)
+        return Checkpoint8(self.backend, codes, mags, tuple(self.shape))
+
+
+class Checkpoint8:
+    """A float tensor kept in 8 bits: codes -127 .. 127 and one magnitude for each 128 consecutive elements.  A code c
+    stands for c m / 127, at most m / 254 from the element, m being the largest magnitude of the block; a block with
+    an infinity or a NaN stands for NaN."""
+
+    KINDS = {"mul": L.CKPT8_MUL, "sigmoid": L.CKPT8_SIGMOID, "tanh": L.CKPT8_TANH, "square": L.CKPT8_SQUARE}
+
+    def __init__(self, backend: CudaB200, codes: torch.Tensor, mags: torch.Tensor, shape):
+        self.backend, self.codes, self.mags = backend, codes, mags
+        self.meta = Meta.contiguous(shape)
+
+    @property
+    def shape(self): return self.meta.shape
+    @property
+    def size(self): return self.meta.size
+
+    def restore(self) -> Tensor:
+        return Tensor(self.backend, self.backend.ckpt8_restore(self.codes, self.mags, self.size), self.meta)
+
+    def grad(self, kind: str, upstream: Tensor) -> Tensor:
+        """f'(r) * upstream for the restored r, which is never written out: "mul" r u; "sigmoid" r (1 - r) u and "tanh"
+        (1 - r r) u with r the op's result; "square" 2 r u with r its input."""
+        if kind not in self.KINDS:
+            raise L.RtbError(L.ERR_INVALID, f"unknown checkpoint map {kind!r}")
+        if upstream.shape != self.shape:
+            raise L.RtbError(L.ERR_SHAPE, f"an upstream of shape {upstream.shape} for a checkpoint of shape {self.shape}")
+        u = _dense(upstream)
+        return Tensor(self.backend, self.backend.ckpt8_grad(self.KINDS[kind], self.codes, self.mags, u.buf, self.size, u.offset), self.meta)
+
+
+def _is_dense(m: Meta) -> bool:
+    """Row-major without gaps (Meta.is_contiguous also takes reversed dims)."""
+    return m.strides == Meta.contiguous(m.shape).strides or m.size == 0
+
+
+def _dense(t: Tensor, force: bool = False) -> Tensor:
+    """`t`, or a row-major copy of it that stands for the same node on the tape."""
+    if _is_dense(t.meta) and not force:
+        return t
+    c = t.contiguous()
+    c.op = t.op
+    return c
+
+
+def _scan_operands(x, axis: int, gate: Tensor, h0: Optional[Tensor]):
+    """-> (gate, its meta over x's shape, h0 dense from the start of its buffer)."""
+    if not 0 <= axis < x.rank:
+        raise L.RtbError(L.ERR_DIM, f"axis {axis} out of range for rank {x.rank}")
+    if any(st == 0 and n != 1 for st, n in zip(gate.strides, gate.shape)):
+        gate = _dense(gate, force=True)     # a stride of 0 marks the dims that broadcasting adds
+    gm = x._spread(gate.meta, "the gate")
+    if h0 is not None:
+        first = tuple(1 if k == axis else n for k, n in enumerate(x.shape))
+        if h0.shape != first:
+            raise L.RtbError(L.ERR_SHAPE, f"h0 of shape {h0.shape}, {first} is needed")
+        h0 = _dense(h0, force=h0.offset != 0)
+    return gate, gm, h0
+
+
+def gated_scan_backward(upstream: Tensor, axis: int, gate: Tensor, h, x: Optional[Tensor] = None, h0: Optional[Tensor] = None,
+                        reverse: bool = False, coupled: bool = False, want=(True, True, True)):
+    """Gradients of `x.gated_scan_at(axis, gate, h0, reverse, coupled)` for the upstream of its states: h is its result or
+    the result's Checkpoint8; x is needed for the coupled gate's gradient.  -> (d_x, d_gate in the gate's shape,
+    d_h0), None for what is not wanted and for d_h0 without h0."""
+    gate, gm, h0 = _scan_operands(upstream, axis, gate, h0)
+    if upstream.size == 0:      # no step at all: nothing reaches the gate or the first state
+        z = [Tensor.zeros(t.shape, t.np_dtype, t.backend) if w and t is not None else None for t, w in zip((upstream, gate, h0), want)]
+        return z[0], z[1], z[2]
+    kept = {}
+    if want[1]:
+        if h is None or h.shape != upstream.shape:
+            raise L.RtbError(L.ERR_SHAPE, f"states of shape {None if h is None else h.shape} for an upstream of shape {upstream.shape}")
+        if isinstance(h, Checkpoint8):
+            kept["ckpt"] = (h.codes, h.mags)
+        else:
+            h = h if h.offset == 0 and _is_dense(h.meta) else h.contiguous()
+            kept["h"] = h.buf
+    b = upstream.backend
+    dx, dg, dh0 = b.gated_scan_backward(upstream.buf, upstream.meta, gate.buf, gm, axis, x=None if x is None else x.buf,
+                                        xm=None if x is None else x.meta, h0=None if h0 is None else h0.buf, reverse=reverse,
+                                        coupled=coupled, want=want, **kept)
+    return (None if dx is None else Tensor(b, dx, Meta.contiguous(upstream.shape)),
+            None if dg is None else Tensor(b, dg, Meta.contiguous(gate.shape)),
+            None if dh0 is None else Tensor(b, dh0, Meta.contiguous(h0.shape)))
+
+
+def cross_entropy_loss(logits: Tensor, targets: Tensor, with_grad: bool = False, reduction: str = "mean"):
+    """Softmax cross-entropy as a rank-0 tensor: logits (..., classes), targets an integer tensor of the leading shape.  A
+    negative target marks a row that does not count (padding), one beyond the classes makes the loss NaN.
+    "mean" divides by the number of counted rows, "sum" does not; with_grad also returns the gradient map."""
+    if logits.rank == 0 or targets.shape != logits.shape[:-1]:
+        raise L.RtbError(L.ERR_SHAPE, f"logits of shape {logits.shape} with targets of shape {targets.shape}")
+    if reduction not in ("mean", "sum"):
+        raise L.RtbError(L.ERR_INVALID, f"unknown reduction {reduction!r}")
+    if targets.buf.dtype.is_floating_point or targets.buf.dtype == torch.bool:
+        raise L.RtbError(L.ERR_DTYPE, f"targets of {targets.buf.dtype}: class numbers are needed")
+    b = logits.backend
+    t = _dense(targets)
+    tb = t.buf[t.offset: t.offset + t.size] if t.offset or t.buf.numel() != t.size else t.buf
+    if tb.dtype != torch.int64:
+        tb = b.convert(tb, torch.int64)
+    classes = logits.shape[-1]
+    rows = targets.size
+    m = logits.meta
+    if logits.rank == 2 and (m.strides[1] == 1 or classes == 1) and m.size:
+        x, pitch = logits, m.strides[0]          # rows of a wider matrix, reversed rows: read in place
+    else:
+        x = _dense(logits)
+        pitch = classes
+    loss, g = b.cross_entropy(x.buf, rows, classes, tb, 0 if reduction == "mean" else 1, with_grad, pitch, x.offset)
+    lt = Tensor(b, loss, Meta.contiguous(()))
+    if with_grad:
+        return lt, Tensor(b, g, Meta.contiguous(logits.shape))
+    return lt
+
+
+def cross_entropy_loss_tracked(logits: Tensor, targets: Tensor, reduction: str = "mean") -> Tensor:
+    """cross_entropy_loss under a grad context: one call gives the loss and its gradient map, and a CrossEntropy node goes on
+    the tape."""
+    if not _grad.is_enabled():
+        return cross_entropy_loss(logits, targets, reduction=reduction)
+    loss, gmap = cross_entropy_loss(logits, targets, True, reduction)
+    _grad.attach_cross_entropy(loss, logits, gmap)
+    return loss
 
 
 def mean_l1_loss(a: Tensor, b: Tensor, with_grad: bool = False):
