@@ -424,10 +424,10 @@ int rtb_convert(rtb_ctx *ctx, int src_dtype, int dst_dtype, const void *src, voi
  *      rtb_gated_step: one step in place, state = gate state + x (or (1 - gate) x) over views of one shape; state must not
  *      be broadcast, and may overlap gate or x only where it is the same view.
  *
- *      Long axes are cut into chunks that run in parallel (results do not depend on timing); chunked calls use the
- *      context workspace.  A carry whose wait runs out (seconds) turns the rest of its sequence to NaN instead
- *      of hanging.  Gates in [-1, 1] behave as the formula; where a PRODUCT of gates within some thousand steps
- *      leaves the type's range, the result may be inf or NaN though every step's is finite. -------------------- */
+ *      Long axes are cut into parts that run in parallel; the results do not depend on timing.  Gates in [-1, 1] behave
+ *      as the formula; where a PRODUCT of gates within some thousand steps leaves the type's range, the result
+ *      may be inf or NaN though every step's is finite.  A view that is not read in place (its innermost dim strided), and
+ *      the gradient of a broadcast gate, may take a block of the context allocator. -------------------------- */
 enum { RTB_SCAN_REVERSE = 1, RTB_SCAN_COUPLED = 2 };
 int rtb_gated_scan(rtb_ctx *ctx, int dtype, int flags, const void *gate, const ptrdiff_t *stride_g, size_t off_g, const void *x,
                    const ptrdiff_t *stride_x, size_t off_x, const void *h0, void *h, size_t rank, const size_t *shape, size_t axis);

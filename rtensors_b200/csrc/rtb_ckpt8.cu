@@ -97,12 +97,11 @@ template <typename T, bool VEC> __device__ __forceinline__ void store4(T *p, siz
     }
 }
 
-__device__ __forceinline__ char4 load_codes(const int8_t *p, size_t i, size_t n) {
-    if (i + 4 <= n) return *reinterpret_cast<const char4 *>(p + i);
-    char4 c = make_char4(0, 0, 0, 0);
-    if (i < n) c.x = p[i];
-    if (i + 1 < n) c.y = p[i + 1];
-    if (i + 2 < n) c.z = p[i + 2];
+__device__ __forceinline__ uint32_t load_codes(const int8_t *p, size_t i, size_t n) {
+    if (i + 4 <= n) return *reinterpret_cast<const uint32_t *>(p + i);
+    uint32_t c = 0;
+    for (int k = 0; k < 3; ++k)
+        if (i + k < n) c |= (uint32_t)(uint8_t)p[i + k] << (8 * k);
     return c;
 }
 __device__ __forceinline__ void store_codes(int8_t *p, size_t i, size_t n, char4 c) {
@@ -159,7 +158,7 @@ __global__ void __launch_bounds__(kThreads) ckpt8_read_kernel(const int8_t *code
     const int lane = threadIdx.x & 31;
     const size_t block0 = ((size_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * kUnroll;
     grid_dep_sync();
-    char4 c[kUnroll];
+    uint32_t c[kUnroll];
     T w[kUnroll][4], m[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -172,10 +171,9 @@ __global__ void __launch_bounds__(kThreads) ckpt8_read_kernel(const int8_t *code
     for (int u = 0; u < kUnroll; ++u) {
         const size_t i = (block0 + u) * kCkpt8Block + lane * 4;
         const Ckpt8Scale<T> scale(m[u]);
-        const int8_t code[4] = {(int8_t)c[u].x, (int8_t)c[u].y, (int8_t)c[u].z, (int8_t)c[u].w};
         T out[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) out[k] = map<T, KIND>(scale.restore(code[k]), KIND >= 0 ? w[u][k] : (T)0);
+        for (int k = 0; k < 4; ++k) out[k] = map<T, KIND>(scale.restore(c[u], k), KIND >= 0 ? w[u][k] : (T)0);
         store4<T, VEC>(dst, i, n, out);
     }
 }

@@ -32,9 +32,13 @@ template <typename T> struct Ckpt8Scale {
         hi = m * r127;
         lo = ckpt8_fma((T)-127, hi, m) * r127;   // the residual itself is exact
     }
-    __device__ __forceinline__ T restore(int8_t code) const {
-        const T c = (T)code;
-        return ckpt8_fma(c, hi, c * lo) * post;
+    __device__ __forceinline__ T restore(T c) const { return ckpt8_fma(c, hi, c * lo) * post; }
+    __device__ __forceinline__ T restore(int8_t code) const { return restore((T)code); }
+    // code k of four packed ones.  f32: the byte becomes the low mantissa byte of 2^23, two instructions where a conversion from 8
+    // bits runs at a quarter of the rate.
+    __device__ __forceinline__ T restore(uint32_t four, int k) const {
+        if constexpr (sizeof(T) == 4) return restore((T)(__uint_as_float(__byte_perm(four ^ 0x80808080u, 0x4b000000u, 0x7540u + k)) - 8388736.0f));
+        else return restore((T)(int8_t)(four >> (8 * k)));
     }
 };
 #endif

@@ -9,15 +9,14 @@
 // kernel body serves both: `s` below is always the PROCESSING index; the host folds the direction into
 // signed strides.
 //
-// Every element is read once and written once.  A tile (chunk of the axis x lanes) stays in registers from its
-// load to its store; in between the CTA learns the carry into its chunk.  Chunks of one lane group form a
-// chain: a tile publishes its own map, waits until some predecessor within kWindow chunks has published its
-// END STATE and the ones in between their maps, and folds those in axis order.  The fold from any end state
-// gives the bits of the fold from the start, so results do not depend on timing.  Tiles are
-// handed out by a ticket in chunk order: a tile only ever waits for tiles whose CTAs are already running.
-// Waits are bounded; a wait that runs out makes the carry NaN.
+// Every element is read once and written once.  The lanes (sequences) are cut into groups, the axis into rounds; a
+// cluster of CTAs owns a group and takes one round after the other, each CTA a consecutive part of it, each warp a part of
+// that.  Within a round the parts' maps travel through (distributed) shared memory, the carry between rounds stays in
+// registers: no CTA waits for memory that another one writes, and no workspace is needed.  The folds have one order,
+// so results are deterministic.  Copies run ahead in a ring of shared-memory stages; a thread (or a warp) copies what it
+// will read itself, so the ring needs no barrier.
 //
-// A product of gates that leaves the type's range inside one chunk (at most a few thousand steps) makes the
+// A product of gates that leaves the type's range inside one round (at most some thousand steps) makes the
 // carry's share inf or NaN where step-by-step evaluation might not; gates in [-1, 1] cannot.
 #include <algorithm>
 #include <vector>
@@ -30,56 +29,101 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kWindow = 32;              // predecessors a tile looks at, one flag per lane of a warp
 constexpr int kMaxLaneDims = 6;
-constexpr unsigned kSpinLimit = 1u << 22;  // polls of about a microsecond
-constexpr size_t kWsHeader = 65536;        // completion counters in front of the workspace (rtb_context.cpp)
-enum : unsigned { kFlagNone = 0, kFlagMap = 1, kFlagState = 2 };
+constexpr unsigned kMaxCluster = 8;
+constexpr unsigned long long kWaitNs = 2000000000ull;   // limit of a wait for another CTA's maps
+
 
 __device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_(double a, double b, double c) { return fma(a, b, c); }
-__device__ __forceinline__ float nan_of(float) { return __int_as_float(0x7fffffff); }
-__device__ __forceinline__ double nan_of(double) { return __longlong_as_double(0x7fffffffffffffffll); }
-
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack {
     T e[V];
 };
 template <typename T, int V> __device__ __forceinline__ Pack<T, V> ld(const T *p) { return *reinterpret_cast<const Pack<T, V> *>(p); }
 template <typename T, int V> __device__ __forceinline__ void st(T *p, const Pack<T, V> &v) { *reinterpret_cast<Pack<T, V> *>(p) = v; }
-// published tile states are read past L1
-template <typename T, int V> __device__ __forceinline__ Pack<T, V> ld_cg(const T *p) {
-    Pack<T, V> v;
-    if constexpr (sizeof(v) == 16) {
-        uint4 q = __ldcg(reinterpret_cast<const uint4 *>(p));
-        memcpy(&v, &q, 16);
+
+// asynchronous copy of BYTES (4, 8 or 16) into shared memory
+template <int BYTES> __device__ __forceinline__ void copy_async(void *smem, const void *gmem) {
+    const unsigned dst = (unsigned)__cvta_generic_to_shared(smem);
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(gmem) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(gmem), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Maps travel between the CTAs of a cluster as asynchronous stores that count their bytes on a barrier of the receiver: unlike
+// a cluster-wide barrier they do not wait for the sender's own global stores.
+__device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ unsigned in_cta(unsigned addr, unsigned rank) {
+    unsigned at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
+    return at;
+}
+template <typename P> __device__ __forceinline__ void send(unsigned to, const P &v, unsigned mbar) {
+    static_assert(sizeof(P) == 4 || sizeof(P) == 8 || sizeof(P) == 16, "one store");
+    if constexpr (sizeof(P) == 16) {
+        uint4 q;
+        memcpy(&q, &v, 16);
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(q.x),
+                     "r"(q.y), "r"(q.z), "r"(q.w), "r"(mbar) : "memory");
+    } else if constexpr (sizeof(P) == 8) {
+        unsigned long long q;
+        memcpy(&q, &v, 8);
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to), "l"(q), "r"(mbar) : "memory");
     } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) v.e[j] = __ldcg(p + j);
+        unsigned q;
+        memcpy(&q, &v, 4);
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to), "r"(q), "r"(mbar) : "memory");
     }
-    return v;
 }
-__device__ __forceinline__ unsigned ld_acquire(const unsigned *p) {
-    unsigned v;
-    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
+__device__ __forceinline__ void mbar_init(unsigned long long *bar) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(bar)) : "memory");
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
-__device__ __forceinline__ void st_release(unsigned *p, unsigned v) {
-    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+__device__ __forceinline__ void mbar_expect(unsigned long long *bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ unsigned long long now_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+// -> whether the phase completed within the limit
+__device__ __forceinline__ bool mbar_wait(unsigned long long *bar, unsigned parity) {
+    unsigned long long began = 0;
+    for (;;) {
+        unsigned done;
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+        if (done) return true;
+        if (!began) began = now_ns();
+        else if (now_ns() - began > kWaitNs) return false;
+    }
+}
+__device__ __forceinline__ float nan_of(float) { return __int_as_float(0x7fffffff); }
+__device__ __forceinline__ double nan_of(double) { return __longlong_as_double(0x7fffffffffffffffll); }
 
 // The dims other than the axis, merged as far as every operand allows, outermost first.  A lane is one
 // sequence; its element s sits at base + s * step in each operand.
 struct LaneDims {
     int nd;
     uint64_t n[kMaxLaneDims];
-    int64_t so[kMaxLaneDims], sg[kMaxLaneDims], sb[kMaxLaneDims], sx[kMaxLaneDims];
+    int64_t so[kMaxLaneDims], sg[kMaxLaneDims], sb[kMaxLaneDims], sx[kMaxLaneDims], sd[kMaxLaneDims];
 };
 
 template <typename T> struct ScanArgs {
     LaneDims dims;
     uint64_t lanes, steps;
-    int64_t to, tg, tb, tx;  // signed steps along the axis in processing order (elements)
-    int64_t o0;              // flat position of processing index 0 in the dense outputs
+    int64_t to, tg, tb, tx, td;  // signed steps along the axis in processing order (elements)
+    int64_t o0, d0;          // flat position of processing index 0 in the dense outputs, and in dg
     const T *g;              // gate, at processing index 0
     const T *b;              // forward: x; backward: the upstream
     const T *x;              // backward, coupled: x
@@ -90,20 +134,16 @@ template <typename T> struct ScanArgs {
     T *out;                  // forward: h; backward: dx (may be null)
     T *dg;                   // backward: gradient of the gate, dense (may be null)
     T *dh0;                  // backward (may be null)
-    // chunk chain (chunks > 1)
-    uint64_t groups, chunks;
-    unsigned long long *ticket;
-    unsigned *flags;         // [group][chunk]
-    T *maps;                 // [group][chunk][2][width]
-    T *states;               // [group][chunk][width]
+    int seg_shift;           // log2 of the neighbouring lanes whose share of dg is summed before it is written
+    unsigned cluster;        // CTAs that share a group of lanes
 };
 
 struct LaneAt {
-    int64_t o, g, b, x;
+    int64_t o, g, b, x, d;
 };
 
-__device__ __forceinline__ LaneAt locate(const LaneDims &d, uint64_t lane) {
-    LaneAt at{0, 0, 0, 0};
+__device__ __forceinline__ LaneAt locate(const LaneDims &d, uint64_t lane, int seg_shift) {
+    LaneAt at{0, 0, 0, 0, 0};
     // 32-bit division wherever the index allows: the 64-bit one costs about a hundred instructions
 #pragma unroll
     for (int k = kMaxLaneDims - 1; k >= 0; --k) {
@@ -121,348 +161,554 @@ __device__ __forceinline__ LaneAt locate(const LaneDims &d, uint64_t lane) {
         at.g += (int64_t)r * d.sg[k];
         at.b += (int64_t)r * d.sb[k];
         at.x += (int64_t)r * d.sx[k];
+        at.d += (int64_t)(k == d.nd - 1 ? r >> seg_shift : r) * d.sd[k];
         lane = q;
     }
     return at;
 }
 
-// Warp-wide: publishes (A, H), the map of tile `chunk` of the chain, learns the state in front of it and
-// publishes the state behind it.  `first` is the state in front of chunk 0.
-template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> chain_carry(const ScanArgs<T> &p, uint64_t group, uint64_t chunk, int lane, const Pack<T, V> &A,
-                                                  const Pack<T, V> &H, const Pack<T, V> &first) {
-    constexpr int W = 32 * V;
-    const uint64_t at = group * p.chunks + chunk;
-    const bool last = chunk + 1 == p.chunks;
-    Pack<T, V> carry = first;
-    if (chunk > 0) {
-        if (!last) {
-            st<T, V>(p.maps + (at * 2) * W + lane * V, A);
-            st<T, V>(p.maps + (at * 2 + 1) * W + lane * V, H);
-            __threadfence();
-            __syncwarp();
-            if (lane == 0) st_release(p.flags + at, kFlagMap);
-        }
-        // lane i watches predecessor chunk - 1 - i
-        const bool mine = (uint64_t)lane < chunk;
-        const unsigned *flag = p.flags + at - 1 - lane;
-        unsigned seen = kFlagNone;
-        int dist = -1;
-        for (unsigned poll = 0; poll < kSpinLimit; ++poll) {
-            if (mine && seen != kFlagState) seen = ld_acquire(flag);
-            const unsigned st_mask = __ballot_sync(0xffffffffu, seen == kFlagState);
-            const unsigned map_mask = __ballot_sync(0xffffffffu, seen != kFlagNone);
-            if (st_mask) {
-                const int d = __ffs(st_mask) - 1;                  // the nearest end state
-                const unsigned nearer = d ? (1u << d) - 1u : 0u;
-                if ((map_mask & nearer) == nearer) {
-                    dist = d;
-                    break;
-                }
-            }
-        }
-        __syncwarp();
-        if (dist < 0) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) carry.e[j] = nan_of(T());
-        } else {
-            const uint64_t from = at - 1 - dist;
-            carry = ld_cg<T, V>(p.states + from * W + lane * V);
-            // fold the maps in between in axis order, a batch of loads ahead of each batch of folds
-            constexpr int kBatch = 4;
-            for (int d = 0; d < dist; d += kBatch) {
-                Pack<T, V> a[kBatch], h[kBatch];
-#pragma unroll
-                for (int k = 0; k < kBatch; ++k)
-                    if (d + k < dist) {
-                        a[k] = ld_cg<T, V>(p.maps + ((from + 1 + d + k) * 2) * W + lane * V);
-                        h[k] = ld_cg<T, V>(p.maps + ((from + 1 + d + k) * 2 + 1) * W + lane * V);
-                    }
-#pragma unroll
-                for (int k = 0; k < kBatch; ++k)
-                    if (d + k < dist) {
-#pragma unroll
-                        for (int j = 0; j < V; ++j) carry.e[j] = fma_(a[k].e[j], carry.e[j], h[k].e[j]);
-                    }
-            }
-        }
-    }
-    if (!last) {
-        Pack<T, V> end;
-#pragma unroll
-        for (int j = 0; j < V; ++j) end.e[j] = fma_(A.e[j], carry.e[j], H.e[j]);
-        st<T, V>(p.states + at * W + lane * V, end);
-        __threadfence();
-        __syncwarp();
-        if (lane == 0) st_release(p.flags + at, kFlagState);
-    }
-    return carry;
-}
-
-__global__ void __launch_bounds__(kThreads) scan_clear_kernel(unsigned long long *ticket, unsigned *flags, size_t n) {
-    grid_dep_sync();
-    if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
-    for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (size_t)gridDim.x * kThreads) flags[i] = kFlagNone;
-}
-
-// The tile this CTA works on; `slot` is shared memory.
-template <typename T> __device__ __forceinline__ uint64_t take_tile(const ScanArgs<T> &p, unsigned long long *slot) {
-    if (p.chunks == 1) return blockIdx.x;
-    if (threadIdx.x == 0) *slot = atomicAdd(p.ticket, 1ull);
-    __syncthreads();
-    return *slot;
-}
-
 enum Mode { kForward = 0, kBackDense = 1, kBackCodes = 2 };
 
-// A kept state, from the dense tensor or from its 8-bit checkpoint.
-template <typename T, int V, int MODE> __device__ __forceinline__ Pack<T, V> kept(const ScanArgs<T> &p, int64_t flat) {
-    if constexpr (MODE == kBackDense) return ld<T, V>(p.h + flat);
-    Pack<T, V> v;
-    if constexpr (MODE == kBackCodes) {
-        const Pack<int8_t, V> c = ld<int8_t, V>(p.codes + flat);
-        const Ckpt8Scale<T> scale(p.mags[flat >> kCkpt8Shift]);   // V divides the block: one magnitude
-#pragma unroll
-        for (int j = 0; j < V; ++j) v.e[j] = scale.restore(c.e[j]);
-    }
-    return v;
+// V neighbouring codes, as bytes of one word
+template <int V> __device__ __forceinline__ uint32_t codes_at(const int8_t *p) {
+    if constexpr (V == 4) return *reinterpret_cast<const uint32_t *>(p);
+    else if constexpr (V == 2) return *reinterpret_cast<const uint16_t *>(p);
+    else return (uint8_t)*p;
 }
 
-// ---- lanes contiguous in memory: a warp covers 32 * V lanes and R steps of the axis, a CTA kWarps * R steps ---------
+// ---- lanes contiguous in memory ----------------------------------------------------------------------------
+// A thread holds V lanes and R steps; LX threads side by side make a group of LX V lanes, the 32 / LX such rows of a warp, the warps
+// of a CTA and the CTAs of a cluster take consecutive parts of a round.
 // GVEC: the gate's lanes are contiguous too; otherwise the V lanes of a thread share one gate value (V = 1: any stride).
-template <typename T, int V, int R, int MODE, bool COUPLED, bool GVEC>
-__global__ void __launch_bounds__(kThreads) scan_lanes_kernel(const __grid_constant__ ScanArgs<T> p) {
-    constexpr int W = 32 * V;
-    __shared__ alignas(16) T sA[kWarps][W], sH[kWarps][W];
-    __shared__ alignas(16) T sC[W];
-    __shared__ unsigned long long slot;
+template <typename T, int V, int R, int MODE, bool COUPLED, bool GVEC> struct LanesRing {
+    static constexpr bool kBack = MODE != kForward;
+    static constexpr int kGateRows = kBack && COUPLED ? R + 1 : R;   // the coupled epilogue wants the gate of the step itself too
+    static constexpr int kVecBytes = sizeof(T) * V;
+    // whole vectors go through the ring; a shared gate, codes and magnitudes are narrow and wait in registers instead
+    static constexpr int kGate = 0;
+    static constexpr int kB = kGate + (GVEC ? kThreads * kGateRows * kVecBytes : 0);
+    static constexpr int kH = kB + kThreads * R * kVecBytes;
+    static constexpr int kX = kH + (MODE == kBackDense ? kThreads * R * kVecBytes : 0);
+    static constexpr int kStageBytes = kX + (kBack && COUPLED ? kThreads * R * kVecBytes : 0);
+};
+
+template <typename T, int V, int LX, int R, int STAGES, int MODE, bool COUPLED, bool GVEC>
+__global__ void __launch_bounds__(kThreads, 2) scan_lanes_kernel(const __grid_constant__ ScanArgs<T> p) {
+    using Ring = LanesRing<T, V, R, MODE, COUPLED, GVEC>;
     using P = Pack<T, V>;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    grid_dep_sync();
-    const uint64_t tile = take_tile(p, &slot);
-    const uint64_t chunk = p.chunks == 1 ? 0 : tile / p.groups, group = p.chunks == 1 ? tile : tile - chunk * p.groups;
+    constexpr int VA = GVEC ? V : 1;   // a shared gate makes one product of gates for the thread's V lanes
+    using PA = Pack<T, VA>;
+    constexpr int W = LX * V, WA = LX * VA, kRows = 32 / LX;
+    constexpr bool kBack = Ring::kBack;
+    extern __shared__ __align__(16) unsigned char ring[];
+    __shared__ alignas(16) T warp_a[2][kWarps][WA], warp_h[2][kWarps][W];
+    const int lane = threadIdx.x % LX, row = threadIdx.x % 32 / LX, warp = threadIdx.x >> 5;
+    const unsigned nc = p.cluster, rank = nc > 1 ? cluster_rank() : 0;
+    T *const cta_maps = (T *)(ring + STAGES * Ring::kStageBytes);   // [2][nc][map WA, state W], in clusters only
+    __shared__ unsigned long long arrived[2];                       // by buffer: the maps of all CTAs are here
+    const uint64_t group = blockIdx.x / nc;
     const uint64_t first_lane = group * W + (uint64_t)lane * V;
     const bool active = first_lane < p.lanes;
-    const LaneAt at = locate(p.dims, active ? first_lane : 0);
-    const int64_t s0 = (int64_t)(chunk * kWarps + warp) * R;
-    const int64_t steps = (int64_t)p.steps;
+    const LaneAt at = locate(p.dims, active ? first_lane : 0, p.seg_shift);
+    const int64_t steps = (int64_t)p.steps, round = (int64_t)nc * kWarps * kRows * R;
+    const int64_t my0 = (int64_t)((rank * kWarps + warp) * kRows + row) * R;
+    const int64_t rounds = (steps + round - 1) / round;
+    const bool need_h = kBack && p.dg;
+    grid_dep_wait();
 
-    auto gate_at = [&](int64_t s) {
-        P v;
-        if constexpr (GVEC) return ld<T, V>(p.g + at.g + s * p.tg);
-        const T one = p.g[at.g + s * p.tg];
+    auto slot = [&](int64_t i, int part, int row, int bytes) { return ring + (i % STAGES) * Ring::kStageBytes + part + (row * kThreads + (int)threadIdx.x) * bytes; };
+    auto issue = [&](int64_t i) {
+        const int64_t s0 = i * round + my0;
+        if (active && s0 < steps) {
+            // backward: gates one step earlier in processing order; row k of the ring is step s0 - 1 + k
+            if constexpr (GVEC) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v.e[j] = one;
-        return v;
-    };
-    P a[R], b[R], hp[MODE == kForward ? 1 : R], x[MODE != kForward && COUPLED ? R : 1], alast;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int64_t s = s0 + r;
-#pragma unroll
-        for (int j = 0; j < V; ++j) a[r].e[j] = (T)1, b[r].e[j] = (T)0;
-        if (active && s < steps) {
-            if constexpr (MODE == kForward) {
-                a[r] = gate_at(s);
-            } else if (s > 0) {
-                a[r] = gate_at(s - 1);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) a[r].e[j] = (T)0;
+                for (int k = 0; k < Ring::kGateRows; ++k) {
+                    const int64_t s = s0 + k - (kBack ? 1 : 0);
+                    if (s >= 0 && s < steps) copy_async<Ring::kVecBytes>(slot(i, Ring::kGate, k, Ring::kVecBytes), p.g + at.g + s * p.tg);
+                }
             }
-            b[r] = ld<T, V>(p.b + at.b + s * p.tb);
-        }
-    }
-    if constexpr (MODE != kForward) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) alast.e[j] = (T)0;
-        if (active) {
-            if (s0 + R - 1 < steps && (COUPLED || (p.dh0 && s0 + R == steps))) alast = gate_at(s0 + R - 1);
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const int64_t s = s0 + r;
-                if (s >= steps) continue;
-                if (p.dg) {
-                    if (s + 1 < steps) {
-                        hp[r] = kept<T, V, MODE>(p, p.o0 + at.o + (s + 1) * p.to);
-                    } else {
+                if (s >= steps) break;
+                copy_async<Ring::kVecBytes>(slot(i, Ring::kB, r, Ring::kVecBytes), p.b + at.b + s * p.tb);
+                if constexpr (kBack) {
+                    if constexpr (MODE == kBackDense)
+                        if (need_h && s + 1 < steps) copy_async<Ring::kVecBytes>(slot(i, Ring::kH, r, Ring::kVecBytes), p.h + p.o0 + at.o + (s + 1) * p.to);
+                    if constexpr (COUPLED)
+                        if (need_h) copy_async<Ring::kVecBytes>(slot(i, Ring::kX, r, Ring::kVecBytes), p.x + at.x + s * p.tx);
+                }
+            }
+        }
+        copy_commit();
+    };
+    // the narrow operands of a round, loaded while the one before it is worked on
+    T gate_now[GVEC ? 1 : Ring::kGateRows] = {}, gate_next[GVEC ? 1 : Ring::kGateRows];
+    uint32_t code_now[MODE == kBackCodes ? R : 1] = {}, code_next[MODE == kBackCodes ? R : 1];
+    T mag_now[MODE == kBackCodes ? R : 1] = {}, mag_next[MODE == kBackCodes ? R : 1];
+    auto fetch = [&](int64_t i) {
+        const int64_t s0 = i * round + my0;
+        if constexpr (!GVEC) {
 #pragma unroll
-                        for (int j = 0; j < V; ++j) hp[r].e[j] = p.h0 ? p.h0[first_lane + j] : (T)0;
+            for (int k = 0; k < Ring::kGateRows; ++k) {
+                const int64_t s = s0 + k - (kBack ? 1 : 0);
+                gate_next[k] = active && s >= 0 && s < steps ? p.g[at.g + s * p.tg] : (T)1;
+            }
+        }
+        if constexpr (MODE == kBackCodes) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int64_t s = s0 + r;
+                code_next[r] = 0, mag_next[r] = (T)0;
+                if (need_h && active && s + 1 < steps) {
+                    const int64_t flat = p.o0 + at.o + (s + 1) * p.to;
+                    code_next[r] = codes_at<V>(p.codes + flat);
+                    mag_next[r] = p.mags[flat >> kCkpt8Shift];   // V divides the block: one magnitude
+                }
+            }
+        }
+    };
+    auto gate_of = [&](int64_t i, int k) {
+        if constexpr (GVEC) return ld<T, VA>((const T *)slot(i, Ring::kGate, k, Ring::kVecBytes));
+        else return PA{{gate_now[k]}};
+    };
+    auto of = [](const PA &v, int j) { return v.e[GVEC ? j : 0]; };
+
+    P carry;   // the state in front of the round
+#pragma unroll
+    for (int j = 0; j < V; ++j) carry.e[j] = !kBack && p.h0 && active ? p.h0[first_lane + j] : (T)0;
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(i);
+    fetch(0);
+    if (nc > 1) {
+        if (threadIdx.x == 0) mbar_init(&arrived[0]), mbar_init(&arrived[1]);
+        cluster_barrier();   // every CTA runs, its barriers are set, before any is written to
+    }
+    bool lost = false;
+
+    for (int64_t i = 0; i < rounds; ++i) {
+        issue(i + STAGES - 1);
+        if constexpr (!GVEC) {
+#pragma unroll
+            for (int k = 0; k < Ring::kGateRows; ++k) gate_now[k] = gate_next[k];
+        }
+        if constexpr (MODE == kBackCodes) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) code_now[r] = code_next[r], mag_now[r] = mag_next[r];
+        }
+        if constexpr (!GVEC || MODE == kBackCodes) fetch(i + 1);
+        copy_wait<STAGES - 1>();
+        const int64_t s0 = i * round + my0;
+        PA a[R];
+        P b[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t s = s0 + r;
+            if (active && s < steps) {
+                if (kBack && s == 0) {
+#pragma unroll
+                    for (int j = 0; j < VA; ++j) a[r].e[j] = (T)0;
+                } else {
+                    a[r] = gate_of(i, r);
+                }
+                b[r] = ld<T, V>((const T *)slot(i, Ring::kB, r, Ring::kVecBytes));
+                if constexpr (!kBack && COUPLED) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) b[r].e[j] = ((T)1 - of(a[r], j)) * b[r].e[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < VA; ++j) a[r].e[j] = (T)1;
+#pragma unroll
+                for (int j = 0; j < V; ++j) b[r].e[j] = (T)0;
+            }
+        }
+        // the thread's map over its R steps
+        PA A = a[0];
+        P H = b[0];
+#pragma unroll
+        for (int r = 1; r < R; ++r) {
+#pragma unroll
+            for (int j = 0; j < VA; ++j) A.e[j] = a[r].e[j] * A.e[j];
+#pragma unroll
+            for (int j = 0; j < V; ++j) H.e[j] = fma_(of(a[r], j), H.e[j], b[r].e[j]);
+        }
+        // the rows in front of the thread's own in its warp
+        PA ex_a;
+        P ex_h;
+        if constexpr (kRows > 1) {
+#pragma unroll
+            for (int d = 1; d < kRows; d <<= 1) {
+                PA pa;
+                P ph;
+#pragma unroll
+                for (int j = 0; j < VA; ++j) pa.e[j] = __shfl_up_sync(0xffffffffu, A.e[j], d * LX);
+#pragma unroll
+                for (int j = 0; j < V; ++j) ph.e[j] = __shfl_up_sync(0xffffffffu, H.e[j], d * LX);
+                if (row >= d) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) H.e[j] = fma_(of(A, j), ph.e[j], H.e[j]);
+#pragma unroll
+                    for (int j = 0; j < VA; ++j) A.e[j] = A.e[j] * pa.e[j];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < VA; ++j) {
+                ex_a.e[j] = __shfl_up_sync(0xffffffffu, A.e[j], LX);
+                if (row == 0) ex_a.e[j] = (T)1;
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                ex_h.e[j] = __shfl_up_sync(0xffffffffu, H.e[j], LX);
+                if (row == 0) ex_h.e[j] = (T)0;
+            }
+        }
+        const int buf = (int)(i & 1);   // a warp is never a whole round ahead of another: two buffers suffice
+        if (row == kRows - 1) {
+            st<T, VA>(&warp_a[buf][warp][lane * VA], A);
+            st<T, V>(&warp_h[buf][warp][lane * V], H);
+        }
+        __syncthreads();
+        P c = carry;
+        if (nc > 1) {
+            if (warp == 0 && row == 0) {
+                A = ld<T, VA>(&warp_a[buf][0][lane * VA]), H = ld<T, V>(&warp_h[buf][0][lane * V]);
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) {
+                    const PA wa = ld<T, VA>(&warp_a[buf][w][lane * VA]);
+                    const P wh = ld<T, V>(&warp_h[buf][w][lane * V]);
+#pragma unroll
+                    for (int j = 0; j < VA; ++j) A.e[j] = wa.e[j] * A.e[j];
+#pragma unroll
+                    for (int j = 0; j < V; ++j) H.e[j] = fma_(of(wa, j), H.e[j], wh.e[j]);
+                }
+                if (lane == 0) mbar_expect(&arrived[buf], nc * (WA + W) * sizeof(T));
+                const unsigned to = smem_addr(cta_maps + (buf * nc + rank) * (WA + W)), bar = smem_addr(&arrived[buf]);
+                for (unsigned q = 0; q < nc; ++q) {
+                    send(in_cta(to + lane * VA * sizeof(T), q), A, in_cta(bar, q));
+                    send(in_cta(to + (WA + lane * V) * sizeof(T), q), H, in_cta(bar, q));
+                }
+            }
+            // a CTA sends the maps of round i + 2 only after it has those of round i + 1 from all, who then have read round i's
+            if (!lost && !mbar_wait(&arrived[buf], (unsigned)(i >> 1) & 1u)) lost = true;
+            if (lost) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) carry.e[j] = nan_of(T());
+            }
+            for (unsigned q = 0; q < nc; ++q) {
+                if (q == rank) c = carry;
+                const T *from = cta_maps + (buf * nc + q) * (WA + W);
+                const PA qa = ld<T, VA>(from + lane * VA);
+                const P qh = ld<T, V>(from + WA + lane * V);
+#pragma unroll
+                for (int j = 0; j < V; ++j) carry.e[j] = fma_(of(qa, j), carry.e[j], qh.e[j]);
+            }
+        }
+        P mine = c;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w == warp) mine = c;
+            if (nc > 1 && w >= warp) break;   // a single CTA folds all of them: that is the next round's carry
+            const PA wa = ld<T, VA>(&warp_a[buf][w][lane * VA]);
+            const P wh = ld<T, V>(&warp_h[buf][w][lane * V]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) c.e[j] = fma_(of(wa, j), c.e[j], wh.e[j]);
+        }
+        if (nc == 1) carry = c;
+        else mine = c;
+        c = mine;
+        if constexpr (kRows > 1) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) c.e[j] = fma_(of(ex_a, j), c.e[j], ex_h.e[j]);
+        }
+        // the states (or the gradients that reach them) take b's place
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) b[r].e[j] = c.e[j] = fma_(of(a[r], j), c.e[j], b[r].e[j]);
+            const int64_t s = s0 + r;
+            if (!active || s >= steps) continue;
+            const int64_t o = p.o0 + at.o + s * p.to;
+            if constexpr (!kBack) {
+                st<T, V>(p.out + o, c);
+            } else {
+                if (p.out) {
+                    P d = c;
+                    if constexpr (COUPLED) {
+                        const PA now = gate_of(i, r + 1);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) d.e[j] = ((T)1 - of(now, j)) * c.e[j];
                     }
-                    if constexpr (COUPLED) x[r] = ld<T, V>(p.x + at.x + s * p.tx);
+                    st<T, V>(p.out + o, d);
+                }
+                if (p.dh0 && s + 1 == steps) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) p.dh0[first_lane + j] = p.g[at.g + j * (GVEC ? 1 : 0) + s * p.tg] * c.e[j];
+                }
+            }
+        }
+        if constexpr (kBack) {
+            if (need_h) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const int64_t s = s0 + r;
+                    P d;
+                    if (active && s + 1 == steps) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) d.e[j] = p.h0 ? p.h0[first_lane + j] : (T)0;
+                    } else if constexpr (MODE == kBackDense) {
+                        d = ld<T, V>((const T *)slot(i, Ring::kH, r, Ring::kVecBytes));
+                    } else {
+                        const Ckpt8Scale<T> scale(mag_now[r]);
+#pragma unroll
+                        for (int j = 0; j < V; ++j) d.e[j] = scale.restore(code_now[r], j);
+                    }
+                    if constexpr (COUPLED) {
+                        const P x = ld<T, V>((const T *)slot(i, Ring::kX, r, Ring::kVecBytes));
+#pragma unroll
+                        for (int j = 0; j < V; ++j) d.e[j] = d.e[j] - x.e[j];
+                    }
+                    // behind the axis, and in idle threads, the ring holds nothing: what is there must not count
+                    const bool here = active && s < steps;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) b[r].e[j] = here ? b[r].e[j] * d.e[j] : (T)0;
+                }
+                if (p.seg_shift == 0) {
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+                        if (active && s0 + r < steps) st<T, V>(p.dg + p.d0 + at.d + (s0 + r) * p.td, b[r]);
+                } else {
+                    // a segment is a power of two of lanes, at least V, and whole within a row of the group
+                    T sum[R];
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        sum[r] = b[r].e[0];
+#pragma unroll
+                        for (int j = 1; j < V; ++j) sum[r] += b[r].e[j];
+                    }
+#pragma unroll
+                    for (int m = 1; m < LX; m <<= 1)
+                        if (m < (1 << p.seg_shift) / V) {
+#pragma unroll
+                            for (int r = 0; r < R; ++r) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], m);
+                        }
+                    if (active && ((lane * V) & ((1 << p.seg_shift) - 1)) == 0) {
+#pragma unroll
+                        for (int r = 0; r < R; ++r)
+                            if (s0 + r < steps) p.dg[p.d0 + at.d + (s0 + r) * p.td] = sum[r];
+                    }
                 }
             }
         }
     }
-    if constexpr (MODE == kForward && COUPLED) {
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-            for (int j = 0; j < V; ++j) b[r].e[j] = ((T)1 - a[r].e[j]) * b[r].e[j];
-    }
-    // the thread's own map over its R steps
-    P A = a[0], H = b[0];
-#pragma unroll
-    for (int r = 1; r < R; ++r)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            A.e[j] = a[r].e[j] * A.e[j];
-            H.e[j] = fma_(a[r].e[j], H.e[j], b[r].e[j]);
-        }
-    st<T, V>(&sA[warp][lane * V], A);
-    st<T, V>(&sH[warp][lane * V], H);
-    __syncthreads();
-    if (warp == 0) {
-        P first;
-#pragma unroll
-        for (int j = 0; j < V; ++j) first.e[j] = MODE == kForward && p.h0 && active ? p.h0[first_lane + j] : (T)0;
-        if (p.chunks > 1) {
-            for (int w = 1; w < kWarps; ++w) {
-                const P wa = ld<T, V>(&sA[w][lane * V]), wh = ld<T, V>(&sH[w][lane * V]);
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    A.e[j] = wa.e[j] * A.e[j];
-                    H.e[j] = fma_(wa.e[j], H.e[j], wh.e[j]);
-                }
-            }
-            first = chain_carry<T, V>(p, group, chunk, lane, A, H, first);
-        }
-        st<T, V>(&sC[lane * V], first);
-    }
-    __syncthreads();
-    if (!active) return;
-    P c = ld<T, V>(&sC[lane * V]);
-    for (int w = 0; w < warp; ++w) {
-        const P wa = ld<T, V>(&sA[w][lane * V]), wh = ld<T, V>(&sH[w][lane * V]);
-#pragma unroll
-        for (int j = 0; j < V; ++j) c.e[j] = fma_(wa.e[j], c.e[j], wh.e[j]);
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int64_t s = s0 + r;
-        if (s >= steps) break;
-#pragma unroll
-        for (int j = 0; j < V; ++j) c.e[j] = fma_(a[r].e[j], c.e[j], b[r].e[j]);
-        const int64_t o = p.o0 + at.o + s * p.to;
-        if constexpr (MODE == kForward) {
-            st<T, V>(p.out + o, c);
-        } else {
-            const P &now = r + 1 < R ? a[r + 1] : alast;   // the gate of step s
-            if (p.out) {
-                P d = c;
-                if constexpr (COUPLED) {
-                    // behind the last step of the axis a[r + 1] is the padding's 1, so alast's rule is applied here too
-                    const P gate = (r + 1 < R && s + 1 == steps) ? gate_at(s) : now;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) d.e[j] = ((T)1 - gate.e[j]) * c.e[j];
-                }
-                st<T, V>(p.out + o, d);
-            }
-            if (p.dg) {
-                P d;
-#pragma unroll
-                for (int j = 0; j < V; ++j) d.e[j] = c.e[j] * (COUPLED ? hp[r].e[j] - x[COUPLED ? r : 0].e[j] : hp[r].e[j]);
-                st<T, V>(p.dg + o, d);
-            }
-            if (p.dh0 && s + 1 == steps) {
-                const P gate = r + 1 < R ? gate_at(s) : now;
-#pragma unroll
-                for (int j = 0; j < V; ++j) p.dh0[first_lane + j] = gate.e[j] * c.e[j];
-            }
-        }
-    }
+    grid_dep_launch();               // late: CTAs of the next kernel that wait beside a long loop slow it down
+    if (nc > 1) cluster_barrier();   // no CTA leaves while another may still write to it
 }
 
-// ---- the axis itself contiguous: a warp covers runs of 32 * V consecutive steps of one lane -------------------------
-// Within a run thread l holds V consecutive steps; their maps are scanned across the warp by shuffles.
+// ---- the axis itself contiguous ---------------------------------------------------------------------------
+// A warp takes K runs of 32 V consecutive steps of one lane; within a run a thread holds V steps, and the threads' maps
+// are scanned across the warp by shuffles.  TEAM warps share a lane: one walks it alone (many lanes, no barrier at all), or a
+// CTA's eight, and the CTAs of a cluster, take consecutive parts of each round.
 // VEC: all operands have unit stride (either sign) along the axis and 16-byte aligned runs.
 template <typename T> __device__ __forceinline__ T shfl_up(T v, int d) { return __shfl_up_sync(0xffffffffu, v, d); }
 template <typename T> __device__ __forceinline__ T shfl_down1(T v) { return __shfl_down_sync(0xffffffffu, v, 1); }
 template <typename T> __device__ __forceinline__ T shfl_at(T v, int l) { return __shfl_sync(0xffffffffu, v, l); }
 
-template <typename T, int V, int K, int MODE, bool COUPLED, bool VEC> struct RowTile {
-    using P = Pack<T, V>;
-    P a[K], b[K], g[MODE == kForward ? 1 : K], hp[MODE == kForward ? 1 : K], x[MODE != kForward && COUPLED ? K : 1];
-    T exA[K], exH[K];   // map of the steps of this tile in front of the thread's own
-    T A, H;             // map of the whole tile (the same in all threads)
+template <typename T, int V, int K, int MODE, bool COUPLED> struct AxisRing {
+    static constexpr int kRun = 32 * V;                      // steps
+    static constexpr int kTile = K * kRun;                   // steps of a warp in a round
+    static constexpr int kPart = kTile * (int)sizeof(T);     // bytes
+    static constexpr int kGate = 0, kB = kPart, kH = 2 * kPart, kX = kH + (MODE == kBackDense ? kPart : 0);
+    static constexpr int kHalo = kX + (MODE != kForward && COUPLED ? kPart : 0);   // the gate before, the state behind
+    static constexpr int kWarpBytes = kHalo + (MODE != kForward ? 16 : 0);
+    static constexpr int kStageBytes = kWarps * kWarpBytes;
+};
 
-    // V steps from s on of an operand with signed step t
-    static __device__ __forceinline__ P run(const T *base, int64_t s, int64_t t, int64_t steps, T pad) {
-        P v;
-        if (VEC) {   // steps is a multiple of V: whole runs only
-            if (s < steps) {
-                if (t > 0) return ld<T, V>(base + s);
-                const P w = ld<T, V>(base - s - (V - 1));
+template <typename T, int V, int K, int STAGES, int TEAM, int MODE, bool COUPLED, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) scan_axis_kernel(const __grid_constant__ ScanArgs<T> p) {
+    using Ring = AxisRing<T, V, K, MODE, COUPLED>;
+    using P = Pack<T, V>;
+    constexpr bool kBack = MODE != kForward;
+    extern __shared__ __align__(16) unsigned char ring[];
+    __shared__ T warp_a[2][kWarps], warp_h[2][kWarps];
+    __shared__ alignas(16) Pack<T, 2> cta_maps[2][kMaxCluster];
+    __shared__ unsigned long long arrived[2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned nc = TEAM > 1 ? p.cluster : 1, rank = nc > 1 ? cluster_rank() : 0;
+    const uint64_t seq = TEAM > 1 ? blockIdx.x / nc : (uint64_t)blockIdx.x * kWarps + warp;
+    if (TEAM == 1 && seq >= p.lanes) return;
+    const LaneAt at = locate(p.dims, seq, 0);
+    const int64_t steps = (int64_t)p.steps;
+    const int64_t round = (int64_t)nc * TEAM * Ring::kTile, my0 = TEAM > 1 ? (int64_t)(rank * kWarps + warp) * Ring::kTile : 0;
+    const int64_t rounds = (steps + round - 1) / round;
+    const bool need_h = kBack && p.dg;
+    grid_dep_wait();
+
+    auto part = [&](int64_t i, int at_byte) { return (T *)(ring + (i % STAGES) * Ring::kStageBytes + warp * Ring::kWarpBytes + at_byte); };
+    // steps [s0, s0 + kTile) of an operand with signed step t into a part of the ring: whole 16-byte vectors as they lie in
+    // memory, or element by element in processing order
+    auto fill = [&](T *to, const T *from, int64_t s0, int64_t t) {
+        if constexpr (VEC) {
 #pragma unroll
-                for (int j = 0; j < V; ++j) v.e[j] = w.e[V - 1 - j];
-                return v;
+            for (int k = 0; k < K; ++k) {
+                const int64_t s = s0 + (k * 32 + lane) * V;
+                if (s < steps) copy_async<16>(to + (k * 32 + lane) * V, t > 0 ? from + s : from - s - (V - 1));
             }
+        } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) v.e[j] = pad;
-            return v;
+            for (int e = 0; e < K * V; ++e) {
+                const int64_t s = s0 + e * 32 + lane;
+                if (s < steps) copy_async<sizeof(T)>(to + e * 32 + lane, from + s * t);
+            }
         }
+    };
+    // V steps of run k, in processing order
+    auto take = [&](const T *from, int k, int64_t t, int64_t s, T pad) {
+        P v = ld<T, V>(from + (k * 32 + lane) * V);
+        if (VEC && t < 0) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v.e[j] = s + j < steps ? base[(s + j) * t] : pad;
-        return v;
-    }
-    static __device__ __forceinline__ void put(T *base, int64_t s, int64_t t, int64_t steps, const P &v) {
-        if (VEC) {
-            if (s >= steps) return;
-            if (t > 0) {
-                st<T, V>(base + s, v);
-                return;
+            for (int j = 0; j < V / 2; ++j) {
+                const T w = v.e[j];
+                v.e[j] = v.e[V - 1 - j], v.e[V - 1 - j] = w;
             }
-            P w;
-#pragma unroll
-            for (int j = 0; j < V; ++j) w.e[j] = v.e[V - 1 - j];
-            st<T, V>(base - s - (V - 1), w);
-            return;
         }
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (s + j < steps) base[(s + j) * t] = v.e[j];
-    }
-
-    __device__ __forceinline__ void load(const ScanArgs<T> &p, const LaneAt &at, uint64_t lane_no, int64_t s0, int lane) {
-        const int64_t steps = (int64_t)p.steps;
+            if (s + j >= steps) v.e[j] = pad;
+        return v;
+    };
+    auto put = [&](T *to, int64_t s, int64_t t, const P &v) {
+        if constexpr (VEC) {
+            if (s >= steps) return;
+            P w = v;
+            if (t < 0) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int64_t s = s0 + (int64_t)(k * 32 + lane) * V;
-            const P gv = run(p.g + at.g, s, p.tg, steps, (T)1);
-            b[k] = run(p.b + at.b, s, p.tb, steps, (T)0);
-            if constexpr (MODE == kForward) {
-                a[k] = gv;
-            } else {
-                g[k] = gv;
-                T before = shfl_up(gv.e[V - 1], 1);   // the gate of the step in front of the run
-                if (lane == 0) before = s > 0 && s - 1 < steps ? p.g[at.g + (s - 1) * p.tg] : (T)0;
-                a[k].e[0] = before;
+                for (int j = 0; j < V; ++j) w.e[j] = v.e[V - 1 - j];
+            }
+            st<T, V>(t > 0 ? to + s : to - s - (V - 1), w);
+        } else {
 #pragma unroll
-                for (int j = 1; j < V; ++j) a[k].e[j] = gv.e[j - 1];
+            for (int j = 0; j < V; ++j)
+                if (s + j < steps) to[(s + j) * t] = v.e[j];
+        }
+    };
+    auto code_of = [&](int64_t s) {
+        const int64_t flat = p.o0 + at.o + s * p.to;
+        return Ckpt8Scale<T>(p.mags[flat >> kCkpt8Shift]).restore(p.codes[flat]);
+    };
+    // V kept states from step s on, out of their codes
+    auto codes_run = [&](int64_t s) {
+        P v;
 #pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (s + j >= steps) a[k].e[j] = (T)1;
-                if (p.dg) {
+        for (int j = 0; j < V; ++j) v.e[j] = (T)0;
+        if constexpr (VEC) {
+            if (s < steps) {
+                const int64_t flat = p.o0 + at.o + (p.to > 0 ? s : -s - (V - 1));   // V aligned codes: one magnitude
+                const uint32_t c = codes_at<V>(p.codes + flat);
+                const Ckpt8Scale<T> scale(p.mags[flat >> kCkpt8Shift]);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) {
-                        const int64_t next = s + j + 1;
-                        hp[k].e[j] = (T)0;
-                        if (next < steps) hp[k].e[j] = kept<T, 1, MODE>(p, p.o0 + at.o + next * p.to).e[0];
-                        else if (next == steps && p.h0) hp[k].e[j] = p.h0[lane_no];
+                for (int j = 0; j < V; ++j) v.e[j] = scale.restore(c, p.to > 0 ? j : V - 1 - j);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (s + j < steps) v.e[j] = code_of(s + j);
+        }
+        return v;
+    };
+    auto issue = [&](int64_t i) {
+        const int64_t s0 = i * round + my0;
+        if (s0 < steps) {
+            fill(part(i, Ring::kGate), p.g + at.g, s0, p.tg);
+            fill(part(i, Ring::kB), p.b + at.b, s0, p.tb);
+            if constexpr (kBack) {
+                if (lane == 0 && s0 > 0) copy_async<sizeof(T)>(part(i, Ring::kHalo), p.g + at.g + (s0 - 1) * p.tg);
+                if (need_h) {
+                    if constexpr (MODE == kBackDense) {
+                        fill(part(i, Ring::kH), p.h + p.o0 + at.o, s0, p.to);
+                        if (lane == 0 && s0 + Ring::kTile < steps)
+                            copy_async<sizeof(T)>(part(i, Ring::kHalo) + 1, p.h + p.o0 + at.o + (s0 + Ring::kTile) * p.to);
                     }
-                    if constexpr (COUPLED) x[k] = run(p.x + at.x, s, p.tx, steps, (T)0);
+                    if constexpr (COUPLED) fill(part(i, Ring::kX), p.x + at.x, s0, p.tx);
                 }
             }
         }
+        copy_commit();
+    };
+
+    T carry = !kBack && p.h0 ? p.h0[seq] : (T)0;
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(i);
+    if (nc > 1) {
+        if (threadIdx.x == 0) mbar_init(&arrived[0]), mbar_init(&arrived[1]);
+        cluster_barrier();   // every CTA runs, its barriers are set, before any is written to
     }
-    __device__ __forceinline__ void compose(int lane) {
-        A = (T)1, H = (T)0;
+    bool lost = false;
+
+    for (int64_t i = 0; i < rounds; ++i) {
+        __syncwarp();                // the stage that is filled next has been read by all lanes
+        issue(i + STAGES - 1);
+        copy_wait<STAGES - 1>();
+        __syncwarp();                // a lane reads what others copied
+        const int64_t s0 = i * round + my0;
+        P a[K], b[K], g[kBack ? K : 1], hp[kBack ? K : 1];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            if constexpr (MODE == kForward && COUPLED) {
+            const int64_t s = s0 + (k * 32 + lane) * V;
+            a[k] = take(part(i, Ring::kGate), k, p.tg, s, (T)1);
+            b[k] = take(part(i, Ring::kB), k, p.tb, s, (T)0);
+            if constexpr (!kBack && COUPLED) {
 #pragma unroll
                 for (int j = 0; j < V; ++j) b[k].e[j] = ((T)1 - a[k].e[j]) * b[k].e[j];
             }
+        }
+        if constexpr (kBack) {
+            // the gates move one step back, the states one ahead
+            T edge = s0 > 0 ? *part(i, Ring::kHalo) : (T)0;
+            T behind = (T)0;
+            if (need_h && s0 + Ring::kTile < steps) {
+                if constexpr (MODE == kBackDense) behind = part(i, Ring::kHalo)[1];
+                else behind = code_of(s0 + Ring::kTile);
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int64_t s = s0 + (k * 32 + lane) * V;
+                g[k] = a[k];
+                T before = shfl_up(g[k].e[V - 1], 1);
+                if (lane == 0) before = edge;
+                edge = shfl_at(g[k].e[V - 1], 31);
+#pragma unroll
+                for (int j = V - 1; j > 0; --j) a[k].e[j] = s + j < steps ? g[k].e[j - 1] : (T)1;
+                a[k].e[0] = s < steps ? before : (T)1;
+                if (need_h) {
+                    if constexpr (MODE == kBackDense) hp[k] = take(part(i, Ring::kH), k, p.to, s, (T)0);
+                    else hp[k] = codes_run(s);
+                }
+            }
+            if (need_h) {
+#pragma unroll
+                for (int k = K - 1; k >= 0; --k) {
+                    T after = shfl_down1(hp[k].e[0]);
+                    if (lane == 31) after = behind;
+                    behind = shfl_at(hp[k].e[0], 0);
+#pragma unroll
+                    for (int j = 0; j + 1 < V; ++j) hp[k].e[j] = hp[k].e[j + 1];
+                    hp[k].e[V - 1] = after;
+                }
+                if (p.h0) {
+#pragma unroll
+                    for (int k = 0; k < K; ++k)
+#pragma unroll
+                        for (int j = 0; j < V; ++j)
+                            if (s0 + (k * 32 + lane) * V + j + 1 == steps) hp[k].e[j] = p.h0[seq];
+                }
+            }
+        }
+        // maps: of the steps in front of the thread's own in its warp, and of the warp's whole part
+        T ex_a[K], ex_h[K], A = (T)1, H = (T)0;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
             T la = a[k].e[0], lh = b[k].e[0];
 #pragma unroll
             for (int j = 1; j < V; ++j) {
@@ -479,27 +725,59 @@ template <typename T, int V, int K, int MODE, bool COUPLED, bool VEC> struct Row
             }
             T ea = shfl_up(la, 1), eh = shfl_up(lh, 1);
             if (lane == 0) ea = (T)1, eh = (T)0;
-            exA[k] = ea * A;
-            exH[k] = fma_(ea, H, eh);
+            ex_a[k] = ea * A;
+            ex_h[k] = fma_(ea, H, eh);
             const T ta = shfl_at(la, 31), th = shfl_at(lh, 31);
             H = fma_(ta, H, th);
             A = ta * A;
         }
-    }
-    __device__ __forceinline__ void finish(const ScanArgs<T> &p, const LaneAt &at, uint64_t lane_no, int64_t s0, int lane, T carry) {
-        const int64_t steps = (int64_t)p.steps;
+        T c = carry;
+        if constexpr (TEAM > 1) {
+            const int buf = (int)(i & 1);
+            if (lane == 0) warp_a[buf][warp] = A, warp_h[buf][warp] = H;
+            __syncthreads();
+            if (nc > 1) {
+                if (warp == 0 && lane < (int)nc) {
+                    T ca = warp_a[buf][0], ch = warp_h[buf][0];
+#pragma unroll
+                    for (int w = 1; w < kWarps; ++w) {
+                        ca = warp_a[buf][w] * ca;
+                        ch = fma_(warp_a[buf][w], ch, warp_h[buf][w]);
+                    }
+                    if (lane == 0) mbar_expect(&arrived[buf], nc * 2 * sizeof(T));
+                    send(in_cta(smem_addr(&cta_maps[buf][rank]), lane), Pack<T, 2>{{ca, ch}}, in_cta(smem_addr(&arrived[buf]), lane));
+                }
+                // a CTA sends the maps of round i + 2 only after it has those of round i + 1 from all, who then have read round i's
+                if (!lost && !mbar_wait(&arrived[buf], (unsigned)(i >> 1) & 1u)) lost = true;
+                if (lost) carry = nan_of(T());
+                for (unsigned q = 0; q < nc; ++q) {
+                    if (q == rank) c = carry;
+                    carry = fma_(cta_maps[buf][q].e[0], carry, cta_maps[buf][q].e[1]);
+                }
+            }
+            T mine = c;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                if (w == warp) mine = c;
+                c = fma_(warp_a[buf][w], c, warp_h[buf][w]);
+            }
+            if (nc == 1) carry = c;
+            c = mine;
+        } else {
+            carry = fma_(A, carry, H);
+        }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int64_t s = s0 + (int64_t)(k * 32 + lane) * V;
-            T c = fma_(exA[k], carry, exH[k]);
+            const int64_t s = s0 + (k * 32 + lane) * V;
+            T v = fma_(ex_a[k], c, ex_h[k]);
             P h;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                c = fma_(a[k].e[j], c, b[k].e[j]);
-                h.e[j] = c;
+                v = fma_(a[k].e[j], v, b[k].e[j]);
+                h.e[j] = v;
             }
-            if constexpr (MODE == kForward) {
-                put(p.out + p.o0 + at.o, s, p.to, steps, h);
+            if constexpr (!kBack) {
+                put(p.out + p.o0 + at.o, s, p.to, h);
             } else {
                 if (p.out) {
                     P d = h;
@@ -507,73 +785,29 @@ template <typename T, int V, int K, int MODE, bool COUPLED, bool VEC> struct Row
 #pragma unroll
                         for (int j = 0; j < V; ++j) d.e[j] = ((T)1 - g[k].e[j]) * h.e[j];
                     }
-                    put(p.out + p.o0 + at.o, s, p.to, steps, d);
+                    put(p.out + p.o0 + at.o, s, p.to, d);
                 }
-                if (p.dg) {
-                    P d;
+                if (need_h) {
+                    P d = hp[k];
+                    if constexpr (COUPLED) {
+                        const P x = take(part(i, Ring::kX), k, p.tx, s, (T)0);
 #pragma unroll
-                    for (int j = 0; j < V; ++j) d.e[j] = h.e[j] * (COUPLED ? hp[k].e[j] - x[COUPLED ? k : 0].e[j] : hp[k].e[j]);
-                    put(p.dg + p.o0 + at.o, s, p.to, steps, d);
+                        for (int j = 0; j < V; ++j) d.e[j] = d.e[j] - x.e[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < V; ++j) d.e[j] = h.e[j] * d.e[j];
+                    put(p.dg + p.d0 + at.d, s, p.td, d);
                 }
                 if (p.dh0) {
 #pragma unroll
                     for (int j = 0; j < V; ++j)
-                        if (s + j + 1 == steps) p.dh0[lane_no] = g[k].e[j] * h.e[j];
+                        if (s + j + 1 == steps) p.dh0[seq] = g[k].e[j] * h.e[j];
                 }
             }
         }
     }
-};
-
-// One CTA per (lane, chunk of kWarps * K * 32 * V steps); chunks of a lane form a chain of width 32 (thread 0's slot counts).
-template <typename T, int V, int K, int MODE, bool COUPLED, bool VEC>
-__global__ void __launch_bounds__(kThreads) scan_axis_kernel(const __grid_constant__ ScanArgs<T> p) {
-    __shared__ T sA[kWarps], sH[kWarps], sC;
-    __shared__ unsigned long long slot;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    grid_dep_sync();
-    const uint64_t tile = take_tile(p, &slot);
-    const uint64_t chunk = p.chunks == 1 ? 0 : tile / p.groups, seq = p.chunks == 1 ? tile : tile - chunk * p.groups;
-    const LaneAt at = locate(p.dims, seq);
-    const int64_t s0 = (int64_t)(chunk * kWarps + warp) * (K * 32 * V);
-    RowTile<T, V, K, MODE, COUPLED, VEC> t;
-    t.load(p, at, seq, s0, lane);
-    t.compose(lane);
-    if (lane == 0) sA[warp] = t.A, sH[warp] = t.H;
-    __syncthreads();
-    if (warp == 0) {
-        Pack<T, 1> A{{t.A}}, H{{t.H}}, first{{MODE == kForward && p.h0 ? p.h0[seq] : (T)0}};
-        if (p.chunks > 1) {
-            for (int w = 1; w < kWarps; ++w) {
-                A.e[0] = sA[w] * A.e[0];
-                H.e[0] = fma_(sA[w], H.e[0], sH[w]);
-            }
-            first = chain_carry<T, 1>(p, seq, chunk, lane, A, H, first);
-        }
-        if (lane == 0) sC = first.e[0];
-    }
-    __syncthreads();
-    T c = sC;
-    for (int w = 0; w < warp; ++w) c = fma_(sA[w], c, sH[w]);
-    t.finish(p, at, seq, s0, lane, c);
-}
-
-// Many lanes: one warp walks its lane from end to end, the carry stays in a register.
-template <typename T, int V, int K, int MODE, bool COUPLED, bool VEC>
-__global__ void __launch_bounds__(kThreads) scan_axis_warp_kernel(const __grid_constant__ ScanArgs<T> p) {
-    const int lane = threadIdx.x & 31;
-    grid_dep_sync();
-    const uint64_t seq = (uint64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-    if (seq >= p.lanes) return;
-    const LaneAt at = locate(p.dims, seq);
-    T carry = MODE == kForward && p.h0 ? p.h0[seq] : (T)0;
-    for (int64_t s0 = 0; s0 < (int64_t)p.steps; s0 += K * 32 * V) {
-        RowTile<T, V, K, MODE, COUPLED, VEC> t;
-        t.load(p, at, seq, s0, lane);
-        t.compose(lane);
-        t.finish(p, at, seq, s0, lane, carry);
-        carry = fma_(t.A, carry, t.H);
-    }
+    grid_dep_launch();               // late, as above
+    if (nc > 1) cluster_barrier();   // no CTA leaves while another may still write to it
 }
 
 // ---- one step in place: state = a state + b over any view ------------------------------------------------
@@ -582,7 +816,7 @@ __global__ void __launch_bounds__(kThreads) step_kernel(LaneDims dims, uint64_t 
     grid_dep_sync();
     const uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) * V;
     if (i >= lanes) return;
-    const LaneAt at = locate(dims, i);
+    const LaneAt at = locate(dims, i, 0);
     Pack<T, V> h = ld<T, V>(state + at.o), a, b = ld<T, V>(x + at.b);
     if constexpr (GVEC) {
         a = ld<T, V>(g + at.g);
@@ -596,36 +830,43 @@ __global__ void __launch_bounds__(kThreads) step_kernel(LaneDims dims, uint64_t 
     st<T, V>(state + at.o, h);
 }
 
+// dst[i] = sum of the k neighbours src[i k ..): what is left of a gate's gradient after the segments
+template <typename T> __global__ void __launch_bounds__(kThreads) neighbour_sum_kernel(const T *src, uint64_t n, unsigned k, T *dst) {
+    grid_dep_sync();
+    const uint64_t i = (uint64_t)blockIdx.x * kThreads + threadIdx.x;
+    if (i >= n) return;
+    T sum = src[i * k];
+    for (unsigned j = 1; j < k; ++j) sum += src[i * k + j];
+    dst[i] = sum;
+}
+
 // ---- host ------------------------------------------------------------------------------------------------
-// Merges the dims of `shape` other than `axis` (axis >= rank: all of them).  -> false when more than kMaxLaneDims remain.
-bool lane_dims(size_t rank, const size_t *shape, size_t axis, const ptrdiff_t *so, const ptrdiff_t *sg, const ptrdiff_t *sb,
-               const ptrdiff_t *sx, LaneDims *out) {
-    out->nd = 0;
+// Merges the dims of `shape` other than `axis` (axis >= rank: all of them) as far as the strides (null: unused) of out, gate,
+// b, x and dg allow.  -> false when more than kMaxLaneDims remain.
+bool lane_dims(size_t rank, const size_t *shape, size_t axis, const ptrdiff_t *const in[5], LaneDims *out) {
     std::vector<uint64_t> n;
-    std::vector<int64_t> s[4];
-    const ptrdiff_t *in[4] = {so, sg, sb, sx};
+    std::vector<int64_t> s[5];
     for (size_t k = 0; k < rank; ++k) {
         if (k == axis || shape[k] == 1) continue;
         bool merge = !n.empty();
-        for (int q = 0; q < 4 && merge; ++q)
+        for (int q = 0; q < 5 && merge; ++q)
             if (in[q] && s[q].back() != (int64_t)in[q][k] * (int64_t)shape[k]) merge = false;
-        if (merge) {
-            n.back() *= shape[k];
-            for (int q = 0; q < 4; ++q) s[q].back() = in[q] ? (int64_t)in[q][k] : 0;
-        } else {
-            n.push_back(shape[k]);
-            for (int q = 0; q < 4; ++q) s[q].push_back(in[q] ? (int64_t)in[q][k] : 0);
+        if (!merge) {
+            n.push_back(1);
+            for (int q = 0; q < 5; ++q) s[q].push_back(0);
         }
+        n.back() *= shape[k];
+        for (int q = 0; q < 5; ++q) s[q].back() = in[q] ? (int64_t)in[q][k] : 0;
     }
     if (n.empty()) {
         n.push_back(1);
-        for (int q = 0; q < 4; ++q) s[q].push_back(0);
+        for (int q = 0; q < 5; ++q) s[q].push_back(0);
     }
     if (n.size() > (size_t)kMaxLaneDims) return false;
     out->nd = (int)n.size();
     for (int k = 0; k < out->nd; ++k) {
         out->n[k] = n[k];
-        out->so[k] = s[0][k], out->sg[k] = s[1][k], out->sb[k] = s[2][k], out->sx[k] = s[3][k];
+        out->so[k] = s[0][k], out->sg[k] = s[1][k], out->sb[k] = s[2][k], out->sx[k] = s[3][k], out->sd[k] = s[4][k];
     }
     return true;
 }
@@ -640,72 +881,101 @@ template <int V> bool strides_whole(const LaneDims &d, const int64_t *s, int64_t
     return true;
 }
 
-template <typename T> int chain_workspace(Ctx *ctx, ScanArgs<T> *p, size_t width) {
-    const size_t tiles = (size_t)(p->groups * p->chunks);
-    const size_t flag_bytes = (tiles * sizeof(unsigned) + 255) & ~size_t(255);
-    const size_t state_bytes = tiles * width * sizeof(T);
-    void *ws = nullptr;
-    int rc = workspace(ctx, 256 + flag_bytes + 3 * state_bytes, &ws);
-    if (rc) return rc;
-    char *at = (char *)ws + kWsHeader;
-    p->ticket = (unsigned long long *)at;
-    p->flags = (unsigned *)(at + 256);
-    p->states = (T *)(at + 256 + flag_bytes);
-    p->maps = (T *)(at + 256 + flag_bytes + state_bytes);
-    const unsigned grid = (unsigned)std::min<size_t>((tiles + kThreads - 1) / kThreads, (size_t)ctx->sm_count);
-    launch_dep(ctx, grid, kThreads, scan_clear_kernel, p->ticket, p->flags, tiles);
-    return check_launch(ctx, "scan_clear_kernel");
-}
-
 constexpr uint64_t kMaxGrid = 0x7fffffffull;
+constexpr uint64_t kShortElements = 1u << 24;   // launches of some 30 us gain more from an early start than they lose
 
-template <typename T, int V, int R, int MODE, bool COUPLED, bool GVEC> int run_lanes(Ctx *ctx, ScanArgs<T> &p) {
-    constexpr uint64_t W = 32 * V, S = (uint64_t)kWarps * R;
-    p.groups = (p.lanes + W - 1) / W;
-    p.chunks = (p.steps + S - 1) / S;
-    if (p.groups > kMaxGrid / p.chunks) return fail(RTB_ERR_TOO_LARGE, "gated scan: %zu x %zu tiles are beyond one launch", (size_t)p.groups, (size_t)p.chunks);
-    if (p.chunks > 1)
-        if (int rc = chain_workspace(ctx, &p, W)) return rc;
-    launch_dep(ctx, (unsigned)(p.groups * p.chunks), kThreads, scan_lanes_kernel<T, V, R, MODE, COUPLED, GVEC>, p);
-    return check_launch(ctx, "scan_lanes_kernel");
+// Raises the kernel's shared-memory limit once per device and launches it in clusters of `cluster` CTAs.
+template <typename T, void (*kernel)(ScanArgs<T>)> int launch_ring(Ctx *ctx, const char *name, uint64_t grid, unsigned cluster, size_t smem, const ScanArgs<T> &p) {
+    if (grid > kMaxGrid) return fail(RTB_ERR_TOO_LARGE, "gated scan: %zu CTAs are beyond one launch", (size_t)grid);
+    static std::atomic<uint64_t> raised[64];   // by device: bytes allowed so far (each kernel instantiates this function)
+    std::atomic<uint64_t> &mark = raised[ctx->device & 63];
+    if (mark.load(std::memory_order_relaxed) < smem) {
+        RTB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        mark.store(smem, std::memory_order_relaxed);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    // A long-running grid of one wave must start on an empty device: started beside its predecessor's last CTAs it lands on
+    // the SMs that happen to be free and stays there (a 270 us backward pass behind a checkpoint: 435 us).
+    cfg.attrs = cluster > 1 ? attr : attr + 1;
+    cfg.numAttrs = (cluster > 1 ? 1 : 0) + (p.lanes * p.steps <= kShortElements ? 1 : 0);
+    if (!cfg.numAttrs) cfg.attrs = nullptr;
+    (void)cudaLaunchKernelEx(&cfg, kernel, p);
+    return check_launch(ctx, name);
 }
 
-template <typename T, int MODE, bool COUPLED> int pick_lanes(Ctx *ctx, ScanArgs<T> &p) {
+// How many CTAs share a group: as many as run at once (two on an SM), as long as each has a part of its own.
+unsigned cluster_for(const Ctx *ctx, uint64_t groups, uint64_t steps, uint64_t part) {
+    unsigned n = 1;
+    while (n < kMaxCluster && groups * n * 2 <= (uint64_t)ctx->sm_count * 2 && steps > (uint64_t)n * part) n *= 2;
+    return n;
+}
+
+template <typename T, int V, int LX, int R, int STAGES, int MODE, bool COUPLED, bool GVEC> int run_width(Ctx *ctx, ScanArgs<T> &p) {
+    constexpr uint64_t W = LX * V;
+    const uint64_t groups = (p.lanes + W - 1) / W, part = (uint64_t)kWarps * (32 / LX) * R;
+    p.cluster = cluster_for(ctx, groups, p.steps, part);
+    const size_t smem = (size_t)STAGES * LanesRing<T, V, R, MODE, COUPLED, GVEC>::kStageBytes + (p.cluster > 1 ? (size_t)p.cluster * 2 * (W + (GVEC ? W : LX)) * sizeof(T) : 0);
+    return launch_ring<T, scan_lanes_kernel<T, V, LX, R, STAGES, MODE, COUPLED, GVEC>>(ctx, "scan_lanes_kernel", groups * p.cluster, p.cluster, smem, p);
+}
+
+// Threads side by side in a group.  8 give rows of 128 bytes, a full line, and the most steps a round can have with them; 4 double the
+// steps again where groups of 8, in clusters of the largest size, would leave most SMs without work.  Measured, f32:
+// (1, 65536, 128) 112 us with 8, 76 with 4; (8, 8192, 1024) 142 us with 8, 171 with 4, 152 with 16, 155 with 32.
+template <typename T, int V> int side_by_side(const Ctx *ctx, const ScanArgs<T> &p) {
+    return (p.lanes + 8 * V - 1) / (8 * V) * kMaxCluster * 2 <= (uint64_t)ctx->sm_count ? 4 : 8;
+}
+
+// Four steps of a thread and two stages of the ring: two CTAs fit an SM in clusters of any size (the coupled backward pass
+// has one operand more and takes three).  Two steps with more stages, eight with one CTA on an SM, 512 threads and three CTAs on
+// an SM were all slower, by 5 to 60 %.
+template <typename T, int V, int MODE, bool COUPLED, bool GVEC> int run_lanes(Ctx *ctx, ScanArgs<T> &p) {
+    constexpr int R = MODE != kForward && COUPLED ? 3 : 4;
+    if (side_by_side<T, V>(ctx, p) == 4) return run_width<T, V, 4, R, 2, MODE, COUPLED, GVEC>(ctx, p);
+    return run_width<T, V, 8, R, 2, MODE, COUPLED, GVEC>(ctx, p);
+}
+
+// The V lanes of a thread are neighbours in every operand (or share the gate), at 16-byte aligned places.
+template <typename T, int MODE> bool lanes_vector(const ScanArgs<T> &p) {
     constexpr int V = 16 / sizeof(T);
-    constexpr int R = MODE == kForward ? 8 : 4;
     const LaneDims &d = p.dims;
     const int in = d.nd - 1;
     const bool gvec = d.sg[in] == 1;
-    // the V lanes of a thread are neighbours in every operand (or share the gate), at 16-byte aligned places
     bool vec = d.n[in] % V == 0 && d.so[in] == 1 && d.sb[in] == 1 && strides_whole<V>(d, d.so, p.to) && strides_whole<V>(d, d.sb, p.tb) &&
                aligned16(p.b) && p.o0 % V == 0 && (gvec || d.sg[in] == 0);
     if (gvec) vec = vec && strides_whole<V>(d, d.sg, p.tg) && aligned16(p.g);
     if (p.x) vec = vec && d.sx[in] == 1 && strides_whole<V>(d, d.sx, p.tx) && aligned16(p.x);
     for (const T *q : {(const T *)p.out, (const T *)p.dg, p.h}) vec = vec && aligned16(q);
     if (MODE == kBackCodes) vec = vec && aligned16((const T *)p.codes);
-    if (vec && gvec) return run_lanes<T, V, R, MODE, COUPLED, true>(ctx, p);
-    if (vec) return run_lanes<T, V, R, MODE, COUPLED, false>(ctx, p);
-    return run_lanes<T, 1, 8, MODE, COUPLED, false>(ctx, p);
+    return vec;
+}
+
+template <typename T, int MODE, bool COUPLED> int pick_lanes(Ctx *ctx, ScanArgs<T> &p, bool vec) {
+    constexpr int V = 16 / sizeof(T);
+    if (vec && p.dims.sg[p.dims.nd - 1] == 1) return run_lanes<T, V, MODE, COUPLED, true>(ctx, p);
+    if (vec) return run_lanes<T, V, MODE, COUPLED, false>(ctx, p);
+    return run_lanes<T, 1, MODE, COUPLED, false>(ctx, p);
 }
 
 template <typename T, int MODE, bool COUPLED, bool VEC> int run_axis(Ctx *ctx, ScanArgs<T> &p) {
-    constexpr int V = 16 / sizeof(T), K = 4;
-    // A warp per lane streams well once a few thousand warps are there; fewer lanes are cut along the axis.
-    constexpr uint64_t S = (uint64_t)kWarps * K * 32 * V;
-    if (p.lanes >= (uint64_t)ctx->sm_count * 16 || p.steps <= K * 32 * V) {
-        const uint64_t grid = (p.lanes + kWarps - 1) / kWarps;
-        if (grid > kMaxGrid) return fail(RTB_ERR_TOO_LARGE, "gated scan: %zu sequences are beyond one launch", (size_t)p.lanes);
-        p.groups = p.chunks = 1;
-        launch_dep(ctx, (unsigned)grid, kThreads, scan_axis_warp_kernel<T, V, K, MODE, COUPLED, VEC>, p);
-        return check_launch(ctx, "scan_axis_warp_kernel");
-    }
-    p.groups = p.lanes;
-    p.chunks = (p.steps + S - 1) / S;
-    if (p.groups > kMaxGrid / p.chunks) return fail(RTB_ERR_TOO_LARGE, "gated scan: %zu x %zu tiles are beyond one launch", (size_t)p.groups, (size_t)p.chunks);
-    if (p.chunks > 1)
-        if (int rc = chain_workspace(ctx, &p, 32)) return rc;
-    launch_dep(ctx, (unsigned)(p.groups * p.chunks), kThreads, scan_axis_kernel<T, V, K, MODE, COUPLED, VEC>, p);
-    return check_launch(ctx, "scan_axis_kernel");
+    constexpr int V = 16 / sizeof(T), K = MODE == kForward ? 4 : 2, S = 3;
+    using Ring = AxisRing<T, V, K, MODE, COUPLED>;
+    constexpr size_t smem = (size_t)S * Ring::kStageBytes;
+    p.cluster = 1;
+    // A warp for each lane wherever that gives every SM eight, or one part is all there is; else a CTA or a cluster.
+    if (p.lanes >= (uint64_t)ctx->sm_count * kWarps || p.steps <= Ring::kTile)
+        return launch_ring<T, scan_axis_kernel<T, V, K, S, 1, MODE, COUPLED, VEC>>(ctx, "scan_axis_kernel", (p.lanes + kWarps - 1) / kWarps, 1, smem, p);
+    constexpr uint64_t part = (uint64_t)kWarps * Ring::kTile;
+    p.cluster = cluster_for(ctx, p.lanes, p.steps, part);
+    return launch_ring<T, scan_axis_kernel<T, V, K, S, kWarps, MODE, COUPLED, VEC>>(ctx, "scan_axis_kernel", p.lanes * p.cluster, p.cluster, smem, p);
 }
 
 template <typename T, int MODE, bool COUPLED> int pick_axis(Ctx *ctx, ScanArgs<T> &p) {
@@ -721,13 +991,13 @@ template <typename T, int MODE, bool COUPLED> int pick_axis(Ctx *ctx, ScanArgs<T
     bool vec = p.steps % V == 0 && unit(p.tg) && unit(p.tb) && unit(p.to) && rows(p.dims.sg) && rows(p.dims.sb) && rows(p.dims.so) &&
                whole(p.g, p.tg) && whole(p.b, p.tb);
     if (p.x) vec = vec && unit(p.tx) && rows(p.dims.sx) && whole(p.x, p.tx);
-    for (const T *q : {(const T *)p.out, (const T *)p.dg}) vec = vec && aligned16(q);
+    for (const T *q : {(const T *)p.out, (const T *)p.dg, p.h, (const T *)p.codes}) vec = vec && aligned16(q);
     return vec ? run_axis<T, MODE, COUPLED, true>(ctx, p) : run_axis<T, MODE, COUPLED, false>(ctx, p);
 }
 
-template <typename T, int MODE> int pick(Ctx *ctx, ScanArgs<T> &p, bool along_axis, bool coupled) {
+template <typename T, int MODE> int pick(Ctx *ctx, ScanArgs<T> &p, bool along_axis, bool coupled, bool vec) {
     if (along_axis) return coupled ? pick_axis<T, MODE, true>(ctx, p) : pick_axis<T, MODE, false>(ctx, p);
-    return coupled ? pick_lanes<T, MODE, true>(ctx, p) : pick_lanes<T, MODE, false>(ctx, p);
+    return coupled ? pick_lanes<T, MODE, true>(ctx, p, vec) : pick_lanes<T, MODE, false>(ctx, p, vec);
 }
 
 // A temporary block of the context allocator, given back when the scope ends (stream order keeps it alive).
@@ -778,11 +1048,53 @@ struct ScanCall {
     void *out, *dg, *dh0;
 };
 
+// The gate's gradient when the gate is broadcast.  Where the innermost lanes share their gate, neighbours in segments of a power
+// of two are summed before anything is written; what is left to sum goes through a tensor of `shape` (the lanes in segments)
+// and rtb_reduce_to_shape.
+struct SharedGate {
+    std::vector<size_t> shape;
+    std::vector<ptrdiff_t> strides, gate_strides;
+    int seg_shift = 0;
+    bool rest = false;   // dims remain to be summed
+};
+
+SharedGate shared_gate(size_t rank, const size_t *shape, const ptrdiff_t *stride_g, size_t axis, uint64_t inner, unsigned widest) {
+    SharedGate s;
+    s.shape.assign(shape, shape + rank);
+    s.gate_strides.assign(stride_g, stride_g + rank);
+    // the trailing dims that were merged into the innermost lane dim
+    size_t k0 = rank;
+    uint64_t n = 1;
+    while (n < inner && k0 > axis + 1) n *= shape[--k0];
+    if (n == inner && widest > 1) {
+        while ((2u << s.seg_shift) <= widest && inner % (2u << s.seg_shift) == 0) ++s.seg_shift;
+        s.shape.resize(k0);
+        s.gate_strides.resize(k0);
+        s.shape.push_back((size_t)(inner >> s.seg_shift));
+        s.gate_strides.push_back(0);
+    }
+    for (size_t k = 0; k < s.shape.size(); ++k) s.rest = s.rest || (s.gate_strides[k] == 0 && s.shape[k] != 1);
+    s.strides.resize(s.shape.size());
+    rtb_meta_contiguous_strides(s.shape.size(), s.shape.data(), s.strides.data());
+    // as strides of the original dims: the merged ones walk lanes, locate() shifts them into segments
+    if (s.shape.size() != rank || s.seg_shift) {
+        s.strides.resize(k0);
+        s.strides.resize(rank);
+        ptrdiff_t step = 1;
+        for (size_t k = rank; k-- > k0;) s.strides[k] = step, step *= (ptrdiff_t)shape[k];
+    }
+    return s;
+}
+
 template <typename T> int run_scan(rtb_ctx *c, Ctx *ctx, int dtype, int flags, ScanCall call, size_t rank, const size_t *shape, size_t axis,
                                    size_t total) {
     std::vector<ptrdiff_t> dense(rank);
     rtb_meta_contiguous_strides(rank, shape, dense.data());
     const bool coupled = flags & RTB_SCAN_COUPLED, need_x = call.back && coupled && call.dg;
+    bool shared = false;
+    if (call.dg)
+        for (size_t k = 0; k < rank; ++k) shared = shared || (call.gate.strides[k] == 0 && shape[k] != 1);
+    const std::vector<ptrdiff_t> gate_strides(call.gate.strides, call.gate.strides + rank);
     // the innermost dim with more than one element decides: the axis itself, or a lane dim
     size_t inner = rank;
     for (size_t k = rank; k-- > 0;)
@@ -792,14 +1104,15 @@ template <typename T> int run_scan(rtb_ctx *c, Ctx *ctx, int dtype, int flags, S
         }
     const bool along_axis = inner >= rank || inner == axis;
     ScanArgs<T> p{};
-    Temp tg(c), tb(c), tx(c);
+    Temp tg(c), tb(c), tx(c), sums(c);
     int rc;
     for (int pass = 0;; ++pass) {
         const bool copy = pass == 1;   // too many lane dims: dense copies have two at most
         if ((rc = in_place_or_copy(c, dtype, rank, shape, inner, copy && !tg.p, total, dense, &call.gate, &tg))) return rc;
         if ((rc = in_place_or_copy(c, dtype, rank, shape, inner, copy && !tb.p, total, dense, &call.b, &tb))) return rc;
         if (need_x && (rc = in_place_or_copy(c, dtype, rank, shape, inner, copy && !tx.p, total, dense, &call.x, &tx))) return rc;
-        if (lane_dims(rank, shape, axis, dense.data(), call.gate.strides, call.b.strides, need_x ? call.x.strides : nullptr, &p.dims)) break;
+        const ptrdiff_t *const in[5] = {dense.data(), call.gate.strides, call.b.strides, need_x ? call.x.strides : nullptr, dense.data()};
+        if (lane_dims(rank, shape, axis, in, &p.dims)) break;
     }
     const int64_t steps = (int64_t)shape[axis];
     const bool down = ((flags & RTB_SCAN_REVERSE) != 0) != call.back;   // processing order runs towards lower indices
@@ -813,15 +1126,53 @@ template <typename T> int run_scan(rtb_ctx *c, Ctx *ctx, int dtype, int flags, S
     p.g = place(call.gate, &p.tg);
     p.b = place(call.b, &p.tb);
     if (need_x) p.x = place(call.x, &p.tx);
-    p.to = down ? -(int64_t)dense[axis] : (int64_t)dense[axis];
-    p.o0 = down ? (steps - 1) * (int64_t)dense[axis] : 0;
+    p.to = p.td = down ? -(int64_t)dense[axis] : (int64_t)dense[axis];
+    p.o0 = p.d0 = down ? (steps - 1) * (int64_t)dense[axis] : 0;
     p.h0 = (const T *)call.h0, p.h = (const T *)call.h;
     p.codes = (const int8_t *)call.codes, p.mags = (const T *)call.mags;
     p.out = (T *)call.out, p.dg = (T *)call.dg, p.dh0 = (T *)call.dh0;
-    std::lock_guard<std::mutex> lock(ctx->ws_mu);
-    if (!call.back) return pick<T, kForward>(ctx, p, along_axis, coupled);
-    if (call.codes) return pick<T, kBackCodes>(ctx, p, along_axis, coupled);
-    return pick<T, kBackDense>(ctx, p, along_axis, coupled);
+    bool vec = !along_axis && (call.back ? (call.codes ? lanes_vector<T, kBackCodes>(p) : lanes_vector<T, kBackDense>(p)) : lanes_vector<T, kForward>(p));
+    SharedGate share;
+    if (shared) {
+        const int in_dim = p.dims.nd - 1;
+        const bool segments = vec && p.dims.sg[in_dim] == 0;
+        share = shared_gate(rank, shape, gate_strides.data(), axis, segments ? p.dims.n[in_dim] : 0, segments ? 16 / sizeof(T) * side_by_side<T, 16 / sizeof(T)>(ctx, p) : 1);
+        if (share.seg_shift) {
+            p.seg_shift = share.seg_shift;
+            const ptrdiff_t *const in[5] = {dense.data(), call.gate.strides, call.b.strides, need_x ? call.x.strides : nullptr, share.strides.data()};
+            if (!lane_dims(rank, shape, axis, in, &p.dims)) return fail(RTB_ERR_TOO_LARGE, "gated scan: more than %d dims", kMaxLaneDims);
+            p.td = down ? -(int64_t)share.strides[axis] : (int64_t)share.strides[axis];
+            p.d0 = down ? (steps - 1) * (int64_t)share.strides[axis] : 0;
+        }
+        if (share.rest) {
+            size_t n = 1;
+            for (size_t v : share.shape) n *= v;
+            if ((rc = rtb_alloc(c, n * sizeof(T), &sums.p))) return rc;
+            p.dg = (T *)sums.p;
+        }
+    }
+    if (!call.back) rc = pick<T, kForward>(ctx, p, along_axis, coupled, vec);
+    else if (call.codes) rc = pick<T, kBackCodes>(ctx, p, along_axis, coupled, vec);
+    else rc = pick<T, kBackDense>(ctx, p, along_axis, coupled, vec);
+    if (rc || !sums.p) return rc;
+    // only a short innermost dim is left: one thread for each sum (a row each is what the axis reduction is built for)
+    size_t left = 1, n_out = 1;
+    bool inner_only = true;
+    for (size_t k = 0; k < share.shape.size(); ++k) {
+        if (share.gate_strides[k] == 0 && share.shape[k] != 1) {
+            inner_only = inner_only && left == 1 && k + 1 == share.shape.size();
+            left *= share.shape[k];
+        } else {
+            n_out *= share.shape[k];
+        }
+    }
+    if (inner_only && left <= 64 && n_out / kThreads < kMaxGrid) {
+        launch_dep(ctx, (unsigned)((n_out + kThreads - 1) / kThreads), kThreads, neighbour_sum_kernel<T>, (const T *)sums.p, (uint64_t)n_out,
+                   (unsigned)left, (T *)call.dg);
+        return check_launch(ctx, "neighbour_sum_kernel");
+    }
+    std::vector<size_t> out_shape(share.shape.size());
+    return rtb_reduce_to_shape(c, dtype, sums.p, share.shape.size(), share.shape.data(), share.gate_strides.data(), call.dg, out_shape.data());
 }
 
 template <typename T, bool COUPLED> int run_step(Ctx *ctx, const LaneDims &d, uint64_t lanes, T *state, const T *g, const T *x) {
@@ -844,7 +1195,8 @@ template <typename T> int step_any(Ctx *ctx, int flags, T *state, const ptrdiff_
     LaneDims d;
     uint64_t lanes = 1;
     for (size_t k = 0; k < rank; ++k) lanes *= shape[k];
-    if (lane_dims(rank, shape, rank, ss, sg, sx, nullptr, &d))
+    const ptrdiff_t *const in[5] = {ss, sg, sx, nullptr, nullptr};
+    if (lane_dims(rank, shape, rank, in, &d))
         return flags & RTB_SCAN_COUPLED ? run_step<T, true>(ctx, d, lanes, state, g, x) : run_step<T, false>(ctx, d, lanes, state, g, x);
     // more dims than one launch takes: peel the outermost one that has extent
     size_t k0 = 0;
@@ -897,18 +1249,14 @@ RTB_API int rtb_gated_scan_backward(rtb_ctx *c, int dtype, int flags, const void
     const size_t total = count_of(rank, shape), es = dtype_size(dtype);
     Ctx *ctx = C(c);
     if (!stride_g) return fail(RTB_ERR_INVALID, "null argument");
-    bool shared = false;   // the gate is broadcast along some dim: its gradient is summed over it
-    size_t gate_n = 1;
-    for (size_t k = 0; k < rank; ++k) {
-        if (stride_g[k] == 0 && shape[k] != 1) shared = true;
-        else gate_n *= shape[k];
-    }
     if (total == 0) {
         // no step and no upstream: what is left of the gradients is zero
         if ((rc = use_device(ctx))) return rc;
-        size_t lanes = 1;
-        for (size_t k = 0; k < rank; ++k)
+        size_t lanes = 1, gate_n = 1;
+        for (size_t k = 0; k < rank; ++k) {
             if (k != axis) lanes *= shape[k];
+            if (stride_g[k] != 0) gate_n *= shape[k];   // the dims it is broadcast along are summed
+        }
         if (d_h0 && lanes) RTB_CUDA(cudaMemsetAsync(d_h0, 0, lanes * es, ctx->stream));
         if (d_gate && gate_n) RTB_CUDA(cudaMemsetAsync(d_gate, 0, gate_n * es, ctx->stream));
         return RTB_OK;
@@ -926,16 +1274,8 @@ RTB_API int rtb_gated_scan_backward(rtb_ctx *c, int dtype, int flags, const void
     call.x = View{x, stride_x, off_x};
     call.h0 = h0, call.h = h, call.codes = codes, call.mags = mags;
     call.out = d_x, call.dg = d_gate, call.dh0 = d_h0;
-    Temp full(c);
-    if (shared && d_gate) {
-        if ((rc = rtb_alloc(c, total * es, &full.p))) return rc;
-        call.dg = full.p;
-    }
-    rc = dtype == RTB_F32 ? run_scan<float>(c, ctx, dtype, flags, call, rank, shape, axis, total)
-                          : run_scan<double>(c, ctx, dtype, flags, call, rank, shape, axis, total);
-    if (rc || !full.p) return rc;
-    std::vector<size_t> out_shape(rank);
-    return rtb_reduce_to_shape(c, dtype, full.p, rank, shape, stride_g, d_gate, out_shape.data());
+    return dtype == RTB_F32 ? run_scan<float>(c, ctx, dtype, flags, call, rank, shape, axis, total)
+                            : run_scan<double>(c, ctx, dtype, flags, call, rank, shape, axis, total);
 }
 
 RTB_API int rtb_gated_step(rtb_ctx *c, int dtype, int flags, void *state, const ptrdiff_t *stride_s, size_t off_s, const void *gate,

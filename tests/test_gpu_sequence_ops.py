@@ -235,9 +235,12 @@ def test_steps_equal_the_scan_and_leave_the_rest_of_a_pool():
         step = [v if v.rank == 2 else v.squeeze(1) for v in step]
         state.gated_step_inplace(*step)
     got = tp.cpu()
-    want = pool.copy()
-    want[:, 4, 8:24] = h[:, -1]
-    assert got.tobytes() == want.tobytes()
+    # the scan associates the same products and sums otherwise than the steps do: each is within the bound of the exact states
+    exact, tol = _scan_ref(x, a, 1, pool[:, 4:5, 8:24], False, False, U[np.float32])
+    _close(h, exact, tol)
+    _close(got[:, 4, 8:24], exact[:, -1], tol[:, -1])
+    got[:, 4, 8:24] = pool[:, 4, 8:24]
+    assert got.tobytes() == pool.tobytes()
 
 
 def test_scan_refusals():
