@@ -41,17 +41,21 @@ template <> struct Bits<double> {
 };
 
 // round(127 x / m), ties to even, exactly.  f32: the quotient in 64 bits decides every case (127 x is exact there, and
-// a quotient that is no tie is at least 2^-33 of itself away from one); the product with the rounded
-// reciprocal is off by less than 2e-5 and decides all but the values that near to a tie.
+// a quotient that is no tie is at least 2^-33 of itself away from one).  x times an approximate 127 / m is off by less
+// than 1e-4 and decides all but the values that near to a tie; adding 1.5 2^23 rounds it and leaves the code in the low byte.
 struct Quantise32 {
     float m, inv;
     bool wide;
-    __device__ __forceinline__ explicit Quantise32(float mag) : m(mag), inv(127.0f / mag), wide(mag < 1e-30f) {}
-    __device__ __forceinline__ int code(float x) const {
-        const float t = x * inv;
-        float q = rintf(t);
-        if (wide || fabsf(t - q) > 0.4999f) q = m > 0.0f ? (float)rint(127.0 * (double)x / (double)m) : 0.0f;
-        return (int)q;
+    __device__ __forceinline__ explicit Quantise32(float mag) : m(mag), wide(!(mag > 1e-30f && mag < 1e37f)) {
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(mag));
+        inv *= 127.0f;
+    }
+    __device__ __forceinline__ uint32_t code(float x) const {   // in the low byte
+        const float magic = 12582912.0f;
+        const float t = fmaf(x, inv, magic);
+        uint32_t c = __float_as_uint(t);
+        if (wide || fabsf(fmaf(x, inv, magic - t)) > 0.4998f) c = m > 0.0f ? (uint32_t)(int)rint(127.0 * (double)x / (double)m) : 0u;
+        return c;
     }
 };
 struct Quantise64 {
@@ -59,7 +63,7 @@ struct Quantise64 {
     __device__ __forceinline__ explicit Quantise64(double mag) : m(mag), down(1.0) {
         if (mag > 1e300) m = mag * 0x1p-20, down = 0x1p-20;   // 127 x stays finite
     }
-    __device__ __forceinline__ int code(double x) const { return m > 0.0 ? (int)rint(127.0 * (x * down) / m) : 0; }
+    __device__ __forceinline__ uint32_t code(double x) const { return m > 0.0 ? (uint32_t)(int)rint(127.0 * (x * down) / m) : 0u; }
 };
 template <typename T> struct QuantiseOf;
 template <> struct QuantiseOf<float> { using type = Quantise32; };
@@ -104,14 +108,13 @@ __device__ __forceinline__ uint32_t load_codes(const int8_t *p, size_t i, size_t
         if (i + k < n) c |= (uint32_t)(uint8_t)p[i + k] << (8 * k);
     return c;
 }
-__device__ __forceinline__ void store_codes(int8_t *p, size_t i, size_t n, char4 c) {
+__device__ __forceinline__ void store_codes(int8_t *p, size_t i, size_t n, uint32_t c) {
     if (i + 4 <= n) {
-        *reinterpret_cast<char4 *>(p + i) = c;
+        *reinterpret_cast<uint32_t *>(p + i) = c;
         return;
     }
-    if (i < n) p[i] = c.x;
-    if (i + 1 < n) p[i + 1] = c.y;
-    if (i + 2 < n) p[i + 2] = c.z;
+    for (int k = 0; k < 3; ++k)
+        if (i + k < n) p[i + k] = (int8_t)(c >> (8 * k));
 }
 
 template <typename T, bool VEC>
@@ -131,13 +134,13 @@ __global__ void __launch_bounds__(kThreads) ckpt8_store_kernel(const T *src, siz
         for (int k = 0; k < 4; ++k) top = max(top, B::abs(v[u][k]));
         top = B::warp_max(top);
         if ((block0 + u) * kCkpt8Block >= n) continue;   // the same in the whole warp
-        char4 c = make_char4(0, 0, 0, 0);
+        uint32_t c = 0;
         T m = B::value(top);
         if (top >= B::inf) {
             m = B::value(B::inf | 1u);   // some NaN
         } else {
             const typename QuantiseOf<T>::type q(m);
-            c = make_char4(q.code(v[u][0]), q.code(v[u][1]), q.code(v[u][2]), q.code(v[u][3]));
+            c = __byte_perm(__byte_perm(q.code(v[u][0]), q.code(v[u][1]), 0x0040), __byte_perm(q.code(v[u][2]), q.code(v[u][3]), 0x0040), 0x5410);
         }
         store_codes(codes, i, n, c);
         if (lane == 0) mags[block0 + u] = m;

@@ -23,6 +23,7 @@
 
 #include "rtb_internal.h"
 #include "rtb_ckpt8.cuh"
+#include "rtb_cluster.cuh"
 
 namespace rtb {
 namespace {
@@ -30,84 +31,10 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxLaneDims = 6;
-constexpr unsigned kMaxCluster = 8;
-constexpr unsigned long long kWaitNs = 2000000000ull;   // limit of a wait for another CTA's maps
 
 
 __device__ __forceinline__ float fma_(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_(double a, double b, double c) { return fma(a, b, c); }
-template <typename T, int V> struct alignas(sizeof(T) * V) Pack {
-    T e[V];
-};
-template <typename T, int V> __device__ __forceinline__ Pack<T, V> ld(const T *p) { return *reinterpret_cast<const Pack<T, V> *>(p); }
-template <typename T, int V> __device__ __forceinline__ void st(T *p, const Pack<T, V> &v) { *reinterpret_cast<Pack<T, V> *>(p) = v; }
-
-// asynchronous copy of BYTES (4, 8 or 16) into shared memory
-template <int BYTES> __device__ __forceinline__ void copy_async(void *smem, const void *gmem) {
-    const unsigned dst = (unsigned)__cvta_generic_to_shared(smem);
-    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(gmem) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(gmem), "n"(BYTES) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int PENDING> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
-
-__device__ __forceinline__ unsigned cluster_rank() {
-    unsigned r;
-    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
-}
-// Maps travel between the CTAs of a cluster as asynchronous stores that count their bytes on a barrier of the receiver: unlike
-// a cluster-wide barrier they do not wait for the sender's own global stores.
-__device__ __forceinline__ unsigned smem_addr(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ unsigned in_cta(unsigned addr, unsigned rank) {
-    unsigned at;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
-    return at;
-}
-template <typename P> __device__ __forceinline__ void send(unsigned to, const P &v, unsigned mbar) {
-    static_assert(sizeof(P) == 4 || sizeof(P) == 8 || sizeof(P) == 16, "one store");
-    if constexpr (sizeof(P) == 16) {
-        uint4 q;
-        memcpy(&q, &v, 16);
-        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "r"(q.x),
-                     "r"(q.y), "r"(q.z), "r"(q.w), "r"(mbar) : "memory");
-    } else if constexpr (sizeof(P) == 8) {
-        unsigned long long q;
-        memcpy(&q, &v, 8);
-        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(to), "l"(q), "r"(mbar) : "memory");
-    } else {
-        unsigned q;
-        memcpy(&q, &v, 4);
-        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to), "r"(q), "r"(mbar) : "memory");
-    }
-}
-__device__ __forceinline__ void mbar_init(unsigned long long *bar) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(bar)) : "memory");
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-}
-__device__ __forceinline__ void mbar_expect(unsigned long long *bar, unsigned bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ unsigned long long now_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-// -> whether the phase completed within the limit
-__device__ __forceinline__ bool mbar_wait(unsigned long long *bar, unsigned parity) {
-    unsigned long long began = 0;
-    for (;;) {
-        unsigned done;
-        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-                     : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
-        if (done) return true;
-        if (!began) began = now_ns();
-        else if (now_ns() - began > kWaitNs) return false;
-    }
-}
 __device__ __forceinline__ float nan_of(float) { return __int_as_float(0x7fffffff); }
 __device__ __forceinline__ double nan_of(double) { return __longlong_as_double(0x7fffffffffffffffll); }
 
@@ -881,50 +808,31 @@ template <int V> bool strides_whole(const LaneDims &d, const int64_t *s, int64_t
     return true;
 }
 
-constexpr uint64_t kMaxGrid = 0x7fffffffull;
 constexpr uint64_t kShortElements = 1u << 24;   // launches of some 30 us gain more from an early start than they lose
 
-// Raises the kernel's shared-memory limit once per device and launches it in clusters of `cluster` CTAs.
-template <typename T, void (*kernel)(ScanArgs<T>)> int launch_ring(Ctx *ctx, const char *name, uint64_t grid, unsigned cluster, size_t smem, const ScanArgs<T> &p) {
-    if (grid > kMaxGrid) return fail(RTB_ERR_TOO_LARGE, "gated scan: %zu CTAs are beyond one launch", (size_t)grid);
-    static std::atomic<uint64_t> raised[64];   // by device: bytes allowed so far (each kernel instantiates this function)
-    std::atomic<uint64_t> &mark = raised[ctx->device & 63];
-    if (mark.load(std::memory_order_relaxed) < smem) {
-        RTB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        mark.store(smem, std::memory_order_relaxed);
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    // A long-running grid of one wave must start on an empty device: started beside its predecessor's last CTAs it lands on
-    // the SMs that happen to be free and stays there (a 270 us backward pass behind a checkpoint: 435 us).
-    cfg.attrs = cluster > 1 ? attr : attr + 1;
-    cfg.numAttrs = (cluster > 1 ? 1 : 0) + (p.lanes * p.steps <= kShortElements ? 1 : 0);
-    if (!cfg.numAttrs) cfg.attrs = nullptr;
-    (void)cudaLaunchKernelEx(&cfg, kernel, p);
-    return check_launch(ctx, name);
-}
-
-// How many CTAs share a group: as many as run at once (two on an SM), as long as each has a part of its own.
-unsigned cluster_for(const Ctx *ctx, uint64_t groups, uint64_t steps, uint64_t part) {
+// How many CTAs share a group: as many as run at once, as long as each has a part of its own.  `smem` says what a size needs.
+template <typename T, void (*kernel)(ScanArgs<T>), typename F> int cluster_for(Ctx *ctx, uint64_t groups, uint64_t steps, uint64_t part, F smem, unsigned *out) {
     unsigned n = 1;
-    while (n < kMaxCluster && groups * n * 2 <= (uint64_t)ctx->sm_count * 2 && steps > (uint64_t)n * part) n *= 2;
-    return n;
+    while (n < kMaxCluster && steps > (uint64_t)n * part) {
+        unsigned fit = 0;
+        if (int rc = clusters_at_once<ScanArgs<T>, kernel>(ctx, kThreads, n * 2, smem(n * 2), &fit)) return rc;
+        if (groups > fit) break;
+        n *= 2;
+    }
+    *out = n;
+    return RTB_OK;
 }
 
 template <typename T, int V, int LX, int R, int STAGES, int MODE, bool COUPLED, bool GVEC> int run_width(Ctx *ctx, ScanArgs<T> &p) {
     constexpr uint64_t W = LX * V;
     const uint64_t groups = (p.lanes + W - 1) / W, part = (uint64_t)kWarps * (32 / LX) * R;
-    p.cluster = cluster_for(ctx, groups, p.steps, part);
-    const size_t smem = (size_t)STAGES * LanesRing<T, V, R, MODE, COUPLED, GVEC>::kStageBytes + (p.cluster > 1 ? (size_t)p.cluster * 2 * (W + (GVEC ? W : LX)) * sizeof(T) : 0);
-    return launch_ring<T, scan_lanes_kernel<T, V, LX, R, STAGES, MODE, COUPLED, GVEC>>(ctx, "scan_lanes_kernel", groups * p.cluster, p.cluster, smem, p);
+    constexpr auto kernel = scan_lanes_kernel<T, V, LX, R, STAGES, MODE, COUPLED, GVEC>;
+    auto smem = [](unsigned cluster) {
+        return (size_t)STAGES * LanesRing<T, V, R, MODE, COUPLED, GVEC>::kStageBytes + (cluster > 1 ? (size_t)cluster * 2 * (W + (GVEC ? W : LX)) * sizeof(T) : 0);
+    };
+    if (int rc = cluster_for<T, kernel>(ctx, groups, p.steps, part, smem, &p.cluster)) return rc;
+    return launch_cluster<ScanArgs<T>, kernel>(ctx, "scan_lanes_kernel", groups * p.cluster, kThreads, p.cluster, smem(p.cluster),
+                                               p.lanes * p.steps <= kShortElements, p);
 }
 
 // Threads side by side in a group.  8 give rows of 128 bytes, a full line, and the most steps a round can have with them; 4 double the
@@ -972,10 +880,10 @@ template <typename T, int MODE, bool COUPLED, bool VEC> int run_axis(Ctx *ctx, S
     p.cluster = 1;
     // A warp for each lane wherever that gives every SM eight, or one part is all there is; else a CTA or a cluster.
     if (p.lanes >= (uint64_t)ctx->sm_count * kWarps || p.steps <= Ring::kTile)
-        return launch_ring<T, scan_axis_kernel<T, V, K, S, 1, MODE, COUPLED, VEC>>(ctx, "scan_axis_kernel", (p.lanes + kWarps - 1) / kWarps, 1, smem, p);
-    constexpr uint64_t part = (uint64_t)kWarps * Ring::kTile;
-    p.cluster = cluster_for(ctx, p.lanes, p.steps, part);
-    return launch_ring<T, scan_axis_kernel<T, V, K, S, kWarps, MODE, COUPLED, VEC>>(ctx, "scan_axis_kernel", p.lanes * p.cluster, p.cluster, smem, p);
+        return launch_cluster<ScanArgs<T>, scan_axis_kernel<T, V, K, S, 1, MODE, COUPLED, VEC>>(ctx, "scan_axis_kernel", (p.lanes + kWarps - 1) / kWarps, kThreads, 1, smem, p.lanes * p.steps <= kShortElements, p);
+    constexpr auto team = scan_axis_kernel<T, V, K, S, kWarps, MODE, COUPLED, VEC>;
+    if (int rc = cluster_for<T, team>(ctx, p.lanes, p.steps, (uint64_t)kWarps * Ring::kTile, [](unsigned) { return smem; }, &p.cluster)) return rc;
+    return launch_cluster<ScanArgs<T>, team>(ctx, "scan_axis_kernel", p.lanes * p.cluster, kThreads, p.cluster, smem, p.lanes * p.steps <= kShortElements, p);
 }
 
 template <typename T, int MODE, bool COUPLED> int pick_axis(Ctx *ctx, ScanArgs<T> &p) {
