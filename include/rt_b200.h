@@ -414,7 +414,8 @@ int rtb_convert(rtb_ctx *ctx, int src_dtype, int dst_dtype, const void *src, voi
  *        h_s = a_s h_{s-1} + (1 - a_s) x_s    with RTB_SCAN_COUPLED
  *      gate and x are views of `shape`; stride 0 broadcasts.  h, h0 and every gradient are dense row-major: h, d_x over
  *      `shape`, h0 and d_h0 over `shape` with dim `axis` as 1, d_gate over `shape` with the dims along which the
- *      gate has stride 0 as 1 (summed over them, as rtb_reduce_to_shape does).  No output may overlap an input.
+ *      gate has stride 0 as 1 (summed over them, as rtb_reduce_to_shape does).  No output may overlap an input.  At most
+ *      2^31 - 2^16 steps (RTB_ERR_TOO_LARGE).
  *      f32 / f64; states are held in the tensors' type, a step is one fused multiply-add.
  *
  *      rtb_gated_scan_backward: `up` is the gradient of every h_s; `h` the states of the forward pass, or NULL with `codes`

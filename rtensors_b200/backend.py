@@ -40,17 +40,6 @@ _TYPESTR = {torch.float32: "<f4", torch.float64: "<f8", torch.int32: "<i4", torc
             torch.int8: "|i1", torch.uint8: "|u1", torch.bool: "|b1"}
 
 
-def _same_dtype(first: torch.Tensor, *rest: Optional[torch.Tensor]):
-    for t in rest:
-        if t is not None and t.dtype != first.dtype:
-            raise L.RtbError(L.ERR_DTYPE, f"operands of {first.dtype} and {t.dtype}")
-
-
-def _same_shape(a: Meta, b: Meta):
-    if a.shape != b.shape:
-        raise L.RtbError(L.ERR_SHAPE, f"views of shapes {a.shape} and {b.shape}")
-
-
 def _axis(axis: int, rank: int) -> int:
     if not 0 <= axis < rank:
         raise L.RtbError(L.ERR_DIM, f"axis {axis} out of range for rank {rank}")
@@ -58,20 +47,11 @@ def _axis(axis: int, rank: int) -> int:
 
 
 def _lanes(meta: Meta, axis: int) -> int:
+    """Sequences of a scan along `axis`: the elements of the other dims."""
     n = 1
     for k, s in enumerate(meta.shape):
         n *= 1 if k == axis else s
     return n
-
-
-def _holds_lanes(buf: Optional[torch.Tensor], meta: Meta, axis: int, what: str):
-    _axis(axis, meta.rank)
-    if buf is not None and buf.numel() < _lanes(meta, axis):
-        raise L.RtbError(L.ERR_BOUNDS, f"{what} needs {_lanes(meta, axis)} elements, its buffer has {buf.numel()}")
-
-
-def _scan_flags(reverse: bool, coupled: bool) -> int:
-    return (L.SCAN_REVERSE if reverse else 0) | (L.SCAN_COUPLED if coupled else 0)
 
 
 class _DeviceBlock:
@@ -90,6 +70,7 @@ class CudaB200:
         if not torch.cuda.is_available():
             raise RuntimeError("CudaB200 needs a CUDA device; there is no CPU fallback")
         self.device = self._index = int(device)
+        self._torch_device = torch.device("cuda", self.device)
         torch.cuda.set_device(self.device)
         self._ctx = C.c_void_p()
         check(lib().rtb_ctx_create(C.c_int(self.device), C.byref(self._ctx)))
@@ -130,7 +111,7 @@ class CudaB200:
 
     def alloc(self, n: int, dtype: torch.dtype) -> torch.Tensor:
         """Uninitialised device buffer (Backend::alloc)."""
-        return torch.empty(int(n), dtype=dtype, device=f"cuda:{self.device}")
+        return torch.empty(int(n), dtype=dtype, device=self._torch_device)
 
     def alloc_from_slice(self, host: np.ndarray) -> torch.Tensor:
         return torch.from_numpy(np.ascontiguousarray(host).reshape(-1)).to(f"cuda:{self.device}")
@@ -410,25 +391,44 @@ class CudaB200:
         return out, oshape
 
     # -- gated linear recurrence, 8-bit checkpoints, cross-entropy ---------------------------------
-    def _own(self, *bufs: Optional[torch.Tensor]):
-        """Every buffer is on this backend's device (a foreign address would fault inside a kernel)."""
-        for b in bufs:
-            if b is not None and b.device.index != self._index:
-                raise L.RtbError(L.ERR_INVALID, f"a buffer on {b.device} was given to the backend of cuda:{self.device}")
+    def _same(self, first: torch.Tensor, *rest: Optional[torch.Tensor]):
+        """One dtype, and every buffer on this backend's device (a foreign address would fault inside a kernel)."""
+        dt, index = first.dtype, self._index
+        if first.get_device() != index:
+            raise L.RtbError(L.ERR_INVALID, f"a buffer on {first.device} was given to the backend of cuda:{index}")
+        for t in rest:
+            if t is None:
+                continue
+            if t.dtype is not dt:
+                raise L.RtbError(L.ERR_DTYPE, f"operands of {dt} and {t.dtype}")
+            if t.get_device() != index:
+                raise L.RtbError(L.ERR_INVALID, f"a buffer on {t.device} was given to the backend of cuda:{index}")
+
+    @staticmethod
+    def _views(shape, *views: Tuple[torch.Tensor, Meta]):
+        """Every view has this shape and lies inside its buffer."""
+        for buf, m in views:
+            if m.shape != shape:
+                raise L.RtbError(L.ERR_SHAPE, f"views of shapes {shape} and {m.shape}")
+            m.check_extent(buf.numel())
+
+    def _first_states(self, h0: Optional[torch.Tensor], meta: Meta, axis: int):
+        if h0 is not None and h0.numel() < _lanes(meta, axis):
+            raise L.RtbError(L.ERR_BOUNDS, f"h0 needs {_lanes(meta, axis)} elements, its buffer has {h0.numel()}")
 
     def gated_scan(self, x: torch.Tensor, xm: Meta, gate: torch.Tensor, gm: Meta, axis: int, h0: Optional[torch.Tensor] = None,
                    reverse: bool = False, coupled: bool = False) -> torch.Tensor:
         """h_s = gate_s h_{s-1} + x_s along `axis` (rtb_gated_scan); gm carries x's shape, stride 0 on broadcast dims; h0 is
         dense over the shape with `axis` as 1.  -> the states, dense row-major."""
-        _same_dtype(x, gate, h0)
-        self._own(x, gate, h0)
-        _same_shape(xm, gm)
-        xm.check_extent(x.numel()); gm.check_extent(gate.numel())
-        _holds_lanes(h0, xm, axis, "h0")
+        _axis(axis, xm.rank)
+        self._same(x, gate, h0)
+        self._views(xm.shape, (x, xm), (gate, gm))
+        self._first_states(h0, xm, axis)
         out = self.alloc(max(xm.size, 1), x.dtype)
-        check(lib().rtb_gated_scan(self._ctx, dtype_code(x), _scan_flags(reverse, coupled), gate.data_ptr(), gm.c_strides, gm.offset,
+        flags = (L.SCAN_REVERSE if reverse else 0) | (L.SCAN_COUPLED if coupled else 0)
+        check(lib().rtb_gated_scan(self._ctx, dtype_code(x), flags, gate.data_ptr(), gm.c_strides, gm.offset,
                                    x.data_ptr(), xm.c_strides, xm.offset, None if h0 is None else h0.data_ptr(), out.data_ptr(),
-                                   xm.rank, xm.c_shape, _axis(axis, xm.rank)))
+                                   xm.rank, xm.c_shape, axis))
         return out
 
     def gated_scan_backward(self, up: torch.Tensor, um: Meta, gate: torch.Tensor, gm: Meta, axis: int,
@@ -438,11 +438,10 @@ class CudaB200:
         """Gradients of gated_scan for the upstream `up` of every state (rtb_gated_scan_backward): h is the forward pass's
         dense result, or ckpt = (codes, mags) its 8-bit checkpoint; x is needed for the coupled gate's gradient.
         -> (d_x, d_gate with the gate's broadcast dims summed, d_h0), None where not wanted (d_h0: without h0)."""
-        _same_dtype(up, gate, h, x, h0)
-        self._own(up, gate, h, x, h0)
-        _same_shape(um, gm)
-        um.check_extent(up.numel()); gm.check_extent(gate.numel())
-        _holds_lanes(h0, um, axis, "h0")
+        _axis(axis, um.rank)
+        self._same(up, gate, h, x, h0)
+        self._views(um.shape, (up, um), (gate, gm))
+        self._first_states(h0, um, axis)
         want_x, want_g, want_h0 = want[0], want[1], want[2] and h0 is not None
         n = um.size
         codes = mags = None
@@ -457,30 +456,29 @@ class CudaB200:
             if coupled:
                 if x is None:
                     raise L.RtbError(L.ERR_INVALID, "the coupled gate's gradient needs x")
-                _same_shape(um, xm)
-                xm.check_extent(x.numel())
-        n_gate = 1
-        for s, st in zip(gm.shape, gm.strides):
-            n_gate *= s if st else 1
-        lanes = n // um.shape[axis] if n else _lanes(um, axis)
+                self._views(um.shape, (x, xm))
         dx = self.alloc(max(n, 1), up.dtype) if want_x else None
-        dg = self.alloc(max(n_gate, 1), up.dtype) if want_g else None
-        dh0 = self.alloc(max(lanes, 1), up.dtype) if want_h0 else None
+        dg = dh0 = None
+        if want_g:
+            n_gate = 1
+            for s, st in zip(gm.shape, gm.strides):
+                n_gate *= s if st else 1
+            dg = self.alloc(max(n_gate, 1), up.dtype)
+        if want_h0:
+            dh0 = self.alloc(max(_lanes(um, axis), 1), up.dtype)
         x_args = (x.data_ptr(), xm.c_strides, xm.offset) if x is not None and coupled and want_g else (None, None, 0)
         check(lib().rtb_gated_scan_backward(
-            self._ctx, dtype_code(up), _scan_flags(reverse, coupled), up.data_ptr(), um.c_strides, um.offset, gate.data_ptr(),
+            self._ctx, dtype_code(up), (L.SCAN_REVERSE if reverse else 0) | (L.SCAN_COUPLED if coupled else 0), up.data_ptr(), um.c_strides, um.offset, gate.data_ptr(),
             gm.c_strides, gm.offset, *x_args, h.data_ptr() if h is not None and want_g else None,
             None if codes is None else codes.data_ptr(), None if mags is None else mags.data_ptr(),
             None if h0 is None else h0.data_ptr(), None if dx is None else dx.data_ptr(), None if dg is None else dg.data_ptr(),
-            None if dh0 is None else dh0.data_ptr(), um.rank, um.c_shape, _axis(axis, um.rank)))
+            None if dh0 is None else dh0.data_ptr(), um.rank, um.c_shape, axis))
         return dx, dg, dh0
 
     def gated_step(self, state: torch.Tensor, sm: Meta, gate: torch.Tensor, gm: Meta, x: torch.Tensor, xm: Meta, coupled: bool = False):
         """One step of the recurrence in place: state = gate state + x over views of one shape (rtb_gated_step)."""
-        _same_dtype(state, gate, x)
-        self._own(state, gate, x)
-        _same_shape(sm, gm); _same_shape(sm, xm)
-        sm.check_extent(state.numel()); gm.check_extent(gate.numel()); xm.check_extent(x.numel())
+        self._same(state, gate, x)
+        self._views(sm.shape, (state, sm), (gate, gm), (x, xm))
         check(lib().rtb_gated_step(self._ctx, dtype_code(state), L.SCAN_COUPLED if coupled else 0, state.data_ptr(), sm.c_strides, sm.offset,
                                    gate.data_ptr(), gm.c_strides, gm.offset, x.data_ptr(), xm.c_strides, xm.offset, sm.rank, sm.c_shape))
 
@@ -489,16 +487,17 @@ class CudaB200:
         n = src.numel() - offset if n is None else n
         if offset < 0 or n < 0 or offset + n > src.numel():
             raise L.RtbError(L.ERR_BOUNDS, f"range [{offset}, {offset + n}) exceeds a buffer of {src.numel()}")
-        self._own(src)
+        self._same(src)
         codes = self.alloc(max(n, 1), torch.int8)
         mags = self.alloc(max(-(-n // L.CKPT8_BLOCK), 1), src.dtype)
         check(lib().rtb_ckpt8_store(self._ctx, dtype_code(src), src.data_ptr() + offset * src.element_size(), n, codes.data_ptr(), mags.data_ptr()))
         return codes, mags
 
     def _check_ckpt(self, codes, mags, n, like):
-        if codes.dtype != torch.int8 or codes.numel() < n or mags.numel() * L.CKPT8_BLOCK < n or mags.dtype != like.dtype:
+        if codes.dtype is not torch.int8 or codes.numel() < n or mags.numel() * L.CKPT8_BLOCK < n or mags.dtype is not like.dtype:
             raise L.RtbError(L.ERR_BOUNDS, f"the checkpoint does not hold {n} elements of {like.dtype}")
-        self._own(codes, mags)
+        self._same(codes)
+        self._same(mags, like)
 
     def ckpt8_restore(self, codes: torch.Tensor, mags: torch.Tensor, n: int) -> torch.Tensor:
         self._check_ckpt(codes, mags, n, mags)
@@ -509,7 +508,6 @@ class CudaB200:
     def ckpt8_grad(self, kind: int, codes: torch.Tensor, mags: torch.Tensor, up: torch.Tensor, n: int, offset: int = 0) -> torch.Tensor:
         """f'(restored) * up without writing the restored tensor (rtb_ckpt8_grad); up: n elements from `offset` on."""
         self._check_ckpt(codes, mags, n, up)
-        self._own(up)
         if offset < 0 or offset + n > up.numel():
             raise L.RtbError(L.ERR_BOUNDS, f"range [{offset}, {offset + n}) exceeds a buffer of {up.numel()}")
         out = self.alloc(max(n, 1), up.dtype)
@@ -527,7 +525,8 @@ class CudaB200:
             raise L.RtbError(L.ERR_BOUNDS, "the logits' rows exceed their buffer")
         if targets.dtype != torch.int64 or targets.numel() < rows or not targets.is_contiguous():
             raise L.RtbError(L.ERR_INVALID, f"cross-entropy needs {rows} dense int64 targets")
-        self._own(logits, targets)
+        self._same(logits)
+        self._same(targets)
         loss = self.alloc(1, logits.dtype)
         g = self.alloc(max(rows * classes, 1), logits.dtype) if with_grad else None
         check(lib().rtb_cross_entropy(self._ctx, dtype_code(logits), logits.data_ptr() + offset * logits.element_size(), rows, classes, pitch,

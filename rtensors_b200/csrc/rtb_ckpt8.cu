@@ -175,8 +175,9 @@ __global__ void __launch_bounds__(kThreads) ckpt8_read_kernel(const int8_t *code
         const size_t i = (block0 + u) * kCkpt8Block + lane * 4;
         const Ckpt8Scale<T> scale(m[u]);
         T out[4];
+        scale.template restore<4>(c[u], out);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) out[k] = map<T, KIND>(scale.restore(c[u], k), KIND >= 0 ? w[u][k] : (T)0);
+        for (int k = 0; k < 4; ++k) out[k] = map<T, KIND>(out[k], KIND >= 0 ? w[u][k] : (T)0);
         store4<T, VEC>(dst, i, n, out);
     }
 }

@@ -20,25 +20,36 @@ __device__ __forceinline__ double ckpt8_fma(double a, double b, double c) { retu
 // single rounded m / 127 would put up to 127 / 2 ulp on m itself).  Tiny magnitudes are scaled up and
 // the result scaled back, so that hi and lo are no subnormals.
 template <typename T> struct Ckpt8Scale {
-    T hi, lo, post;
+    T hi, lo;
+    bool small;
     __device__ __forceinline__ explicit Ckpt8Scale(T m) {
-        const T tiny = sizeof(T) == 4 ? (T)1e-30f : (T)1e-280;
         const T up = sizeof(T) == 4 ? (T)18446744073709551616.0 : (T)1.3407807929942597e154;      // 2^64, 2^512
-        const T down = sizeof(T) == 4 ? (T)5.421010862427522e-20 : (T)7.458340731200207e-155;      // 2^-64, 2^-512
-        const bool small = m < tiny;
-        m = small ? m * up : m;
-        post = small ? down : (T)1;
+        small = m < (sizeof(T) == 4 ? (T)1e-30f : (T)1e-280);
+        if (small) m = m * up;
         const T r127 = (T)(1.0 / 127.0);
         hi = m * r127;
         lo = ckpt8_fma((T)-127, hi, m) * r127;   // the residual itself is exact
     }
-    __device__ __forceinline__ T restore(T c) const { return ckpt8_fma(c, hi, c * lo) * post; }
-    __device__ __forceinline__ T restore(int8_t code) const { return restore((T)code); }
-    // code k of four packed ones.  f32: the byte becomes the low mantissa byte of 2^23, two instructions where a conversion from 8
-    // bits runs at a quarter of the rate.
-    __device__ __forceinline__ T restore(uint32_t four, int k) const {
-        if constexpr (sizeof(T) == 4) return restore((T)(__uint_as_float(__byte_perm(four ^ 0x80808080u, 0x4b000000u, 0x7540u + k)) - 8388736.0f));
-        else return restore((T)(int8_t)(four >> (8 * k)));
+    __device__ __forceinline__ T restore(int8_t code) const { return down(times((T)code)); }
+    // the first N of four packed codes.  f32: a byte becomes the low mantissa byte of 2^23, two instructions where a conversion from
+    // 8 bits runs at an eighth of the rate.
+    template <int N> __device__ __forceinline__ void restore(uint32_t four, T *out) const {
+        if constexpr (sizeof(T) == 4) four ^= 0x80808080u;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            if constexpr (sizeof(T) == 4) out[k] = times((T)(__uint_as_float(__byte_perm(four, 0x4b000000u, 0x7540u + k)) - 8388736.0f));
+            else out[k] = times((T)(int8_t)(four >> (8 * k)));
+        }
+        if (small) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) out[k] = down(out[k]);
+        }
+    }
+
+  private:
+    __device__ __forceinline__ T times(T c) const { return ckpt8_fma(c, hi, c * lo); }
+    __device__ __forceinline__ T down(T v) const {
+        return small ? v * (sizeof(T) == 4 ? (T)5.421010862427522e-20 : (T)7.458340731200207e-155) : v;   // 2^-64, 2^-512
     }
 };
 #endif

@@ -63,6 +63,9 @@ template <typename T> struct ScanArgs {
     T *dh0;                  // backward (may be null)
     int seg_shift;           // log2 of the neighbouring lanes whose share of dg is summed before it is written
     unsigned cluster;        // CTAs that share a group of lanes
+    struct Strides {
+        int64_t g, b, x, o, d;
+    } bytes, round_bytes;    // to, tg ... in bytes, and those of a whole round
 };
 
 struct LaneAt {
@@ -137,67 +140,90 @@ __global__ void __launch_bounds__(kThreads, 2) scan_lanes_kernel(const __grid_co
     const uint64_t first_lane = group * W + (uint64_t)lane * V;
     const bool active = first_lane < p.lanes;
     const LaneAt at = locate(p.dims, active ? first_lane : 0, p.seg_shift);
-    const int64_t steps = (int64_t)p.steps, round = (int64_t)nc * kWarps * kRows * R;
-    const int64_t my0 = (int64_t)((rank * kWarps + warp) * kRows + row) * R;
-    const int64_t rounds = (steps + round - 1) / round;
+    const int steps = (int)p.steps, round = (int)nc * kWarps * kRows * R;
+    const int my0 = (int)((rank * kWarps + warp) * kRows + row) * R;
+    const int rounds = (steps + round - 1) / round;
     const bool need_h = kBack && p.dg;
     grid_dep_wait();
 
-    auto slot = [&](int64_t i, int part, int row, int bytes) { return ring + (i % STAGES) * Ring::kStageBytes + part + (row * kThreads + (int)threadIdx.x) * bytes; };
-    auto issue = [&](int64_t i) {
-        const int64_t s0 = i * round + my0;
-        if (active && s0 < steps) {
-            // backward: gates one step earlier in processing order; row k of the ring is step s0 - 1 + k
+    // Addresses advance by byte strides out of the constant bank.  Backward: row k of the gate's ring is the step in front of row
+    // k's own; a kept state is the one behind it.
+    auto ptr = [&](const T *base, int64_t lane_at, int64_t t, int off) { return (const char *)(base + lane_at) + (my0 + off) * t; };
+    const char *in_g = ptr(p.g, at.g, p.bytes.g, kBack ? -1 : 0), *in_b = ptr(p.b, at.b, p.bytes.b, 0);
+    const char *in_h = MODE == kBackDense ? ptr(p.h, p.o0 + at.o, p.bytes.o, 1) : nullptr, *in_x = kBack && COUPLED ? ptr(p.x, at.x, p.bytes.x, 0) : nullptr;
+    int64_t in_c = MODE == kBackCodes ? p.o0 + at.o + (my0 + 1) * p.to : 0;   // flat position of a code
+    char *to_o = (char *)(p.out + p.o0 + at.o) + my0 * p.bytes.o;
+    char *to_d = kBack ? (char *)(p.dg + p.d0 + at.d) + my0 * p.bytes.d : nullptr;
+    const char *at_g = in_g;
+    // steps left from the thread's first of the round on: of the round that is copied, fetched, worked on
+    int left_in = active ? steps - my0 : 0, left_f = left_in, left = left_in;
+
+    auto slot = [&](int stage, int part, int k) { return ring + stage * Ring::kStageBytes + part + (k * kThreads + (int)threadIdx.x) * Ring::kVecBytes; };
+    auto issue = [&](int stage, bool start) {
+        if (left_in > 0) {
             if constexpr (GVEC) {
+                const char *q = in_g;
 #pragma unroll
-                for (int k = 0; k < Ring::kGateRows; ++k) {
-                    const int64_t s = s0 + k - (kBack ? 1 : 0);
-                    if (s >= 0 && s < steps) copy_async<Ring::kVecBytes>(slot(i, Ring::kGate, k, Ring::kVecBytes), p.g + at.g + s * p.tg);
+                for (int k = 0; k < Ring::kGateRows; ++k, q += p.bytes.g)
+                    if (k - (kBack ? 1 : 0) < left_in && !(kBack && k == 0 && start && my0 == 0)) copy_async<Ring::kVecBytes>(slot(stage, Ring::kGate, k), q);
+            }
+            const char *q = in_b;
+#pragma unroll
+            for (int r = 0; r < R; ++r, q += p.bytes.b)
+                if (r < left_in) copy_async<Ring::kVecBytes>(slot(stage, Ring::kB, r), q);
+            if constexpr (MODE == kBackDense) {
+                if (need_h) {
+                    q = in_h;
+#pragma unroll
+                    for (int r = 0; r < R; ++r, q += p.bytes.o)
+                        if (r + 1 < left_in) copy_async<Ring::kVecBytes>(slot(stage, Ring::kH, r), q);
                 }
             }
+            if constexpr (kBack && COUPLED) {
+                if (need_h) {
+                    q = in_x;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int64_t s = s0 + r;
-                if (s >= steps) break;
-                copy_async<Ring::kVecBytes>(slot(i, Ring::kB, r, Ring::kVecBytes), p.b + at.b + s * p.tb);
-                if constexpr (kBack) {
-                    if constexpr (MODE == kBackDense)
-                        if (need_h && s + 1 < steps) copy_async<Ring::kVecBytes>(slot(i, Ring::kH, r, Ring::kVecBytes), p.h + p.o0 + at.o + (s + 1) * p.to);
-                    if constexpr (COUPLED)
-                        if (need_h) copy_async<Ring::kVecBytes>(slot(i, Ring::kX, r, Ring::kVecBytes), p.x + at.x + s * p.tx);
+                    for (int r = 0; r < R; ++r, q += p.bytes.x)
+                        if (r < left_in) copy_async<Ring::kVecBytes>(slot(stage, Ring::kX, r), q);
                 }
             }
         }
         copy_commit();
+        in_b += p.round_bytes.b, left_in -= round;
+        if constexpr (GVEC) in_g += p.round_bytes.g;
+        if constexpr (MODE == kBackDense) in_h += p.round_bytes.o;
+        if constexpr (kBack && COUPLED) in_x += p.round_bytes.x;
     };
     // the narrow operands of a round, loaded while the one before it is worked on
     T gate_now[GVEC ? 1 : Ring::kGateRows] = {}, gate_next[GVEC ? 1 : Ring::kGateRows];
     uint32_t code_now[MODE == kBackCodes ? R : 1] = {}, code_next[MODE == kBackCodes ? R : 1];
     T mag_now[MODE == kBackCodes ? R : 1] = {}, mag_next[MODE == kBackCodes ? R : 1];
-    auto fetch = [&](int64_t i) {
-        const int64_t s0 = i * round + my0;
+    auto fetch = [&](bool start) {
         if constexpr (!GVEC) {
+            const char *q = at_g;
 #pragma unroll
-            for (int k = 0; k < Ring::kGateRows; ++k) {
-                const int64_t s = s0 + k - (kBack ? 1 : 0);
-                gate_next[k] = active && s >= 0 && s < steps ? p.g[at.g + s * p.tg] : (T)1;
+            for (int k = 0; k < Ring::kGateRows; ++k, q += p.bytes.g) {
+                gate_next[k] = (T)1;
+                if (k - (kBack ? 1 : 0) < left_f && !(kBack && k == 0 && start && my0 == 0)) gate_next[k] = *(const T *)q;
             }
+            at_g += p.round_bytes.g;
         }
         if constexpr (MODE == kBackCodes) {
+            int64_t flat = in_c;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int64_t s = s0 + r;
+            for (int r = 0; r < R; ++r, flat += p.to) {
                 code_next[r] = 0, mag_next[r] = (T)0;
-                if (need_h && active && s + 1 < steps) {
-                    const int64_t flat = p.o0 + at.o + (s + 1) * p.to;
+                if (need_h && r + 1 < left_f) {
                     code_next[r] = codes_at<V>(p.codes + flat);
                     mag_next[r] = p.mags[flat >> kCkpt8Shift];   // V divides the block: one magnitude
                 }
             }
+            in_c += p.round_bytes.o / (int)sizeof(T);
         }
+        left_f -= round;
     };
-    auto gate_of = [&](int64_t i, int k) {
-        if constexpr (GVEC) return ld<T, VA>((const T *)slot(i, Ring::kGate, k, Ring::kVecBytes));
+    auto gate_of = [&](int stage, int k) {
+        if constexpr (GVEC) return ld<T, VA>((const T *)slot(stage, Ring::kGate, k));
         else return PA{{gate_now[k]}};
     };
     auto of = [](const PA &v, int j) { return v.e[GVEC ? j : 0]; };
@@ -206,16 +232,17 @@ __global__ void __launch_bounds__(kThreads, 2) scan_lanes_kernel(const __grid_co
 #pragma unroll
     for (int j = 0; j < V; ++j) carry.e[j] = !kBack && p.h0 && active ? p.h0[first_lane + j] : (T)0;
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue(i);
-    fetch(0);
+    for (int i = 0; i < STAGES - 1; ++i) issue(i, i == 0);
+    fetch(true);
     if (nc > 1) {
         if (threadIdx.x == 0) mbar_init(&arrived[0]), mbar_init(&arrived[1]);
         cluster_barrier();   // every CTA runs, its barriers are set, before any is written to
     }
     bool lost = false;
 
-    for (int64_t i = 0; i < rounds; ++i) {
-        issue(i + STAGES - 1);
+    int stage = 0;
+    for (int i = 0; i < rounds; ++i) {
+        issue(stage == 0 ? STAGES - 1 : stage - 1, false);
         if constexpr (!GVEC) {
 #pragma unroll
             for (int k = 0; k < Ring::kGateRows; ++k) gate_now[k] = gate_next[k];
@@ -224,22 +251,20 @@ __global__ void __launch_bounds__(kThreads, 2) scan_lanes_kernel(const __grid_co
 #pragma unroll
             for (int r = 0; r < R; ++r) code_now[r] = code_next[r], mag_now[r] = mag_next[r];
         }
-        if constexpr (!GVEC || MODE == kBackCodes) fetch(i + 1);
+        if constexpr (!GVEC || MODE == kBackCodes) fetch(false);
         copy_wait<STAGES - 1>();
-        const int64_t s0 = i * round + my0;
+        const bool at_start = kBack && i == 0 && my0 == 0;   // in front of the first step there is no gate
         PA a[R];
         P b[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int64_t s = s0 + r;
-            if (active && s < steps) {
-                if (kBack && s == 0) {
+            if (r < left) {
+                a[r] = gate_of(stage, r);
+                if (r == 0 && at_start) {
 #pragma unroll
                     for (int j = 0; j < VA; ++j) a[r].e[j] = (T)0;
-                } else {
-                    a[r] = gate_of(i, r);
                 }
-                b[r] = ld<T, V>((const T *)slot(i, Ring::kB, r, Ring::kVecBytes));
+                b[r] = ld<T, V>((const T *)slot(stage, Ring::kB, r));
                 if constexpr (!kBack && COUPLED) {
 #pragma unroll
                     for (int j = 0; j < V; ++j) b[r].e[j] = ((T)1 - of(a[r], j)) * b[r].e[j];
@@ -291,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_lanes_kernel(const __grid_co
                 if (row == 0) ex_h.e[j] = (T)0;
             }
         }
-        const int buf = (int)(i & 1);   // a warp is never a whole round ahead of another: two buffers suffice
+        const int buf = i & 1;   // a warp is never a whole round ahead of another: two buffers suffice
         if (row == kRows - 1) {
             st<T, VA>(&warp_a[buf][warp][lane * VA], A);
             st<T, V>(&warp_h[buf][warp][lane * V], H);
@@ -354,24 +379,23 @@ __global__ void __launch_bounds__(kThreads, 2) scan_lanes_kernel(const __grid_co
         for (int r = 0; r < R; ++r) {
 #pragma unroll
             for (int j = 0; j < V; ++j) b[r].e[j] = c.e[j] = fma_(of(a[r], j), c.e[j], b[r].e[j]);
-            const int64_t s = s0 + r;
-            if (!active || s >= steps) continue;
-            const int64_t o = p.o0 + at.o + s * p.to;
+            if (r >= left) continue;
+            T *const o = (T *)(to_o + r * p.bytes.o);
             if constexpr (!kBack) {
-                st<T, V>(p.out + o, c);
+                st<T, V>(o, c);
             } else {
                 if (p.out) {
                     P d = c;
                     if constexpr (COUPLED) {
-                        const PA now = gate_of(i, r + 1);
+                        const PA now = gate_of(stage, r + 1);
 #pragma unroll
                         for (int j = 0; j < V; ++j) d.e[j] = ((T)1 - of(now, j)) * c.e[j];
                     }
-                    st<T, V>(p.out + o, d);
+                    st<T, V>(o, d);
                 }
-                if (p.dh0 && s + 1 == steps) {
+                if (r + 1 == left && p.dh0) {
 #pragma unroll
-                    for (int j = 0; j < V; ++j) p.dh0[first_lane + j] = p.g[at.g + j * (GVEC ? 1 : 0) + s * p.tg] * c.e[j];
+                    for (int j = 0; j < V; ++j) p.dh0[first_lane + j] = p.g[at.g + j * (GVEC ? 1 : 0) + (int64_t)(steps - 1) * p.tg] * c.e[j];
                 }
             }
         }
@@ -379,32 +403,26 @@ __global__ void __launch_bounds__(kThreads, 2) scan_lanes_kernel(const __grid_co
             if (need_h) {
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    const int64_t s = s0 + r;
                     P d;
-                    if (active && s + 1 == steps) {
+                    if constexpr (MODE == kBackDense) d = ld<T, V>((const T *)slot(stage, Ring::kH, r));
+                    else Ckpt8Scale<T>(mag_now[r]).template restore<V>(code_now[r], d.e);
+                    if (r + 1 == left) {   // the last step: the state in front of the first one
 #pragma unroll
                         for (int j = 0; j < V; ++j) d.e[j] = p.h0 ? p.h0[first_lane + j] : (T)0;
-                    } else if constexpr (MODE == kBackDense) {
-                        d = ld<T, V>((const T *)slot(i, Ring::kH, r, Ring::kVecBytes));
-                    } else {
-                        const Ckpt8Scale<T> scale(mag_now[r]);
-#pragma unroll
-                        for (int j = 0; j < V; ++j) d.e[j] = scale.restore(code_now[r], j);
                     }
                     if constexpr (COUPLED) {
-                        const P x = ld<T, V>((const T *)slot(i, Ring::kX, r, Ring::kVecBytes));
+                        const P x = ld<T, V>((const T *)slot(stage, Ring::kX, r));
 #pragma unroll
                         for (int j = 0; j < V; ++j) d.e[j] = d.e[j] - x.e[j];
                     }
                     // behind the axis, and in idle threads, the ring holds nothing: what is there must not count
-                    const bool here = active && s < steps;
 #pragma unroll
-                    for (int j = 0; j < V; ++j) b[r].e[j] = here ? b[r].e[j] * d.e[j] : (T)0;
+                    for (int j = 0; j < V; ++j) b[r].e[j] = r < left ? b[r].e[j] * d.e[j] : (T)0;
                 }
                 if (p.seg_shift == 0) {
 #pragma unroll
                     for (int r = 0; r < R; ++r)
-                        if (active && s0 + r < steps) st<T, V>(p.dg + p.d0 + at.d + (s0 + r) * p.td, b[r]);
+                        if (r < left) st<T, V>((T *)(to_d + r * p.bytes.d), b[r]);
                 } else {
                     // a segment is a power of two of lanes, at least V, and whole within a row of the group
                     T sum[R];
@@ -420,14 +438,17 @@ __global__ void __launch_bounds__(kThreads, 2) scan_lanes_kernel(const __grid_co
 #pragma unroll
                             for (int r = 0; r < R; ++r) sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], m);
                         }
-                    if (active && ((lane * V) & ((1 << p.seg_shift) - 1)) == 0) {
+                    if (((lane * V) & ((1 << p.seg_shift) - 1)) == 0) {
 #pragma unroll
                         for (int r = 0; r < R; ++r)
-                            if (s0 + r < steps) p.dg[p.d0 + at.d + (s0 + r) * p.td] = sum[r];
+                            if (r < left) *(T *)(to_d + r * p.bytes.d) = sum[r];
                     }
                 }
             }
+            to_d += p.round_bytes.d;
         }
+        to_o += p.round_bytes.o, left -= round;
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
     grid_dep_launch();               // late: CTAs of the next kernel that wait beside a long loop slow it down
     if (nc > 1) cluster_barrier();   // no CTA leaves while another may still write to it
@@ -533,9 +554,10 @@ __global__ void __launch_bounds__(kThreads, 2) scan_axis_kernel(const __grid_con
             if (s < steps) {
                 const int64_t flat = p.o0 + at.o + (p.to > 0 ? s : -s - (V - 1));   // V aligned codes: one magnitude
                 const uint32_t c = codes_at<V>(p.codes + flat);
-                const Ckpt8Scale<T> scale(p.mags[flat >> kCkpt8Shift]);
+                P w;
+                Ckpt8Scale<T>(p.mags[flat >> kCkpt8Shift]).template restore<V>(c, w.e);
 #pragma unroll
-                for (int j = 0; j < V; ++j) v.e[j] = scale.restore(c, p.to > 0 ? j : V - 1 - j);
+                for (int j = 0; j < V; ++j) v.e[j] = w.e[p.to > 0 ? j : V - 1 - j];
             }
         } else {
 #pragma unroll
@@ -831,6 +853,9 @@ template <typename T, int V, int LX, int R, int STAGES, int MODE, bool COUPLED, 
         return (size_t)STAGES * LanesRing<T, V, R, MODE, COUPLED, GVEC>::kStageBytes + (cluster > 1 ? (size_t)cluster * 2 * (W + (GVEC ? W : LX)) * sizeof(T) : 0);
     };
     if (int rc = cluster_for<T, kernel>(ctx, groups, p.steps, part, smem, &p.cluster)) return rc;
+    const int64_t es = sizeof(T), n = (int64_t)(p.cluster * part) * es;
+    p.bytes = {p.tg * es, p.tb * es, p.tx * es, p.to * es, p.td * es};
+    p.round_bytes = {p.tg * n, p.tb * n, p.tx * n, p.to * n, p.td * n};
     return launch_cluster<ScanArgs<T>, kernel>(ctx, "scan_lanes_kernel", groups * p.cluster, kThreads, p.cluster, smem(p.cluster),
                                                p.lanes * p.steps <= kShortElements, p);
 }
@@ -842,12 +867,19 @@ template <typename T, int V> int side_by_side(const Ctx *ctx, const ScanArgs<T> 
     return (p.lanes + 8 * V - 1) / (8 * V) * kMaxCluster * 2 <= (uint64_t)ctx->sm_count ? 4 : 8;
 }
 
-// Four steps of a thread and two stages of the ring: two CTAs fit an SM in clusters of any size (the coupled backward pass
-// has one operand more and takes three).  Two steps with more stages, eight with one CTA on an SM, 512 threads and three CTAs on
-// an SM were all slower, by 5 to 60 %.
+// Steps of a thread, with two stages of the ring.  More steps make fewer rounds, each of which costs the same exchange, and take
+// more registers and shared memory (beyond 104 KB one CTA fits an SM, not two).  us at 65536 x 1024 and, behind the slash,
+// 8 x 8192 x 1024, f32, per channel or with one gate for 64 or 128 channels:
+//   forward, per channel     4: 173 / 141   6: 150 / 151   8: 156 / 147        shared   4: 210 / 148   6: 172 / 126   8: 146 / 114
+//   backward, dense          4: 239 / 263   6: 246 / 236   8: 265 / 251        shared   4: 187 / 156   6: 170 / 155   8: 201 / 187
+//   backward from codes      4: 246 / 207   6: 299 / 282                       shared   4: 191 / 160   6: 175 / 150   8: 192 / 175
+//   backward, coupled        3: 308 / 262   4: 325 / 305   6: 307 / 283        shared   3: 244 / 203   4: 225 / 195   6: 247 / 230
 template <typename T, int V, int MODE, bool COUPLED, bool GVEC> int run_lanes(Ctx *ctx, ScanArgs<T> &p) {
-    constexpr int R = MODE != kForward && COUPLED ? 3 : 4;
+    constexpr bool back = MODE != kForward;
+    constexpr int R = GVEC ? (back ? (COUPLED ? 3 : MODE == kBackDense ? 6 : 4) : 6) : (back ? (COUPLED ? 4 : 6) : 8);
     if (side_by_side<T, V>(ctx, p) == 4) return run_width<T, V, 4, R, 2, MODE, COUPLED, GVEC>(ctx, p);
+    if constexpr (!back && GVEC)   // many lanes: no clusters, the exchange is cheap
+        if (p.lanes >= (uint64_t)ctx->sm_count * 8 * V) return run_width<T, V, 8, 4, 2, MODE, COUPLED, GVEC>(ctx, p);
     return run_width<T, V, 8, R, 2, MODE, COUPLED, GVEC>(ctx, p);
 }
 
@@ -946,6 +978,8 @@ int check_scan(rtb_ctx *c, int dtype, int flags, size_t rank, const size_t *shap
     if (rank > RTB_MAX_RANK) return fail(RTB_ERR_DIM, "rank %zu exceeds %d", rank, RTB_MAX_RANK);
     if (rank && !shape) return fail(RTB_ERR_INVALID, "null shape");
     if (axis >= rank) return fail(RTB_ERR_DIM, "axis %zu out of range for rank %zu", axis, rank);
+    // steps are counted in 32 bits inside the kernels, a round (at most 2^16 steps) beyond the last one included
+    if (shape[axis] > 0x7fff0000u) return fail(RTB_ERR_TOO_LARGE, "gated scan: %zu steps, 2^31 - 2^16 is the limit", shape[axis]);
     return RTB_OK;
 }
 

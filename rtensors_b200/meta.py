@@ -18,7 +18,7 @@ class Meta:
 
     @staticmethod
     def contiguous(shape: Sequence[int]) -> "Meta":
-        return _contiguous(tuple(int(s) for s in shape))
+        return _contiguous(shape if type(shape) is tuple else tuple(shape))
 
     @property
     def rank(self) -> int:
@@ -33,7 +33,7 @@ class Meta:
     def c_strides(self):
         return diffs(self.strides)
 
-    @property
+    @cached_property
     def size(self) -> int:
         n = 1
         for s in self.shape:
@@ -104,6 +104,7 @@ class Meta:
 
 @lru_cache(maxsize=4096)
 def _contiguous(shape: Tuple[int, ...]) -> Meta:
+    shape = tuple(int(s) for s in shape)
     out = (C.c_ssize_t * max(len(shape), 1))()
     lib().rtb_meta_contiguous_strides(C.c_size_t(len(shape)), sizes(shape), out)
     return Meta(shape, tuple(out[: len(shape)]), 0)

@@ -312,7 +312,7 @@ class Tensor:
         if meta.shape == self.meta.shape:
             return meta
         shape, _, strides = broadcast_params(self.meta, meta)
-        if shape != tuple(self.shape):
+        if shape != self.meta.shape:
             raise L.RtbError(L.ERR_BROADCAST, f"{what} of shape {meta.shape} does not broadcast to {self.shape}")
         return Meta(shape, strides, meta.offset)
 
@@ -338,7 +338,7 @@ class Tensor:
         """The tensor in 8 bits an element (see Checkpoint8), in row-major order of its shape."""
         c = _dense(self)
         codes, mags = self.backend.ckpt8_store(c.buf, c.size, c.offset)
-        return Checkpoint8(self.backend, codes, mags, tuple(self.shape))
+        return Checkpoint8(self.backend, codes, mags, self.meta.shape)
 
 
 class Checkpoint8:
@@ -387,9 +387,9 @@ def _dense(t: Tensor, force: bool = False) -> Tensor:
 
 def _scan_operands(x, axis: int, gate: Tensor, h0: Optional[Tensor]):
     """-> (gate, its meta over x's shape, h0 dense from the start of its buffer)."""
-    if not 0 <= axis < x.rank:
+    if not 0 <= axis < len(x.meta.shape):
         raise L.RtbError(L.ERR_DIM, f"axis {axis} out of range for rank {x.rank}")
-    if any(st == 0 and n != 1 for st, n in zip(gate.strides, gate.shape)):
+    if 0 in gate.meta.strides and any(st == 0 and n != 1 for st, n in zip(gate.strides, gate.shape)):
         gate = _dense(gate, force=True)     # a stride of 0 marks the dims that broadcasting adds
     gm = x._spread(gate.meta, "the gate")
     if h0 is not None:
