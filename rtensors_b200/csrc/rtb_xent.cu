@@ -6,11 +6,12 @@
 // A row is read once: its logits stay in registers as exp(x - m) for a maximum m of the thread's own, (m, sum) pairs are merged
 // over the threads of the row, and the map is what is in the registers times one factor.  HBM-bound: 4 bytes read
 // and 4 written per element in f32.
-//   up to 64 classes      8 threads share a row, four rows a warp
-//   up to 4 KB a row      a warp
-//   up to 512 KB a row    a CTA, or a cluster of up to 8 that exchange their pairs through shared memory; rows are copied ahead
-//                         into a ring of stages
+//   up to 16 classes      a thread for each row
+//   up to 4 KB a row      4 to 32 threads of a warp
+//   up to 1 MB a row      a CTA of up to 512 threads, 256 bytes of the row in each; beyond 128 KB a cluster of up to 8 CTAs that exchange
+//                         their pairs through shared memory
 //   beyond                a CTA reads the row twice (the second time mostly from L2)
+// A CTA copies the rows ahead into shared memory, vector by vector as it takes a row's vectors from there into registers.
 //
 // A row with t < 0 does not count (padding): its map is zero and its logits are not read.  t >= classes gives NaN for the row
 // and the loss.  Rows are dealt out statically and every sum has a fixed order: results are deterministic.
@@ -269,11 +270,15 @@ __global__ void __launch_bounds__(256) xent_warp_kernel(const __grid_constant__ 
     finish_loss<T, 256>(p, mine);
 }
 
-// ---- a CTA, or each CTA of a cluster, holds a slice of THREADS * NV packs of N ----------------------------------
-template <typename T, int THREADS, int NV, int N, int STAGES>
+// ---- a CTA, or each CTA of a cluster, holds THREADS * NV vectors of 16 bytes of a row ----------------------------
+// Vectors lie at 16-byte boundaries of the logits; where a row starts in the middle of one (an odd number of classes), its first
+// and last vectors are partly the row's.
+// AHEAD rows are in shared memory or on their way; a row's vectors are taken, and replaced, in kGroups parts, so that copies never
+// all wait for the last of a row.
+template <typename T, int THREADS, int NV, int AHEAD>
 __global__ void __launch_bounds__(THREADS, 512 / THREADS) xent_cta_kernel(const __grid_constant__ XentArgs<T> p) {
-    constexpr int kWarps = THREADS / 32;
-    extern __shared__ __align__(16) unsigned char ring[];   // [stage][pack][thread]: a thread copies what it reads itself
+    constexpr int kWarps = THREADS / 32, N = Vec<T>::N, kGroups = 4, kGroup = NV / kGroups;
+    extern __shared__ __align__(16) unsigned char ring[];   // [row ahead][vector][thread]: a thread copies what it reads itself
     __shared__ alignas(16) Lse<T> pairs[2][kMaxCluster * kWarps];
     __shared__ unsigned long long arrived[2];
     __shared__ unsigned long long sn[kWarps];
@@ -281,28 +286,44 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) xent_cta_kernel(const 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned nc = p.cluster, rank = nc > 1 ? cluster_rank() : 0;
     const size_t stride = gridDim.x / nc;
-    const size_t slice = (size_t)THREADS * NV * N, j0 = rank * slice;   // of the row
     const size_t row0 = blockIdx.x / nc;
+    const int classes = (int)p.classes;
     grid_dep_wait();
     const T inv_n = map_factor<T, THREADS>(p, sn);
     auto target_of = [&](size_t r) { return r < p.rows ? p.targets[r] : (int64_t)-1; };
-    auto slot = [&](int stage, int k) { return reinterpret_cast<P *>(ring) + (stage * NV + k) * THREADS + threadIdx.x; };
-    auto issue = [&](size_t r, int stage, int64_t t) {
+    auto slot = [&](int ahead, int k) { return reinterpret_cast<P *>(ring) + (ahead * NV + k) * THREADS + threadIdx.x; };
+    auto row_at = [&](size_t r) { return p.logits + (int64_t)r * p.pitch; };
+    // elements of the row's first vector that lie in front of the row
+    auto phase_of = [&](const T *x) { return (int)(((uintptr_t)x & 15u) / sizeof(T)); };
+    // the class of vector k's first element: below zero, or the vector beyond `classes`, at the row's ends
+    auto class_of = [&](int k, int phase) { return ((int)(rank * NV + k) * THREADS + (int)threadIdx.x) * N - phase; };
+    auto copy_group = [&](size_t r, int64_t t, int ahead, int group) {
         if (t >= 0) {
-            const T *x = p.logits + (int64_t)r * p.pitch;
+            const T *x = row_at(r);
+            const int phase = phase_of(x);
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const size_t j = j0 + (size_t)(k * THREADS + threadIdx.x) * N;
-                if (j < p.classes) copy_async<sizeof(P)>(slot(stage, k), x + j);
+            for (int k = group * kGroup; k < (group + 1) * kGroup; ++k) {
+                const int j = class_of(k, phase);
+                if (j >= classes) continue;
+                if (j >= 0) {
+                    copy_async_16(slot(ahead, k), x + j, j + N <= classes ? 16 : (unsigned)(classes - j) * (unsigned)sizeof(T));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (j + i >= 0 && j + i < classes) copy_async<sizeof(T)>(&slot(ahead, k)->e[i], x + j + i);
+                }
             }
         }
         copy_commit();
     };
-    int64_t t[STAGES];   // targets of the rows in the ring, t[0] of the one that is worked on
+    int64_t t_of[AHEAD + 1];   // targets of this row and of those ahead
 #pragma unroll
-    for (int i = 0; i < STAGES; ++i) t[i] = target_of(row0 + i * stride);
+    for (int a = 0; a <= AHEAD; ++a) t_of[a] = target_of(row0 + a * stride);
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue(row0 + i * stride, i, t[i]);
+    for (int a = 0; a < AHEAD; ++a)
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g) copy_group(row0 + a * stride, t_of[a], a, g);
+    int ahead = 0;
     if (nc > 1) {
         if (threadIdx.x == 0) mbar_init(&arrived[0]), mbar_init(&arrived[1]);
         cluster_barrier();   // every CTA runs, its barriers are set, before any is written to
@@ -310,39 +331,44 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) xent_cta_kernel(const 
     bool lost = false;
     XentPartial mine{0.0, 0};
     unsigned counted = 0;    // rows worked on: which buffer, which phase
-    int stage = 0;
     for (size_t r = row0; r < p.rows; r += stride) {
-        const int64_t far = target_of(r + STAGES * stride);
-        issue(r + (STAGES - 1) * stride, stage == 0 ? STAGES - 1 : stage - 1, t[STAGES - 1]);
-        copy_wait<STAGES - 1>();
-        const int64_t tr = t[0];
-        if (tr < 0) {
-            if (p.map) {
+        const int64_t t_far = target_of(r + (AHEAD + 1) * stride), t = t_of[0];
+        const int phase = t < 0 ? 0 : phase_of(row_at(r));
+        T e[NV * N];
+        T xt = (T)0;          // the target's logit, in the thread that holds it: the map may take the logits' place
+        bool mine_t = false;
+        const bool bad = t >= (int64_t)classes, first = rank == 0 && threadIdx.x == 0;
+        const int tt = bad ? -N : (int)t;   // no class in any vector where the target is beyond them
 #pragma unroll
-                for (int k = 0; k < NV; ++k) {
-                    const size_t j = j0 + (size_t)(k * THREADS + threadIdx.x) * N;
-                    if (j < p.classes) st<T, N>(p.map + r * p.classes + j, P{});
-                }
-            }
-        } else {
-            const bool bad = (uint64_t)tr >= p.classes, first = rank == 0 && threadIdx.x == 0;
-            T xt = (T)0;          // the target's logit, in the thread that holds it: the map may take the logits' place
-            bool mine_t = false;
-            T e[NV * N];
+        for (int group = 0; group < kGroups; ++group) {
+            copy_wait<AHEAD * kGroups - 1>();
+            if (t >= 0) {
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const size_t j = j0 + (size_t)(k * THREADS + threadIdx.x) * N;
-                P q;
-                if (j < p.classes) q = *slot(stage, k);
+                for (int k = group * kGroup; k < (group + 1) * kGroup; ++k) {
+                    const int j = class_of(k, phase);
+                    P q;
+                    if (j < classes) q = *slot(ahead, k);
 #pragma unroll
-                for (int i = 0; i < N; ++i) e[k * N + i] = j < p.classes ? q.e[i] : lowest<T>();
-                if (j / N == (size_t)tr / N && j < p.classes) {
-                    mine_t = true;
+                    for (int i = 0; i < N; ++i) e[k * N + i] = j < classes ? q.e[i] : lowest<T>();
+                    if (j < 0 || j + N > classes) {
+#pragma unroll
+                        for (int i = 0; i < N; ++i)
+                            if (j + i < 0 || j + i >= classes) e[k * N + i] = lowest<T>();
+                    }
 #pragma unroll
                     for (int i = 0; i < N; ++i)
-                        if (j + i == (size_t)tr) xt = e[k * N + i];
+                        if (j + i == tt) xt = e[k * N + i], mine_t = true;
                 }
             }
+            copy_group(r + AHEAD * stride, t_of[AHEAD], ahead, group);
+        }
+        if (t < 0) {
+            if (p.map) {
+                T *g = p.map + r * p.classes;
+                for (int j = (int)(rank * NV * THREADS * N + threadIdx.x), k = 0; k < NV * N; ++k, j += THREADS)
+                    if (j < classes) g[j] = (T)0;
+            }
+        } else {
             const Lse<T> own = exponentials(e);
             Lse<T> l{warp_max(own.m), (T)0};
             l.s = own.s * own.factor(l.m);
@@ -371,28 +397,33 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) xent_cta_kernel(const 
             if (first) mine.rows += 1;
             if (p.map) {
                 T *g = p.map + r * p.classes;
+                const bool whole = ((uintptr_t)(g - phase) & 15u) == 0;   // the map's vectors lie as the logits' do
                 const T inv_s = bad ? nan_<T>() : (T)1 / sum;
                 const T to_p = own.factor(m) * inv_s, to_map = to_p * inv_n;
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
-                    const size_t j = j0 + (size_t)(k * THREADS + threadIdx.x) * N;
-                    if (j >= p.classes) continue;
+                    const int j = class_of(k, phase);
+                    if (j >= classes) continue;
                     P q;
 #pragma unroll
                     for (int i = 0; i < N; ++i) q.e[i] = e[k * N + i] * to_map;
-                    if (j / N == (size_t)tr / N) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if (j + i == tt) q.e[i] = (e[k * N + i] * to_p - (T)1) * inv_n;
+                    if (whole && j >= 0 && j + N <= classes) {
+                        st<T, N>(g + j, q);
+                    } else {
 #pragma unroll
                         for (int i = 0; i < N; ++i)
-                            if (j + i == (size_t)tr) q.e[i] = (e[k * N + i] * to_p - (T)1) * inv_n;
+                            if (j + i >= 0 && j + i < classes) g[j + i] = q.e[i];
                     }
-                    st<T, N>(g + j, q);
                 }
             }
         }
 #pragma unroll
-        for (int i = 0; i + 1 < STAGES; ++i) t[i] = t[i + 1];
-        t[STAGES - 1] = far;
-        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        for (int a = 0; a < AHEAD; ++a) t_of[a] = t_of[a + 1];
+        t_of[AHEAD] = t_far;
+        ahead = ahead + 1 == AHEAD ? 0 : ahead + 1;
     }
     grid_dep_launch();
     if (nc > 1) cluster_barrier();   // no CTA leaves while another may still write to it
@@ -462,7 +493,8 @@ template <typename T, void (*kernel)(XentArgs<T>)> int run(Ctx *ctx, const char 
         if (int rc = check_launch(ctx, "xent_count_kernel")) return rc;
         p.counts = counts;
     }
-    return launch_cluster<XentArgs<T>, kernel>(ctx, name, grid, threads, p.cluster, smem, true, p);
+    // behind the tiny count, or short itself: it may start early
+    return launch_cluster<XentArgs<T>, kernel>(ctx, name, grid, threads, p.cluster, smem, p.counts || p.rows * p.classes <= (size_t(1) << 24), p);
 }
 
 template <typename T, int TPR, int NV, int N> int run_warp(Ctx *ctx, XentArgs<T> &p) {
@@ -471,38 +503,50 @@ template <typename T, int TPR, int NV, int N> int run_warp(Ctx *ctx, XentArgs<T>
     return run<T, xent_warp_kernel<T, TPR, NV, N>>(ctx, "xent_warp_kernel", p, grid, 256, 0);
 }
 
-template <typename T, int THREADS, int N> int run_cta(Ctx *ctx, XentArgs<T> &p, unsigned cluster) {
-    constexpr int NV = 128 / (N * (int)sizeof(T)), STAGES = 3;   // 128 bytes of a row in each thread
-    constexpr size_t smem = (size_t)STAGES * THREADS * 128;
+template <typename T, int THREADS, int NV, int AHEAD> int run_cta(Ctx *ctx, XentArgs<T> &p, unsigned cluster) {
+    constexpr size_t smem = (size_t)AHEAD * THREADS * NV * 16;
     p.cluster = cluster;
     // as many clusters as run at once (a CTA of 512 threads fills an SM, four of 128 do), the rows dealt out among them
     unsigned fit = 0;
-    if (int rc = clusters_at_once<XentArgs<T>, xent_cta_kernel<T, THREADS, NV, N, STAGES>>(ctx, THREADS, cluster, smem, &fit)) return rc;
+    if (int rc = clusters_at_once<XentArgs<T>, xent_cta_kernel<T, THREADS, NV, AHEAD>>(ctx, THREADS, cluster, smem, &fit)) return rc;
     const size_t clusters = std::max<size_t>(1, std::min<size_t>(p.rows, fit));
-    return run<T, xent_cta_kernel<T, THREADS, NV, N, STAGES>>(ctx, "xent_cta_kernel", p, clusters * cluster, THREADS, smem);
+    return run<T, xent_cta_kernel<T, THREADS, NV, AHEAD>>(ctx, "xent_cta_kernel", p, clusters * cluster, THREADS, smem);
 }
 
-template <typename T, int N> int pick_size(Ctx *ctx, XentArgs<T> &p) {
-    const size_t bytes = p.classes * sizeof(T);
-    if (p.classes <= 64) return run_warp<T, 8, 8, 1>(ctx, p);
-    if (bytes <= 1024) return run_warp<T, 32, 32 / (N * (int)sizeof(T)), N>(ctx, p);
-    if (bytes <= 4096) return run_warp<T, 32, 128 / (N * (int)sizeof(T)), N>(ctx, p);
-    if (bytes <= 128 * 128) return run_cta<T, 128, N>(ctx, p, 1);
+template <typename T> int pick_size(Ctx *ctx, XentArgs<T> &p, bool vec) {
+    constexpr int N = Vec<T>::N;
+    const size_t n = p.classes, bytes = n * sizeof(T);
+    if (n <= 16) return run_warp<T, 1, 16, 1>(ctx, p);
+    if (vec) {
+        if (n <= 64) return run_warp<T, 4, 16 / N, N>(ctx, p);
+        if (n <= 128) return run_warp<T, 8, 16 / N, N>(ctx, p);
+        if (n <= 256) return run_warp<T, 16, 16 / N, N>(ctx, p);
+        if (bytes <= 4096) return run_warp<T, 32, 8, N>(ctx, p);
+    } else {
+        if (n <= 64) return run_warp<T, 8, 8, 1>(ctx, p);
+        if (n <= 256) return run_warp<T, 32, 8, 1>(ctx, p);
+        if (bytes <= 4096) return run_warp<T, 32, 128 / (int)sizeof(T), 1>(ctx, p);
+    }
+    const size_t room = bytes + 16;   // a row that starts inside a vector takes one more
+    if (room <= 128 * 8 * 16) return run_cta<T, 128, 8, 3>(ctx, p, 1);
+    if (room <= 128 * 16 * 16) return run_cta<T, 128, 16, 1>(ctx, p, 1);
+    if (room <= 256 * 16 * 16) return run_cta<T, 256, 16, 1>(ctx, p, 1);
     for (unsigned cluster = 1; cluster <= kMaxCluster; cluster *= 2)
-        if (bytes <= (size_t)cluster * 512 * 128) return run_cta<T, 512, N>(ctx, p, cluster);
+        if (room <= (size_t)cluster * 512 * 16 * 16) return run_cta<T, 512, 16, 1>(ctx, p, cluster);
     const size_t grid = std::min<size_t>(p.rows, (size_t)ctx->sm_count * 4);
-    return run<T, xent_twice_kernel<T, N>>(ctx, "xent_twice_kernel", p, grid, 512, 0);
+    if (vec) return run<T, xent_twice_kernel<T, N>>(ctx, "xent_twice_kernel", p, grid, 512, 0);
+    return run<T, xent_twice_kernel<T, 1>>(ctx, "xent_twice_kernel", p, grid, 512, 0);
 }
 
 template <typename T>
 int pick(Ctx *ctx, const T *logits, size_t rows, size_t classes, int64_t pitch, const int64_t *targets, int mean, T *loss, T *map) {
-    constexpr int N = Vec<T>::N;
+    constexpr size_t N = Vec<T>::N;
     std::lock_guard<std::mutex> lock(ctx->ws_mu);
     XentArgs<T> p{};
     p.logits = logits, p.rows = rows, p.classes = classes, p.pitch = pitch, p.targets = targets, p.mean = mean, p.loss = loss, p.map = map;
     p.cluster = 1;
-    const bool vec = classes % N == 0 && pitch % N == 0 && (((uintptr_t)logits | (uintptr_t)map) & 15u) == 0;
-    return vec ? pick_size<T, N>(ctx, p) : pick_size<T, 1>(ctx, p);
+    const bool vec = classes % N == 0 && pitch % (int64_t)N == 0 && (((uintptr_t)logits | (uintptr_t)map) & 15u) == 0;
+    return pick_size<T>(ctx, p, vec);
 }
 
 }  // namespace
