@@ -8,7 +8,7 @@
 // and 4 written per element in f32.
 //   up to 16 classes      a thread for each row
 //   up to 4 KB a row      4 to 32 threads of a warp
-//   up to 1 MB a row      a CTA of up to 512 threads, 256 bytes of the row in each; beyond 128 KB a cluster of up to 8 CTAs that exchange
+//   up to 1 MB a row      a CTA of up to 1024 threads, 128 bytes of the row in each; beyond 128 KB a cluster of up to 8 CTAs that exchange
 //                         their pairs through shared memory
 //   beyond                a CTA reads the row twice (the second time mostly from L2)
 // A CTA copies the rows ahead into shared memory, vector by vector as it takes a row's vectors from there into registers.
@@ -37,13 +37,6 @@ __device__ __forceinline__ float log_(float x) { return logf(x); }
 __device__ __forceinline__ double log_(double x) { return log(x); }
 __device__ __forceinline__ float max_(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double max_(double a, double b) { return fmax(a, b); }
-// exp for the bulk: 2^(x log2 e), the argument rounded once more, off by (|x| + 2) 2^-23 of the result at most
-__device__ __forceinline__ float fast_exp(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
-    return y;
-}
-__device__ __forceinline__ double fast_exp(double x) { return exp(x); }
 template <typename T> __device__ __forceinline__ T lowest() { return -(T)INFINITY; }
 template <typename T> __device__ __forceinline__ T nan_() { return (T)NAN; }
 
@@ -58,45 +51,63 @@ __device__ __forceinline__ double warp_max(double v) {
     return v;
 }
 
-// (maximum m, sum of exp(x - m)) of some logits.  Entries of -inf add nothing and keep a maximum of -inf harmless; a NaN is
-// skipped by the maximum and kept by the sum.
+// Sums of exponentials are kept relative to a shift c: s = sum of exp(x) / e^c.  f64: c is a maximum of the logits.  f32: powers of
+// two, c = rint(m log2 e) and s = sum of 2^(x log2 e - c): one fused multiply-add rounds each exponent once, and bringing
+// sums to a common shift is exact.  Logits beyond 1e37, whose product with log2 e may overflow, are first taken
+// relative to m itself; their shifts stay apart from each other and in order.  c = -inf: no logit above -inf yet.
+// A NaN is skipped by the maximum and kept by the sum.
+constexpr float kLog2e = 1.4426950408889634f, kFar = 1e37f;
 template <typename T> struct alignas(2 * sizeof(T)) Lse {
-    T m, s;
-    __device__ __forceinline__ T factor(T top) const { return m == lowest<T>() ? (T)1 : exp_(m - top); }
-    __device__ __forceinline__ void merge(T m2, T s2) {
-        const Lse o{m2, s2};
-        const T top = max_(m, m2);
-        s = s * factor(top) + o.s * o.factor(top);
-        m = top;
-    }
-    template <int N> __device__ __forceinline__ void add(const T *x) {
-        T top = m;
-#pragma unroll
-        for (int k = 0; k < N; ++k) top = max_(top, x[k]);
-        if (top > m) {
-            s = m == lowest<T>() ? s : s * exp_(m - top);
-            m = top;
-        }
-#pragma unroll
-        for (int k = 0; k < N; ++k) s += x[k] == lowest<T>() ? (T)0 : exp_(x[k] - m);
-    }
+    T c, s;
 };
-
-// x becomes exp(x - m) for the maximum of these n values (0 in place of a maximum of -inf)
-template <typename T, int N> __device__ __forceinline__ Lse<T> exponentials(T (&x)[N]) {
-    Lse<T> l{lowest<T>(), (T)0};
-#pragma unroll
-    for (int k = 0; k < N; ++k) l.m = max_(l.m, x[k]);
-    const T base = l.m == lowest<T>() ? (T)0 : l.m;
-    T part[4] = {};
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        x[k] = fast_exp(x[k] - base);
-        part[k % 4] += x[k];
-    }
-    l.s = (part[0] + part[1]) + (part[2] + part[3]);
-    return l;
+__device__ __forceinline__ float shift_of(float m) {
+    if (m == -INFINITY) return m;
+    return fabsf(m) <= kFar ? rintf(m * kLog2e) : m * 0.9f + copysignf(kFar, m);
 }
+__device__ __forceinline__ double shift_of(double m) { return m; }
+__device__ __forceinline__ float exp2_(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// what a sum of shift c is multiplied by to have the shift `top` >= c
+__device__ __forceinline__ float rescale(float c, float top) {
+    if (c == -INFINITY) return 1.0f;
+    const float d = c - top;   // a whole number
+    return d >= -126.0f ? __int_as_float(((int)d + 127) << 23) : (d == d ? 0.0f : d);
+}
+__device__ __forceinline__ double rescale(double c, double top) { return c == -(double)INFINITY ? 1.0 : exp(c - top); }
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar && m != -INFINITY; }
+__device__ __forceinline__ bool is_far(double) { return false; }
+// exponential of x relative to the shift c, or, far out, to the maximum itself
+__device__ __forceinline__ float exp_near(float x, float c) { return exp2_(fmaf(x, kLog2e, -c)); }
+__device__ __forceinline__ float exp_far(float x, float m) { return exp2_((x - m) * kLog2e); }
+__device__ __forceinline__ double exp_near(double x, double c) { return exp(x - c); }
+__device__ __forceinline__ double exp_far(double x, double m) { return exp(x - m); }
+// x becomes the exponentials of N values
+template <typename T, int N> __device__ __forceinline__ Lse<T> lse_of(T (&x)[N]) {
+    T m[4] = {lowest<T>(), lowest<T>(), lowest<T>(), lowest<T>()}, s[4] = {};
+#pragma unroll
+    for (int k = 0; k < N; ++k) m[k % 4] = max_(m[k % 4], x[k]);
+    const T top = max_(max_(m[0], m[1]), max_(m[2], m[3]));
+    if (is_far(top)) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = exp_far(x[k], top);
+    } else {
+        const T c = top == lowest<T>() ? (T)0 : shift_of(top);
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = exp_near(x[k], c);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) s[k % 4] += x[k];
+    return Lse<T>{shift_of(top), (s[0] + s[1]) + (s[2] + s[3])};
+}
+// log(sum of exponentials) - target: without cancellation where the target is near the maximum.  p: its softmax
+__device__ __forceinline__ float minus_log(const Lse<float> &l, float target, float p) {
+    if (fabsf(l.c) > kFar) return -logf(p);
+    return 0.6931471805599453f * (log2f(l.s) - fmaf(target, kLog2e, -l.c));
+}
+__device__ __forceinline__ double minus_log(const Lse<double> &l, double target, double) { return log(l.s) - (target - l.c); }
 
 // number of rows that count, as kCountCtas partial counts
 __global__ void __launch_bounds__(256) xent_count_kernel(const int64_t *targets, size_t rows, unsigned long long *counts) {
@@ -194,11 +205,6 @@ template <typename T, int THREADS> __device__ __forceinline__ void finish_loss(c
     }
 }
 
-// a row's loss from its maximum, sum and target logit
-template <typename T> __device__ __forceinline__ double row_loss(const Lse<T> &l, T target, bool bad) {
-    return bad ? (double)NAN : (double)(log_(l.s) - (target - l.m));
-}
-
 // ---- rows of up to TPR * NV packs of N: TPR threads of a warp hold a row ---------------------------------------
 template <typename T, int TPR, int NV, int N>
 __global__ void __launch_bounds__(256) xent_warp_kernel(const __grid_constant__ XentArgs<T> p) {
@@ -207,11 +213,17 @@ __global__ void __launch_bounds__(256) xent_warp_kernel(const __grid_constant__ 
     const int in_row = threadIdx.x % TPR, slot = threadIdx.x / TPR;
     grid_dep_sync();
     const T inv_n = map_factor<T, 256>(p, sn);
+    // one thread a row: its map goes through shared memory, so that a warp writes consecutive addresses
+    __shared__ alignas(16) T tile[TPR == 1 ? 256 * NV * N : 1];
     XentPartial mine{0.0, 0};
-    for (size_t r0 = (size_t)blockIdx.x * G; r0 < p.rows; r0 += (size_t)gridDim.x * G) {
+    const size_t step = (size_t)gridDim.x * G;
+    int64_t t_next = (size_t)blockIdx.x * G + slot < p.rows ? p.targets[(size_t)blockIdx.x * G + slot] : -1;
+    for (size_t r0 = (size_t)blockIdx.x * G; r0 < p.rows; r0 += step) {
         const size_t r = r0 + slot;
-        const int64_t t = r < p.rows ? p.targets[r] : -1;
+        const int64_t t = t_next;
+        t_next = r + step < p.rows ? p.targets[r + step] : -1;   // ahead: whether a row is read depends on it
         const bool counted = t >= 0, bad = (uint64_t)t >= p.classes;
+        const int tt = bad ? -1 : (int)t;
         const T *x = p.logits + (counted ? (int64_t)r * p.pitch : 0);
         T e[NV * N];
         T xt = (T)0;          // the target's logit, in the thread that holds it: the map may take the logits' place
@@ -229,25 +241,28 @@ __global__ void __launch_bounds__(256) xent_warp_kernel(const __grid_constant__ 
                 }
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    if (j + i == (size_t)t) xt = e[k * N + i], mine_t = true;
+                    if ((int)j + i == tt) xt = e[k * N + i], mine_t = true;
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) e[k * N + i] = lowest<T>();
             }
         }
-        Lse<T> l = exponentials(e);
-        const Lse<T> own = l;
-        // the row's maximum first: one rescaling, then a plain sum
-        T top = l.m;
+        const Lse<T> own = lse_of(e);
+        T et = (T)0;
+#pragma unroll
+        for (int k = 0; k < NV * N; ++k)
+            if ((k / N * TPR + in_row) * N + k % N == tt) et = e[k];
+        // the row's shift first: one rescaling, then a plain sum
+        T top = own.c;
 #pragma unroll
         for (int d = TPR / 2; d; d >>= 1) top = max_(top, __shfl_xor_sync(0xffffffffu, top, d));
-        const T f = own.factor(top);
+        const T f = rescale(own.c, top);
         T sum = own.s * f;
 #pragma unroll
         for (int d = TPR / 2; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        l = Lse<T>{top, sum};
         if (counted) {
-            if (mine_t || (bad && in_row == 0)) mine.loss += row_loss(l, xt, bad);
+            if (mine_t) mine.loss += (double)minus_log(Lse<T>{top, sum}, xt, et * f / sum);
+            if (bad && in_row == 0) mine.loss = NAN;
             if (in_row == 0) mine.rows += 1;
         }
         if (p.map && r < p.rows) {
@@ -261,9 +276,18 @@ __global__ void __launch_bounds__(256) xent_warp_kernel(const __grid_constant__ 
                 Vec<T> q;
 #pragma unroll
                 for (int i = 0; i < N; ++i)
-                    q.e[i] = counted ? (e[k * N + i] * to_p - (j + i == (size_t)t ? (T)1 : (T)0)) * inv_n : (T)0;
-                if constexpr (N > 1) *reinterpret_cast<Vec<T> *>(g + j) = q;
+                    q.e[i] = counted ? (e[k * N + i] * to_p - ((int)j + i == tt ? (T)1 : (T)0)) * inv_n : (T)0;
+                if constexpr (TPR == 1) tile[slot * p.classes + j] = q.e[0];
+                else if constexpr (N > 1) *reinterpret_cast<Vec<T> *>(g + j) = q;
                 else g[j] = q.e[0];
+            }
+        }
+        if constexpr (TPR == 1) {
+            if (p.map) {
+                const size_t n = min((size_t)G, p.rows - r0) * p.classes;
+                __syncthreads();
+                for (size_t i = threadIdx.x; i < n; i += 256) p.map[r0 * p.classes + i] = tile[i];
+                __syncthreads();
             }
         }
     }
@@ -273,11 +297,12 @@ __global__ void __launch_bounds__(256) xent_warp_kernel(const __grid_constant__ 
 // ---- a CTA, or each CTA of a cluster, holds THREADS * NV vectors of 16 bytes of a row ----------------------------
 // Vectors lie at 16-byte boundaries of the logits; where a row starts in the middle of one (an odd number of classes), its first
 // and last vectors are partly the row's.
-// AHEAD rows are in shared memory or on their way; a row's vectors are taken, and replaced, in kGroups parts, so that copies never
-// all wait for the last of a row.
-template <typename T, int THREADS, int NV, int AHEAD>
-__global__ void __launch_bounds__(THREADS, 512 / THREADS) xent_cta_kernel(const __grid_constant__ XentArgs<T> p) {
-    constexpr int kWarps = THREADS / 32, N = Vec<T>::N, kGroups = 4, kGroup = NV / kGroups;
+// AHEAD rows are in shared memory or on their way.  A row's vectors are taken, and replaced by a later row's, one by one, so that
+// copies never all wait for the last of a row.
+// ALIGNED: every row is whole vectors.
+template <typename T, int THREADS, int NV, int AHEAD, bool ALIGNED>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) xent_cta_kernel(const __grid_constant__ XentArgs<T> p) {
+    constexpr int kWarps = THREADS / 32, N = Vec<T>::N;
     extern __shared__ __align__(16) unsigned char ring[];   // [row ahead][vector][thread]: a thread copies what it reads itself
     __shared__ alignas(16) Lse<T> pairs[2][kMaxCluster * kWarps];
     __shared__ unsigned long long arrived[2];
@@ -294,35 +319,44 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) xent_cta_kernel(const 
     auto slot = [&](int ahead, int k) { return reinterpret_cast<P *>(ring) + (ahead * NV + k) * THREADS + threadIdx.x; };
     auto row_at = [&](size_t r) { return p.logits + (int64_t)r * p.pitch; };
     // elements of the row's first vector that lie in front of the row
-    auto phase_of = [&](const T *x) { return (int)(((uintptr_t)x & 15u) / sizeof(T)); };
-    // the class of vector k's first element: below zero, or the vector beyond `classes`, at the row's ends
-    auto class_of = [&](int k, int phase) { return ((int)(rank * NV + k) * THREADS + (int)threadIdx.x) * N - phase; };
-    auto copy_group = [&](size_t r, int64_t t, int ahead, int group) {
-        if (t >= 0) {
-            const T *x = row_at(r);
-            const int phase = phase_of(x);
+    auto phase_of = [&](const T *x) { return ALIGNED ? 0 : (int)(((uintptr_t)x & 15u) / sizeof(T)); };
+    // the class of the thread's first vector's first element; that of vector k is k * kStep further, below zero or its vector
+    // beyond `classes` at the row's ends
+    constexpr int kStep = THREADS * N;
+    const int class0 = (int)(rank * NV * THREADS + threadIdx.x) * N;
+    struct Row {
+        const T *x;      // the thread's first class, possibly in front of the row
+        int first, left; // its number; classes from it to the end (0: nothing to copy)
+    };
+    auto row_of = [&](size_t r, int64_t t) {
+        const T *x = row_at(t < 0 ? 0 : r);
+        const int first = class0 - phase_of(x);
+        return Row{x + first, first, t < 0 ? 0 : classes - first};
+    };
+    auto copy_vector = [&](const Row &row, int ahead, int k) {
+        if (k * kStep < row.left) {
+            if (ALIGNED) {
+                copy_async<16>(slot(ahead, k), row.x + k * kStep);
+            } else if (k > 0 || row.first >= 0) {
+                copy_async_16(slot(ahead, k), row.x + k * kStep, k * kStep + N <= row.left ? 16 : (unsigned)(row.left - k * kStep) * (unsigned)sizeof(T));
+            } else {
 #pragma unroll
-            for (int k = group * kGroup; k < (group + 1) * kGroup; ++k) {
-                const int j = class_of(k, phase);
-                if (j >= classes) continue;
-                if (j >= 0) {
-                    copy_async_16(slot(ahead, k), x + j, j + N <= classes ? 16 : (unsigned)(classes - j) * (unsigned)sizeof(T));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        if (j + i >= 0 && j + i < classes) copy_async<sizeof(T)>(&slot(ahead, k)->e[i], x + j + i);
-                }
+                for (int i = 0; i < N; ++i)
+                    if (row.first + i >= 0 && i < row.left) copy_async<sizeof(T)>(&slot(ahead, k)->e[i], row.x + i);
             }
         }
         copy_commit();
     };
     int64_t t_of[AHEAD + 1];   // targets of this row and of those ahead
 #pragma unroll
-    for (int a = 0; a <= AHEAD; ++a) t_of[a] = target_of(row0 + a * stride);
+    for (int d = 0; d <= AHEAD; ++d) t_of[d] = target_of(row0 + d * stride);
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a)
+    for (int d = 0; d < AHEAD; ++d) {
+        const Row row = row_of(row0 + d * stride, t_of[d]);
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) copy_group(row0 + a * stride, t_of[a], a, g);
+        for (int k = 0; k < NV; ++k)
+            copy_vector(row, d, k);
+    }
     int ahead = 0;
     if (nc > 1) {
         if (threadIdx.x == 0) mbar_init(&arrived[0]), mbar_init(&arrived[1]);
@@ -333,34 +367,34 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) xent_cta_kernel(const 
     unsigned counted = 0;    // rows worked on: which buffer, which phase
     for (size_t r = row0; r < p.rows; r += stride) {
         const int64_t t_far = target_of(r + (AHEAD + 1) * stride), t = t_of[0];
-        const int phase = t < 0 ? 0 : phase_of(row_at(r));
+        const Row row = row_of(r, t), later = row_of(r + AHEAD * stride, t_of[AHEAD]);
         T e[NV * N];
         T xt = (T)0;          // the target's logit, in the thread that holds it: the map may take the logits' place
-        bool mine_t = false;
-        const bool bad = t >= (int64_t)classes, first = rank == 0 && threadIdx.x == 0;
-        const int tt = bad ? -N : (int)t;   // no class in any vector where the target is beyond them
+        const bool bad = t >= (int64_t)classes, leader = rank == 0 && threadIdx.x == 0;
+        const int tt = (int)t - row.first;   // the target seen from the thread's first class
+        const bool mine_t = t >= 0 && !bad && tt >= 0 && tt < NV * kStep && tt % kStep < N;
 #pragma unroll
-        for (int group = 0; group < kGroups; ++group) {
-            copy_wait<AHEAD * kGroups - 1>();
-            if (t >= 0) {
+        for (int k = 0; k < NV; ++k) {
+            copy_wait<AHEAD * NV - 1>();
+            if (k * kStep < row.left) {
+                const P q = *slot(ahead, k);
 #pragma unroll
-                for (int k = group * kGroup; k < (group + 1) * kGroup; ++k) {
-                    const int j = class_of(k, phase);
-                    P q;
-                    if (j < classes) q = *slot(ahead, k);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) e[k * N + i] = j < classes ? q.e[i] : lowest<T>();
-                    if (j < 0 || j + N > classes) {
-#pragma unroll
-                        for (int i = 0; i < N; ++i)
-                            if (j + i < 0 || j + i >= classes) e[k * N + i] = lowest<T>();
-                    }
+                for (int i = 0; i < N; ++i) e[k * N + i] = q.e[i];
+                if (!ALIGNED && ((k == 0 && row.first < 0) || k * kStep + N > row.left)) {
 #pragma unroll
                     for (int i = 0; i < N; ++i)
-                        if (j + i == tt) xt = e[k * N + i], mine_t = true;
+                        if (row.first + k * kStep + i < 0 || k * kStep + i >= row.left) e[k * N + i] = lowest<T>();
                 }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) e[k * N + i] = lowest<T>();
             }
-            copy_group(r + AHEAD * stride, t_of[AHEAD], ahead, group);
+            copy_vector(later, ahead, k);
+        }
+        if (mine_t) {
+#pragma unroll
+            for (int k = 0; k < NV * N; ++k)
+                if (k / N * kStep + k % N == tt) xt = e[k];
         }
         if (t < 0) {
             if (p.map) {
@@ -369,9 +403,9 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) xent_cta_kernel(const 
                     if (j < classes) g[j] = (T)0;
             }
         } else {
-            const Lse<T> own = exponentials(e);
-            Lse<T> l{warp_max(own.m), (T)0};
-            l.s = own.s * own.factor(l.m);
+            const Lse<T> own = lse_of(e);
+            Lse<T> l{warp_max(own.c), (T)0};
+            l.s = own.s * rescale(own.c, l.c);
 #pragma unroll
             for (int d = 16; d; d >>= 1) l.s += __shfl_xor_sync(0xffffffffu, l.s, d);
             const int buf = (int)(counted & 1);   // a warp is never a whole row ahead of another: two buffers suffice
@@ -385,43 +419,48 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) xent_cta_kernel(const 
             }
             ++counted;
             // all warps merge the pairs the same way
-            T m = lowest<T>();
-            for (unsigned k = lane; k < nc * kWarps; k += 32) m = max_(m, pairs[buf][k].m);
-            m = warp_max(m);
+            T c = lowest<T>();
+            for (unsigned k = lane; k < nc * kWarps; k += 32) c = max_(c, pairs[buf][k].c);
+            c = warp_max(c);
             T sum = (T)0;
-            for (unsigned k = lane; k < nc * kWarps; k += 32) sum += pairs[buf][k].s * pairs[buf][k].factor(m);
+            for (unsigned k = lane; k < nc * kWarps; k += 32) sum += pairs[buf][k].s * rescale(pairs[buf][k].c, c);
 #pragma unroll
             for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             if (lost) sum = nan_<T>();
-            if (mine_t || (bad && first)) mine.loss += row_loss(Lse<T>{m, sum}, xt, bad);
-            if (first) mine.rows += 1;
+            const T inv_s = bad ? nan_<T>() : (T)1 / sum;
+            const T to_p = rescale(own.c, c) * inv_s, to_map = to_p * inv_n;
+            if (leader) mine.rows += 1;
+            if (leader && bad) mine.loss = NAN;
+            T et = (T)0;
+            if (mine_t) {
+#pragma unroll
+                for (int k = 0; k < NV * N; ++k)
+                    if (k / N * kStep + k % N == tt) et = e[k];
+                mine.loss += (double)minus_log(Lse<T>{c, sum}, xt, et * to_p);
+            }
             if (p.map) {
                 T *g = p.map + r * p.classes;
-                const bool whole = ((uintptr_t)(g - phase) & 15u) == 0;   // the map's vectors lie as the logits' do
-                const T inv_s = bad ? nan_<T>() : (T)1 / sum;
-                const T to_p = own.factor(m) * inv_s, to_map = to_p * inv_n;
+                g += row.first;
+                const bool whole = ALIGNED || ((uintptr_t)g & 15u) == 0;   // the map's vectors lie as the logits' do
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
-                    const int j = class_of(k, phase);
-                    if (j >= classes) continue;
+                    if (k * kStep >= row.left) continue;
                     P q;
 #pragma unroll
                     for (int i = 0; i < N; ++i) q.e[i] = e[k * N + i] * to_map;
-#pragma unroll
-                    for (int i = 0; i < N; ++i)
-                        if (j + i == tt) q.e[i] = (e[k * N + i] * to_p - (T)1) * inv_n;
-                    if (whole && j >= 0 && j + N <= classes) {
-                        st<T, N>(g + j, q);
+                    if (ALIGNED || (whole && (k > 0 || row.first >= 0) && k * kStep + N <= row.left)) {
+                        st<T, N>(g + k * kStep, q);
                     } else {
 #pragma unroll
                         for (int i = 0; i < N; ++i)
-                            if (j + i >= 0 && j + i < classes) g[j + i] = q.e[i];
+                            if (row.first + k * kStep + i >= 0 && k * kStep + i < row.left) g[k * kStep + i] = q.e[i];
                     }
                 }
+                if (mine_t) g[tt] = (et * to_p - (T)1) * inv_n;   // over what the thread has just written there
             }
         }
 #pragma unroll
-        for (int a = 0; a < AHEAD; ++a) t_of[a] = t_of[a + 1];
+        for (int d = 0; d < AHEAD; ++d) t_of[d] = t_of[d + 1];
         t_of[AHEAD] = t_far;
         ahead = ahead + 1 == AHEAD ? 0 : ahead + 1;
     }
@@ -451,26 +490,41 @@ __global__ void __launch_bounds__(512) xent_twice_kernel(const __grid_constant__
                 for (size_t k = threadIdx.x; k < packs; k += THREADS) st<T, N>(g + k * N, P{});
             continue;
         }
-        Lse<T> l{lowest<T>(), (T)0};
-        for (size_t k = threadIdx.x; k < packs; k += THREADS) l.template add<N>(ld<T, N>(x + k * N).e);
+        T m = lowest<T>(), sum = (T)0;   // the sum relative to this thread's maximum so far
+        for (size_t k = threadIdx.x; k < packs; k += THREADS) {
+            const P q = ld<T, N>(x + k * N);
+            T top = m;
 #pragma unroll
-        for (int d = 16; d; d >>= 1) l.merge(__shfl_xor_sync(0xffffffffu, l.m, d), __shfl_xor_sync(0xffffffffu, l.s, d));
-        if (lane == 0) pairs[warp] = l;
+            for (int j = 0; j < N; ++j) top = max_(top, q.e[j]);
+            if (top > m) {
+                sum = m == lowest<T>() ? sum : sum * exp_(m - top);
+                m = top;
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) sum += q.e[j] == lowest<T>() ? (T)0 : exp_(q.e[j] - m);
+        }
+        const T warp_top = warp_max(m);
+        sum = m == lowest<T>() ? sum : sum * exp_(m - warp_top);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) pairs[warp] = Lse<T>{warp_top, sum};
         __syncthreads();
-        l = pairs[0];
-        for (int w = 1; w < kWarps; ++w) l.merge(pairs[w].m, pairs[w].s);
+        m = pairs[0].c;
+        for (int w = 1; w < kWarps; ++w) m = max_(m, pairs[w].c);
+        sum = (T)0;
+        for (int w = 0; w < kWarps; ++w) sum += pairs[w].c == lowest<T>() ? pairs[w].s : pairs[w].s * exp_(pairs[w].c - m);
         const bool bad = (uint64_t)t >= p.classes;
         if (threadIdx.x == 0) {
-            mine.loss += row_loss(l, bad ? (T)0 : x[t], bad);
+            mine.loss += bad ? (double)NAN : (double)(log_(sum) - (x[t] - m));
             mine.rows += 1;
         }
         __syncthreads();   // the pairs are written again for the next row, x[t] may be overwritten below
         if (g) {
-            const T inv_s = bad ? nan_<T>() : (T)1 / l.s;
+            const T inv_s = bad ? nan_<T>() : (T)1 / sum;
             for (size_t k = threadIdx.x; k < packs; k += THREADS) {
                 P q = ld<T, N>(x + k * N);
 #pragma unroll
-                for (int j = 0; j < N; ++j) q.e[j] = (exp_(q.e[j] - l.m) * inv_s - (k * N + j == (size_t)t ? (T)1 : (T)0)) * inv_n;
+                for (int j = 0; j < N; ++j) q.e[j] = (exp_(q.e[j] - m) * inv_s - (k * N + j == (size_t)t ? (T)1 : (T)0)) * inv_n;
                 st<T, N>(g + k * N, q);
             }
         }
@@ -503,14 +557,21 @@ template <typename T, int TPR, int NV, int N> int run_warp(Ctx *ctx, XentArgs<T>
     return run<T, xent_warp_kernel<T, TPR, NV, N>>(ctx, "xent_warp_kernel", p, grid, 256, 0);
 }
 
-template <typename T, int THREADS, int NV, int AHEAD> int run_cta(Ctx *ctx, XentArgs<T> &p, unsigned cluster) {
+template <typename T, int THREADS, int NV, int AHEAD, bool ALIGNED> int run_rows(Ctx *ctx, XentArgs<T> &p) {
+    constexpr auto kernel = xent_cta_kernel<T, THREADS, NV, AHEAD, ALIGNED>;
     constexpr size_t smem = (size_t)AHEAD * THREADS * NV * 16;
-    p.cluster = cluster;
-    // as many clusters as run at once (a CTA of 512 threads fills an SM, four of 128 do), the rows dealt out among them
+    // as many clusters as run at once (a CTA of 1024 threads fills an SM, eight of 128 do), the rows dealt out among them
     unsigned fit = 0;
-    if (int rc = clusters_at_once<XentArgs<T>, xent_cta_kernel<T, THREADS, NV, AHEAD>>(ctx, THREADS, cluster, smem, &fit)) return rc;
+    if (int rc = clusters_at_once<XentArgs<T>, kernel>(ctx, THREADS, p.cluster, smem, &fit)) return rc;
     const size_t clusters = std::max<size_t>(1, std::min<size_t>(p.rows, fit));
-    return run<T, xent_cta_kernel<T, THREADS, NV, AHEAD>>(ctx, "xent_cta_kernel", p, clusters * cluster, THREADS, smem);
+    return run<T, kernel>(ctx, "xent_cta_kernel", p, clusters * p.cluster, THREADS, smem);
+}
+// Rows that need six vectors of a thread at most leave room to copy two rows ahead.
+template <typename T, int THREADS> int run_cta(Ctx *ctx, XentArgs<T> &p, unsigned cluster, bool vec, size_t room) {
+    p.cluster = cluster;
+    if (cluster == 1 && room <= (size_t)THREADS * 6 * 16)
+        return vec ? run_rows<T, THREADS, 6, 2, true>(ctx, p) : run_rows<T, THREADS, 6, 2, false>(ctx, p);
+    return vec ? run_rows<T, THREADS, 8, 1, true>(ctx, p) : run_rows<T, THREADS, 8, 1, false>(ctx, p);
 }
 
 template <typename T> int pick_size(Ctx *ctx, XentArgs<T> &p, bool vec) {
@@ -527,12 +588,13 @@ template <typename T> int pick_size(Ctx *ctx, XentArgs<T> &p, bool vec) {
         if (n <= 256) return run_warp<T, 32, 8, 1>(ctx, p);
         if (bytes <= 4096) return run_warp<T, 32, 128 / (int)sizeof(T), 1>(ctx, p);
     }
-    const size_t room = bytes + 16;   // a row that starts inside a vector takes one more
-    if (room <= 128 * 8 * 16) return run_cta<T, 128, 8, 3>(ctx, p, 1);
-    if (room <= 128 * 16 * 16) return run_cta<T, 128, 16, 1>(ctx, p, 1);
-    if (room <= 256 * 16 * 16) return run_cta<T, 256, 16, 1>(ctx, p, 1);
+    const size_t room = bytes + (vec ? 0 : 16);   // a row that starts inside a vector takes one more
+    if (room <= 64 * 128) return run_cta<T, 64>(ctx, p, 1, vec, room);
+    if (room <= 128 * 128) return run_cta<T, 128>(ctx, p, 1, vec, room);
+    if (room <= 256 * 128) return run_cta<T, 256>(ctx, p, 1, vec, room);
+    if (room <= 512 * 128) return run_cta<T, 512>(ctx, p, 1, vec, room);
     for (unsigned cluster = 1; cluster <= kMaxCluster; cluster *= 2)
-        if (room <= (size_t)cluster * 512 * 16 * 16) return run_cta<T, 512, 16, 1>(ctx, p, cluster);
+        if (room <= (size_t)cluster * 1024 * 128) return run_cta<T, 1024>(ctx, p, cluster, vec, room);
     const size_t grid = std::min<size_t>(p.rows, (size_t)ctx->sm_count * 4);
     if (vec) return run<T, xent_twice_kernel<T, N>>(ctx, "xent_twice_kernel", p, grid, 512, 0);
     return run<T, xent_twice_kernel<T, 1>>(ctx, "xent_twice_kernel", p, grid, 512, 0);
