@@ -12,23 +12,28 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;                                  // blocks of a warp, loads of all in flight at once
 constexpr int kTileBlocks = kWarps * kUnroll;
 
-template <typename T> struct alignas(16) Vec {
-    static constexpr int N = 16 / sizeof(T);
-    T e[N];
-};
-
+// max |x| of a block.  A NaN wins (max.NaN), and as bits NaN > inf > every finite magnitude, so one comparison tells.
 template <typename T> struct Bits;
 template <> struct Bits<float> {
     using U = uint32_t;
     static constexpr U inf = 0x7f800000u;
-    static __device__ __forceinline__ U abs(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+    static __device__ __forceinline__ float top(float a, float b) {
+        float m;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)));
+        return m;
+    }
+    static __device__ __forceinline__ U bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
     static __device__ __forceinline__ float value(U u) { return __uint_as_float(u); }
     static __device__ __forceinline__ U warp_max(U u) { return __reduce_max_sync(0xffffffffu, u); }
 };
 template <> struct Bits<double> {
     using U = unsigned long long;
     static constexpr U inf = 0x7ff0000000000000ull;
-    static __device__ __forceinline__ U abs(double x) { return (U)__double_as_longlong(x) & 0x7fffffffffffffffull; }
+    static __device__ __forceinline__ double top(double a, double b) {
+        const U u = max(bits(a), bits(b));
+        return __longlong_as_double((long long)u);
+    }
+    static __device__ __forceinline__ U bits(double x) { return (U)__double_as_longlong(x) & 0x7fffffffffffffffull; }
     static __device__ __forceinline__ double value(U u) { return __longlong_as_double((long long)u); }
     static __device__ __forceinline__ U warp_max(U u) {
 #pragma unroll
@@ -50,35 +55,68 @@ struct Quantise32 {
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(mag));
         inv *= 127.0f;
     }
-    __device__ __forceinline__ uint32_t code(float x) const {   // in the low byte
+    // four codes, packed
+    __device__ __forceinline__ uint32_t codes(const float x[4]) const {
         const float magic = 12582912.0f;
-        const float t = fmaf(x, inv, magic);
-        uint32_t c = __float_as_uint(t);
-        if (wide || fabsf(fmaf(x, inv, magic - t)) > 0.4998f) c = m > 0.0f ? (uint32_t)(int)rint(127.0 * (double)x / (double)m) : 0u;
-        return c;
+        uint32_t c[4];
+        float off = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float t = fmaf(x[k], inv, magic);
+            c[k] = __float_as_uint(t);
+            off = fmaxf(off, fabsf(fmaf(x[k], inv, magic - t)));
+        }
+        if (wide || off > 0.4998f) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) c[k] = m > 0.0f ? (uint32_t)(int)rint(127.0 * (double)x[k] / (double)m) : 0u;
+        }
+        return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     }
 };
+// f64: the quotient as IEEE arithmetic gives it; the product with the reciprocal decides all but the values within 1e-9 of a tie.
 struct Quantise64 {
-    double m, down;
-    __device__ __forceinline__ explicit Quantise64(double mag) : m(mag), down(1.0) {
+    double m, inv, down;
+    bool wide;
+    __device__ __forceinline__ explicit Quantise64(double mag) : m(mag), inv(127.0 / mag), down(1.0), wide(!(mag > 1e-280 && mag < 1e300)) {
         if (mag > 1e300) m = mag * 0x1p-20, down = 0x1p-20;   // 127 x stays finite
     }
-    __device__ __forceinline__ uint32_t code(double x) const { return m > 0.0 ? (uint32_t)(int)rint(127.0 * (x * down) / m) : 0u; }
+    __device__ __forceinline__ uint32_t codes(const double x[4]) const {
+        const double magic = 6755399441055744.0;   // 1.5 2^52
+        uint32_t c[4];
+        double off = 0.0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const double t = fma(x[k], inv, magic);
+            c[k] = (uint32_t)__double2loint(t);
+            off = fmax(off, fabs(fma(x[k], inv, magic - t)));
+        }
+        if (wide || off > 0.499999999) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) c[k] = m > 0.0 ? (uint32_t)(int)rint(127.0 * (x[k] * down) / m) : 0u;
+        }
+        return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    }
 };
 template <typename T> struct QuantiseOf;
 template <> struct QuantiseOf<float> { using type = Quantise32; };
 template <> struct QuantiseOf<double> { using type = Quantise64; };
 
-// lane l holds elements 4 l .. 4 l + 3 of its block
+// Lane l holds elements 4 l .. 4 l + 3 of its block: one access of 16 bytes, in f64 of 32 (two of 16 would each touch every line of
+// the block's kilobyte).
+__device__ __forceinline__ void vector4(const float *p, float v[4]) {
+    const float4 q = *reinterpret_cast<const float4 *>(p);
+    v[0] = q.x, v[1] = q.y, v[2] = q.z, v[3] = q.w;
+}
+__device__ __forceinline__ void vector4(const double *p, double v[4]) {
+    asm volatile("ld.global.v4.f64 {%0, %1, %2, %3}, [%4];" : "=d"(v[0]), "=d"(v[1]), "=d"(v[2]), "=d"(v[3]) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void put_vector4(float *p, const float v[4]) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void put_vector4(double *p, const double v[4]) {
+    asm volatile("st.global.v4.f64 [%0], {%1, %2, %3, %4};" ::"l"(p), "d"(v[0]), "d"(v[1]), "d"(v[2]), "d"(v[3]) : "memory");
+}
 template <typename T, bool VEC> __device__ __forceinline__ void load4(const T *p, size_t i, size_t n, T v[4]) {
     if (VEC && i + 4 <= n) {
-        constexpr int N = Vec<T>::N;
-#pragma unroll
-        for (int k = 0; k < 4; k += N) {
-            const Vec<T> q = *reinterpret_cast<const Vec<T> *>(p + i + k);
-#pragma unroll
-            for (int j = 0; j < N; ++j) v[k + j] = q.e[j];
-        }
+        vector4(p + i, v);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = i + k < n ? p[i + k] : (T)0;
@@ -86,14 +124,7 @@ template <typename T, bool VEC> __device__ __forceinline__ void load4(const T *p
 }
 template <typename T, bool VEC> __device__ __forceinline__ void store4(T *p, size_t i, size_t n, const T v[4]) {
     if (VEC && i + 4 <= n) {
-        constexpr int N = Vec<T>::N;
-#pragma unroll
-        for (int k = 0; k < 4; k += N) {
-            Vec<T> q;
-#pragma unroll
-            for (int j = 0; j < N; ++j) q.e[j] = v[k + j];
-            *reinterpret_cast<Vec<T> *>(p + i + k) = q;
-        }
+        put_vector4(p + i, v);
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -129,18 +160,14 @@ __global__ void __launch_bounds__(kThreads) ckpt8_store_kernel(const T *src, siz
     for (int u = 0; u < kUnroll; ++u) {
         using B = Bits<T>;
         const size_t i = (block0 + u) * kCkpt8Block + lane * 4;
-        typename B::U top = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, B::abs(v[u][k]));
-        top = B::warp_max(top);
+        const typename B::U top = B::warp_max(B::bits(B::top(B::top(v[u][0], v[u][1]), B::top(v[u][2], v[u][3]))));
         if ((block0 + u) * kCkpt8Block >= n) continue;   // the same in the whole warp
         uint32_t c = 0;
         T m = B::value(top);
         if (top >= B::inf) {
             m = B::value(B::inf | 1u);   // some NaN
         } else {
-            const typename QuantiseOf<T>::type q(m);
-            c = __byte_perm(__byte_perm(q.code(v[u][0]), q.code(v[u][1]), 0x0040), __byte_perm(q.code(v[u][2]), q.code(v[u][3]), 0x0040), 0x5410);
+            c = typename QuantiseOf<T>::type(m).codes(v[u]);
         }
         store_codes(codes, i, n, c);
         if (lane == 0) mags[block0 + u] = m;
@@ -189,12 +216,12 @@ int tiles(size_t n, unsigned *grid) {
     return RTB_OK;
 }
 
-template <typename T> bool aligned16(const T *p) { return ((uintptr_t)p & 15u) == 0; }
+template <typename T> bool aligned4(const T *p) { return ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0; }
 
 template <typename T> int store_typed(Ctx *ctx, const T *src, size_t n, int8_t *codes, T *mags) {
     unsigned grid = 0;
     if (int rc = tiles(n, &grid)) return rc;
-    if (aligned16(src)) launch_dep(ctx, grid, kThreads, ckpt8_store_kernel<T, true>, src, n, codes, mags);
+    if (aligned4(src)) launch_dep(ctx, grid, kThreads, ckpt8_store_kernel<T, true>, src, n, codes, mags);
     else launch_dep(ctx, grid, kThreads, ckpt8_store_kernel<T, false>, src, n, codes, mags);
     return check_launch(ctx, "ckpt8_store_kernel");
 }
@@ -202,7 +229,7 @@ template <typename T> int store_typed(Ctx *ctx, const T *src, size_t n, int8_t *
 template <typename T, int KIND> int read_typed(Ctx *ctx, const int8_t *codes, const T *mags, const T *up, size_t n, T *dst) {
     unsigned grid = 0;
     if (int rc = tiles(n, &grid)) return rc;
-    if (aligned16(up) && aligned16(dst)) launch_dep(ctx, grid, kThreads, ckpt8_read_kernel<T, KIND, true>, codes, mags, up, n, dst);
+    if (aligned4(up) && aligned4(dst)) launch_dep(ctx, grid, kThreads, ckpt8_read_kernel<T, KIND, true>, codes, mags, up, n, dst);
     else launch_dep(ctx, grid, kThreads, ckpt8_read_kernel<T, KIND, false>, codes, mags, up, n, dst);
     return check_launch(ctx, "ckpt8_read_kernel");
 }

@@ -31,14 +31,14 @@ template <typename T> struct Ckpt8Scale {
         lo = ckpt8_fma((T)-127, hi, m) * r127;   // the residual itself is exact
     }
     __device__ __forceinline__ T restore(int8_t code) const { return down(times((T)code)); }
-    // the first N of four packed codes.  f32: a byte becomes the low mantissa byte of 2^23, two instructions where a conversion from
-    // 8 bits runs at an eighth of the rate.
+    // the first N of four packed codes.  A byte becomes the lowest mantissa byte of 2^23 (2^52): two instructions where a
+    // conversion from 8 bits runs at an eighth of the rate.
     template <int N> __device__ __forceinline__ void restore(uint32_t four, T *out) const {
-        if constexpr (sizeof(T) == 4) four ^= 0x80808080u;
+        four ^= 0x80808080u;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            if constexpr (sizeof(T) == 4) out[k] = times((T)(__uint_as_float(__byte_perm(four, 0x4b000000u, 0x7540u + k)) - 8388736.0f));
-            else out[k] = times((T)(int8_t)(four >> (8 * k)));
+            if constexpr (sizeof(T) == 4) out[k] = times(__uint_as_float(__byte_perm(four, 0x4b000000u, 0x7540u + k)) - 8388736.0f);
+            else out[k] = times(__hiloint2double(0x43300000, (int)__byte_perm(four, 0u, 0x4440u + k)) - 4503599627370624.0);
         }
         if (small) {
 #pragma unroll
