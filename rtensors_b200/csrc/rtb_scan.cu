@@ -860,11 +860,16 @@ template <typename T, int V, int LX, int R, int STAGES, int MODE, bool COUPLED, 
                                                p.lanes * p.steps <= kShortElements, p);
 }
 
-// Threads side by side in a group.  8 give rows of 128 bytes, a full line, and the most steps a round can have with them; 4 double the
-// steps again where groups of 8, in clusters of the largest size, would leave most SMs without work.  Measured, f32:
-// (1, 65536, 128) 112 us with 8, 76 with 4; (8, 8192, 1024) 142 us with 8, 171 with 4, 152 with 16, 155 with 32.
+// Threads side by side in a group.  With vectors, 8 give rows of 128 bytes, a full line, and the most steps a round can have with
+// them; 4 double the steps again where groups of 8, in clusters of the largest size, would leave most SMs without work.  Measured,
+// f32: (1, 65536, 128) 112 us with 8, 76 with 4; (8, 8192, 1024) 142 us with 8, 171 with 4, 152 with 16, 155 with 32.
+// By elements (V = 1), 32 give the full line, and 8 serve few lanes: (8, 8192, 1023) 186 us with 32, 212 with 8; (1, 40000, 75)
+// 90 us with 32, 34 with 8.
 template <typename T, int V> int side_by_side(const Ctx *ctx, const ScanArgs<T> &p) {
-    return (p.lanes + 8 * V - 1) / (8 * V) * kMaxCluster * 2 <= (uint64_t)ctx->sm_count ? 4 : 8;
+    constexpr int wide = V == 1 ? 32 : 8;
+    const uint64_t groups = (p.lanes + wide * V - 1) / (wide * V);
+    if (V == 1) return groups * kMaxCluster < (uint64_t)ctx->sm_count ? 8 : 32;
+    return groups * kMaxCluster * 2 <= (uint64_t)ctx->sm_count ? 4 : 8;
 }
 
 // Steps of a thread, with two stages of the ring.  More steps make fewer rounds, each of which costs the same exchange, and take
@@ -874,13 +879,20 @@ template <typename T, int V> int side_by_side(const Ctx *ctx, const ScanArgs<T> 
 //   backward, dense          4: 239 / 263   6: 246 / 236   8: 265 / 251        shared   4: 187 / 156   6: 170 / 155   8: 201 / 187
 //   backward from codes      4: 246 / 207   6: 299 / 282                       shared   4: 191 / 160   6: 175 / 150   8: 192 / 175
 //   backward, coupled        3: 308 / 262   4: 325 / 305   6: 307 / 283        shared   3: 244 / 203   4: 225 / 195   6: 247 / 230
+// By elements, at 8 x 8192 x 1023: forward 8: 186, 12: 192, 16: 191 (shared 16: 171, 8: 218); backward 8: 344, 12: 359, 16: 482.
 template <typename T, int V, int MODE, bool COUPLED, bool GVEC> int run_lanes(Ctx *ctx, ScanArgs<T> &p) {
     constexpr bool back = MODE != kForward;
-    constexpr int R = GVEC ? (back ? (COUPLED ? 3 : MODE == kBackDense ? 6 : 4) : 6) : (back ? (COUPLED ? 4 : 6) : 8);
-    if (side_by_side<T, V>(ctx, p) == 4) return run_width<T, V, 4, R, 2, MODE, COUPLED, GVEC>(ctx, p);
-    if constexpr (!back && GVEC)   // many lanes: no clusters, the exchange is cheap
-        if (p.lanes >= (uint64_t)ctx->sm_count * 8 * V) return run_width<T, V, 8, 4, 2, MODE, COUPLED, GVEC>(ctx, p);
-    return run_width<T, V, 8, R, 2, MODE, COUPLED, GVEC>(ctx, p);
+    if constexpr (V == 1) {
+        constexpr int R = sizeof(T) == 4 ? (back || GVEC ? 8 : 16) : (back ? 4 : GVEC ? 6 : 8);
+        if (side_by_side<T, 1>(ctx, p) == 8) return run_width<T, 1, 8, R, 2, MODE, COUPLED, GVEC>(ctx, p);
+        return run_width<T, 1, 32, R, 2, MODE, COUPLED, GVEC>(ctx, p);
+    } else {
+        constexpr int R = GVEC ? (back ? (COUPLED ? 3 : MODE == kBackDense ? 6 : 4) : 6) : (back ? (COUPLED ? 4 : 6) : 8);
+        if (side_by_side<T, V>(ctx, p) == 4) return run_width<T, V, 4, R, 2, MODE, COUPLED, GVEC>(ctx, p);
+        if constexpr (!back && GVEC)   // many lanes: no clusters, the exchange is cheap
+            if (p.lanes >= (uint64_t)ctx->sm_count * 8 * V) return run_width<T, V, 8, 4, 2, MODE, COUPLED, GVEC>(ctx, p);
+        return run_width<T, V, 8, R, 2, MODE, COUPLED, GVEC>(ctx, p);
+    }
 }
 
 // The V lanes of a thread are neighbours in every operand (or share the gate), at 16-byte aligned places.
@@ -902,7 +914,7 @@ template <typename T, int MODE, bool COUPLED> int pick_lanes(Ctx *ctx, ScanArgs<
     constexpr int V = 16 / sizeof(T);
     if (vec && p.dims.sg[p.dims.nd - 1] == 1) return run_lanes<T, V, MODE, COUPLED, true>(ctx, p);
     if (vec) return run_lanes<T, V, MODE, COUPLED, false>(ctx, p);
-    return run_lanes<T, 1, MODE, COUPLED, false>(ctx, p);
+    return p.dims.sg[p.dims.nd - 1] ? run_lanes<T, 1, MODE, COUPLED, true>(ctx, p) : run_lanes<T, 1, MODE, COUPLED, false>(ctx, p);
 }
 
 template <typename T, int MODE, bool COUPLED, bool VEC> int run_axis(Ctx *ctx, ScanArgs<T> &p) {

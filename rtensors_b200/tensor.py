@@ -7,6 +7,7 @@ copies a non-contiguous view, full reductions return a rank-0 tensor.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Sequence
 
 import numpy as np
@@ -311,10 +312,10 @@ class Tensor:
         """`meta` broadcast to this tensor's shape."""
         if meta.shape == self.meta.shape:
             return meta
-        shape, _, strides = broadcast_params(self.meta, meta)
-        if shape != self.meta.shape:
+        m = _spread(meta, self.meta.shape)
+        if m is None:
             raise L.RtbError(L.ERR_BROADCAST, f"{what} of shape {meta.shape} does not broadcast to {self.shape}")
-        return Meta(shape, strides, meta.offset)
+        return m
 
     def gated_scan_at(self, axis: int, gate: "Tensor", h0: Optional["Tensor"] = None, reverse: bool = False,
                       coupled: bool = False) -> "Tensor":
@@ -369,6 +370,12 @@ class Checkpoint8:
             raise L.RtbError(L.ERR_SHAPE, f"an upstream of shape {upstream.shape} for a checkpoint of shape {self.shape}")
         u = _dense(upstream)
         return Tensor(self.backend, self.backend.ckpt8_grad(self.KINDS[kind], self.codes, self.mags, u.buf, self.size, u.offset), self.meta)
+
+
+@lru_cache(maxsize=4096)
+def _spread(meta: Meta, shape) -> Optional[Meta]:
+    got, _, strides = broadcast_params(Meta.contiguous(shape), meta)
+    return Meta(got, strides, meta.offset) if got == shape else None
 
 
 def _is_dense(m: Meta) -> bool:
