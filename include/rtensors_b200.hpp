@@ -563,7 +563,95 @@ template <typename T> class TensorBase {
     TensorBase logsumexp() const { return reduce_ex<T>(-1, ReductionOpTypes::LogSumExp); }
     TensorBase<uint64_t> argmax() const { return reduce_ex<uint64_t>(-1, ReductionOpTypes::ArgMax); }
     TensorBase<uint64_t> argmin() const { return reduce_ex<uint64_t>(-1, ReductionOpTypes::ArgMin); }
+
+    // `m` broadcast to this tensor's shape: its strides, 0 along the dims that are added or stretched
+    std::vector<ptrdiff_t> strides_over(const MetaTensor &m) const {
+        const size_t r = meta.rank();
+        if (m.rank() > r) throw TensorError(RTB_ERR_BROADCAST, "an operand has more dims than the tensor");
+        std::vector<ptrdiff_t> st(r, 0);
+        for (size_t k = 0; k < m.rank(); ++k) {
+            const size_t d = r - m.rank() + k;
+            if (m.shape[k] == meta.shape[d]) st[d] = m.strides[k];
+            else if (m.shape[k] != 1) throw TensorError(RTB_ERR_BROADCAST, "an operand does not broadcast to the tensor");
+        }
+        return st;
+    }
+
+    // The gated linear recurrence h_s = gate_s h_{s-1} + x_s along `axis`, x being this tensor (rtb_gated_scan); flags:
+    // RTB_SCAN_REVERSE, RTB_SCAN_COUPLED; h0, if any, has this shape with `axis` as 1.
+    TensorBase gated_scan_at(size_t axis, const TensorBase &gate, const TensorBase *h0 = nullptr, int flags = 0) const {
+        if (axis >= meta.rank()) throw TensorError(RTB_ERR_DIM, "axis out of range");
+        const TensorBase g = gate.is_contiguous() ? gate : gate.contiguous();
+        const std::vector<ptrdiff_t> sg = strides_over(g.meta);
+        TensorBase first = *this;
+        if (h0) {
+            std::vector<size_t> want = meta.shape;
+            want[axis] = 1;
+            if (h0->shape() != want) throw TensorError(RTB_ERR_SHAPE, "h0 needs the tensor's shape with the axis as 1");
+            first = h0->contiguous();
+        }
+        check(rtb_meta_check_extent(meta.rank(), meta.shape.data(), meta.strides.data(), meta.offset, buf->len));
+        check(rtb_meta_check_extent(meta.rank(), meta.shape.data(), sg.data(), g.meta.offset, g.buf->len));
+        MetaTensor om = MetaTensor::contiguous(meta.shape);
+        TensorBase out{backend, backend->template alloc<T>(om.size() ? om.size() : 1), om};
+        check(rtb_gated_scan(backend->ctx(), DTypeOf<T>::value, flags, g.buf->ptr, sg.data(), g.meta.offset, buf->ptr, meta.strides.data(),
+                             meta.offset, h0 ? first.buf->ptr : nullptr, out.buf->ptr, meta.rank(), meta.shape.data(), axis));
+        return out;
+    }
+    // one step in place with this tensor as the state (rtb_gated_step); flags: RTB_SCAN_COUPLED
+    TensorBase &gated_step_inplace(const TensorBase &gate, const TensorBase &x, int flags = 0) {
+        const std::vector<ptrdiff_t> sg = strides_over(gate.meta), sx = strides_over(x.meta);
+        check(rtb_meta_check_extent(meta.rank(), meta.shape.data(), meta.strides.data(), meta.offset, buf->len));
+        check(rtb_meta_check_extent(meta.rank(), meta.shape.data(), sg.data(), gate.meta.offset, gate.buf->len));
+        check(rtb_meta_check_extent(meta.rank(), meta.shape.data(), sx.data(), x.meta.offset, x.buf->len));
+        check(rtb_gated_step(backend->ctx(), DTypeOf<T>::value, flags, buf->ptr, meta.strides.data(), meta.offset, gate.buf->ptr, sg.data(),
+                             gate.meta.offset, x.buf->ptr, sx.data(), x.meta.offset, meta.rank(), meta.shape.data()));
+        return *this;
+    }
 };
+
+// A float tensor kept in 8 bits an element (rtb_ckpt8_*): codes and one magnitude for each RTB_CKPT8_BLOCK elements.
+template <typename T> struct Checkpoint8 {
+    const Cuda *backend;
+    Cuda::BufPtr<int8_t> codes;
+    Cuda::BufPtr<T> mags;
+    MetaTensor meta;
+
+    static Checkpoint8 of(const TensorBase<T> &t) {
+        const TensorBase<T> c = t.contiguous();
+        const size_t n = c.size(), blocks = (n + RTB_CKPT8_BLOCK - 1) / RTB_CKPT8_BLOCK;
+        Checkpoint8 k{t.backend, t.backend->template alloc<int8_t>(n ? n : 1), t.backend->template alloc<T>(blocks ? blocks : 1), c.meta};
+        check(rtb_ckpt8_store(t.backend->ctx(), DTypeOf<T>::value, c.buf->ptr, n, k.codes->ptr, k.mags->ptr));
+        return k;
+    }
+    TensorBase<T> restore() const {
+        const size_t n = meta.size();
+        TensorBase<T> out{backend, backend->template alloc<T>(n ? n : 1), meta};
+        check(rtb_ckpt8_restore(backend->ctx(), DTypeOf<T>::value, codes->ptr, mags->ptr, n, out.buf->ptr));
+        return out;
+    }
+    // f'(restored) * upstream, kind = RTB_CKPT8_MUL / _SIGMOID / _TANH / _SQUARE
+    TensorBase<T> grad(int kind, const TensorBase<T> &upstream) const {
+        if (upstream.shape() != meta.shape) throw TensorError(RTB_ERR_SHAPE, "the upstream has another shape than the checkpoint");
+        const TensorBase<T> u = upstream.contiguous();
+        const size_t n = meta.size();
+        TensorBase<T> out{backend, backend->template alloc<T>(n ? n : 1), meta};
+        check(rtb_ckpt8_grad(backend->ctx(), DTypeOf<T>::value, kind, codes->ptr, mags->ptr, u.buf->ptr, n, out.buf->ptr));
+        return out;
+    }
+};
+
+// mean softmax cross-entropy of (rows, classes) logits as a rank-0 tensor (rtb_cross_entropy); a negative target is padding
+template <typename T> TensorBase<T> cross_entropy_loss(const TensorBase<T> &logits, const TensorBase<int64_t> &targets) {
+    if (logits.shape().size() != 2 || targets.shape().size() != 1 || targets.shape()[0] != logits.shape()[0])
+        throw TensorError(RTB_ERR_SHAPE, "cross_entropy_loss needs (rows, classes) logits and (rows) targets");
+    const TensorBase<T> x = logits.contiguous();
+    const TensorBase<int64_t> t = targets.contiguous();
+    TensorBase<T> out{logits.backend, logits.backend->template alloc<T>(1), MetaTensor::contiguous({})};
+    check(rtb_cross_entropy(logits.backend->ctx(), DTypeOf<T>::value, x.buf->ptr, x.shape()[0], x.shape()[1], (ptrdiff_t)x.shape()[1],
+                            t.buf->ptr, 0, out.buf->ptr, nullptr));
+    return out;
+}
 
 // mean(|input - target|) as a rank-0 tensor (src/ops/broadcast/l1.rs:79-84), fused
 template <typename T> TensorBase<T> mean_l1_loss(const TensorBase<T> &input, const TensorBase<T> &target) {

@@ -267,23 +267,29 @@ int read_any(rtb_ctx *c, int dtype, int kind, const int8_t *codes, const void *m
 using namespace rtb;
 
 RTB_API int rtb_ckpt8_store(rtb_ctx *c, int dtype, const void *src, size_t n, int8_t *codes, void *mags) {
-    if (int rc = check_ckpt(c, dtype)) return rc;
-    if (n == 0) return RTB_OK;
-    if (!src || !codes || !mags) return fail(RTB_ERR_INVALID, "null argument");
-    if ((uintptr_t)codes & 3u) return fail(RTB_ERR_INVALID, "the codes must be 4-byte aligned");
-    Ctx *ctx = reinterpret_cast<Ctx *>(c);
-    if (int rc = use_device(ctx)) return rc;
-    return dtype == RTB_F32 ? store_typed<float>(ctx, (const float *)src, n, codes, (float *)mags)
-                            : store_typed<double>(ctx, (const double *)src, n, codes, (double *)mags);
+    return guarded([&]() -> int {
+        if (int rc = check_ckpt(c, dtype)) return rc;
+        if (n == 0) return RTB_OK;
+        if (!src || !codes || !mags) return fail(RTB_ERR_INVALID, "null argument");
+        if ((uintptr_t)codes & 3u) return fail(RTB_ERR_INVALID, "the codes must be 4-byte aligned");
+        Ctx *ctx = reinterpret_cast<Ctx *>(c);
+        if (int rc = use_device(ctx)) return rc;
+        return dtype == RTB_F32 ? store_typed<float>(ctx, (const float *)src, n, codes, (float *)mags)
+                                : store_typed<double>(ctx, (const double *)src, n, codes, (double *)mags);
+    });
 }
 
 RTB_API int rtb_ckpt8_restore(rtb_ctx *c, int dtype, const int8_t *codes, const void *mags, size_t n, void *dst) {
-    if (int rc = check_ckpt(c, dtype)) return rc;
-    return read_any(c, dtype, -1, codes, mags, nullptr, n, dst);
+    return guarded([&]() -> int {
+        if (int rc = check_ckpt(c, dtype)) return rc;
+        return read_any(c, dtype, -1, codes, mags, nullptr, n, dst);
+    });
 }
 
 RTB_API int rtb_ckpt8_grad(rtb_ctx *c, int dtype, int kind, const int8_t *codes, const void *mags, const void *up, size_t n, void *dst) {
-    if (int rc = check_ckpt(c, dtype)) return rc;
-    if (kind < RTB_CKPT8_MUL || kind > RTB_CKPT8_SQUARE) return fail(RTB_ERR_INVALID, "unknown checkpoint map %d", kind);
-    return read_any(c, dtype, kind, codes, mags, up, n, dst);
+    return guarded([&]() -> int {
+        if (int rc = check_ckpt(c, dtype)) return rc;
+        if (kind < RTB_CKPT8_MUL || kind > RTB_CKPT8_SQUARE) return fail(RTB_ERR_INVALID, "unknown checkpoint map %d", kind);
+        return read_any(c, dtype, kind, codes, mags, up, n, dst);
+    });
 }

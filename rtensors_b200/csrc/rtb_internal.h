@@ -4,8 +4,10 @@
 #include <cstdint>
 #include <atomic>
 #include <cstring>
+#include <exception>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <utility>
 #include <vector>
@@ -27,6 +29,17 @@ int cuda_fail(cudaError_t e, const char *what);
         cudaError_t e__ = (call);                                            \
         if (e__ != cudaSuccess) return ::rtb::cuda_fail(e__, #call);         \
     } while (0)
+
+// Runs the body of a C entry point: no C++ exception leaves it.
+template <typename F> int guarded(F body) {
+    try {
+        return body();
+    } catch (const std::bad_alloc &) {
+        return fail(RTB_ERR_ALLOC, "out of host memory");
+    } catch (const std::exception &e) {
+        return fail(RTB_ERR_INVALID, "%s", e.what());
+    }
+}
 
 // ---- dtype properties ------------------------------------------------------------------------
 size_t dtype_size(int dtype);  // 0 for an unknown code

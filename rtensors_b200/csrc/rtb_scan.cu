@@ -1179,76 +1179,82 @@ static size_t count_of(size_t rank, const size_t *shape) {
 
 RTB_API int rtb_gated_scan(rtb_ctx *c, int dtype, int flags, const void *gate, const ptrdiff_t *stride_g, size_t off_g, const void *x,
                            const ptrdiff_t *stride_x, size_t off_x, const void *h0, void *h, size_t rank, const size_t *shape, size_t axis) {
-    int rc = check_scan(c, dtype, flags, rank, shape, axis);
-    if (rc) return rc;
-    const size_t total = count_of(rank, shape);
-    if (total == 0) return RTB_OK;
-    if (!gate || !x || !h || !stride_g || !stride_x) return fail(RTB_ERR_INVALID, "null argument");
-    Ctx *ctx = C(c);
-    if ((rc = use_device(ctx))) return rc;
-    ScanCall call{};
-    call.gate = View{gate, stride_g, off_g};
-    call.b = View{x, stride_x, off_x};
-    call.h0 = h0, call.out = h;
-    return dtype == RTB_F32 ? run_scan<float>(c, ctx, dtype, flags, call, rank, shape, axis, total)
-                            : run_scan<double>(c, ctx, dtype, flags, call, rank, shape, axis, total);
+    return guarded([&]() -> int {
+        int rc = check_scan(c, dtype, flags, rank, shape, axis);
+        if (rc) return rc;
+        const size_t total = count_of(rank, shape);
+        if (total == 0) return RTB_OK;
+        if (!gate || !x || !h || !stride_g || !stride_x) return fail(RTB_ERR_INVALID, "null argument");
+        Ctx *ctx = C(c);
+        if ((rc = use_device(ctx))) return rc;
+        ScanCall call{};
+        call.gate = View{gate, stride_g, off_g};
+        call.b = View{x, stride_x, off_x};
+        call.h0 = h0, call.out = h;
+        return dtype == RTB_F32 ? run_scan<float>(c, ctx, dtype, flags, call, rank, shape, axis, total)
+                                : run_scan<double>(c, ctx, dtype, flags, call, rank, shape, axis, total);
+    });
 }
 
 RTB_API int rtb_gated_scan_backward(rtb_ctx *c, int dtype, int flags, const void *up, const ptrdiff_t *stride_u, size_t off_u,
                                     const void *gate, const ptrdiff_t *stride_g, size_t off_g, const void *x, const ptrdiff_t *stride_x,
                                     size_t off_x, const void *h, const int8_t *codes, const void *mags, const void *h0, void *d_x,
                                     void *d_gate, void *d_h0, size_t rank, const size_t *shape, size_t axis) {
-    int rc = check_scan(c, dtype, flags, rank, shape, axis);
-    if (rc) return rc;
-    const size_t total = count_of(rank, shape), es = dtype_size(dtype);
-    Ctx *ctx = C(c);
-    if (!stride_g) return fail(RTB_ERR_INVALID, "null argument");
-    if (total == 0) {
-        // no step and no upstream: what is left of the gradients is zero
-        if ((rc = use_device(ctx))) return rc;
-        size_t lanes = 1, gate_n = 1;
-        for (size_t k = 0; k < rank; ++k) {
-            if (k != axis) lanes *= shape[k];
-            if (stride_g[k] != 0) gate_n *= shape[k];   // the dims it is broadcast along are summed
+    return guarded([&]() -> int {
+        int rc = check_scan(c, dtype, flags, rank, shape, axis);
+        if (rc) return rc;
+        const size_t total = count_of(rank, shape), es = dtype_size(dtype);
+        Ctx *ctx = C(c);
+        if (!stride_g) return fail(RTB_ERR_INVALID, "null argument");
+        if (total == 0) {
+            // no step and no upstream: what is left of the gradients is zero
+            if ((rc = use_device(ctx))) return rc;
+            size_t lanes = 1, gate_n = 1;
+            for (size_t k = 0; k < rank; ++k) {
+                if (k != axis) lanes *= shape[k];
+                if (stride_g[k] != 0) gate_n *= shape[k];   // the dims it is broadcast along are summed
+            }
+            if (d_h0 && lanes) RTB_CUDA(cudaMemsetAsync(d_h0, 0, lanes * es, ctx->stream));
+            if (d_gate && gate_n) RTB_CUDA(cudaMemsetAsync(d_gate, 0, gate_n * es, ctx->stream));
+            return RTB_OK;
         }
-        if (d_h0 && lanes) RTB_CUDA(cudaMemsetAsync(d_h0, 0, lanes * es, ctx->stream));
-        if (d_gate && gate_n) RTB_CUDA(cudaMemsetAsync(d_gate, 0, gate_n * es, ctx->stream));
-        return RTB_OK;
-    }
-    if (!up || !gate || !stride_u) return fail(RTB_ERR_INVALID, "null argument");
-    if (d_gate && !h && (!codes || !mags)) return fail(RTB_ERR_INVALID, "the gate's gradient needs the states or their checkpoint");
-    if (h && codes) return fail(RTB_ERR_INVALID, "states and a checkpoint of them at once");
-    if (d_gate && (flags & RTB_SCAN_COUPLED) && (!x || !stride_x)) return fail(RTB_ERR_INVALID, "the coupled gate's gradient needs x");
-    if (!d_x && !d_gate && !d_h0) return RTB_OK;
-    if ((rc = use_device(ctx))) return rc;
-    ScanCall call{};
-    call.back = true;
-    call.gate = View{gate, stride_g, off_g};
-    call.b = View{up, stride_u, off_u};
-    call.x = View{x, stride_x, off_x};
-    call.h0 = h0, call.h = h, call.codes = codes, call.mags = mags;
-    call.out = d_x, call.dg = d_gate, call.dh0 = d_h0;
-    return dtype == RTB_F32 ? run_scan<float>(c, ctx, dtype, flags, call, rank, shape, axis, total)
-                            : run_scan<double>(c, ctx, dtype, flags, call, rank, shape, axis, total);
+        if (!up || !gate || !stride_u) return fail(RTB_ERR_INVALID, "null argument");
+        if (d_gate && !h && (!codes || !mags)) return fail(RTB_ERR_INVALID, "the gate's gradient needs the states or their checkpoint");
+        if (h && codes) return fail(RTB_ERR_INVALID, "states and a checkpoint of them at once");
+        if (d_gate && (flags & RTB_SCAN_COUPLED) && (!x || !stride_x)) return fail(RTB_ERR_INVALID, "the coupled gate's gradient needs x");
+        if (!d_x && !d_gate && !d_h0) return RTB_OK;
+        if ((rc = use_device(ctx))) return rc;
+        ScanCall call{};
+        call.back = true;
+        call.gate = View{gate, stride_g, off_g};
+        call.b = View{up, stride_u, off_u};
+        call.x = View{x, stride_x, off_x};
+        call.h0 = h0, call.h = h, call.codes = codes, call.mags = mags;
+        call.out = d_x, call.dg = d_gate, call.dh0 = d_h0;
+        return dtype == RTB_F32 ? run_scan<float>(c, ctx, dtype, flags, call, rank, shape, axis, total)
+                                : run_scan<double>(c, ctx, dtype, flags, call, rank, shape, axis, total);
+    });
 }
 
 RTB_API int rtb_gated_step(rtb_ctx *c, int dtype, int flags, void *state, const ptrdiff_t *stride_s, size_t off_s, const void *gate,
                            const ptrdiff_t *stride_g, size_t off_g, const void *x, const ptrdiff_t *stride_x, size_t off_x, size_t rank,
                            const size_t *shape) {
-    if (!c) return fail(RTB_ERR_INVALID, "null ctx");
-    if (dtype != RTB_F32 && dtype != RTB_F64) return fail(RTB_ERR_DTYPE, "the gated step is defined for f32 and f64 only");
-    if (flags & ~RTB_SCAN_COUPLED) return fail(RTB_ERR_INVALID, "unknown step flags %d", flags);
-    if (rank > RTB_MAX_RANK) return fail(RTB_ERR_DIM, "rank %zu exceeds %d", rank, RTB_MAX_RANK);
-    if (rank && (!shape || !stride_s || !stride_g || !stride_x)) return fail(RTB_ERR_INVALID, "null shape or strides");
-    if (count_of(rank, shape) == 0) return RTB_OK;
-    if (!state || !gate || !x) return fail(RTB_ERR_INVALID, "null argument");
-    for (size_t k = 0; k < rank; ++k)
-        if (stride_s[k] == 0 && shape[k] != 1) return fail(RTB_ERR_SHAPE, "the state's dim %zu is broadcast: it cannot be written", k);
-    Ctx *ctx = C(c);
-    if (int rc = use_device(ctx)) return rc;
-    if (dtype == RTB_F32)
-        return step_any<float>(ctx, flags, (float *)state + off_s, stride_s, (const float *)gate + off_g, stride_g, (const float *)x + off_x,
-                               stride_x, rank, shape);
-    return step_any<double>(ctx, flags, (double *)state + off_s, stride_s, (const double *)gate + off_g, stride_g, (const double *)x + off_x,
-                            stride_x, rank, shape);
+    return guarded([&]() -> int {
+        if (!c) return fail(RTB_ERR_INVALID, "null ctx");
+        if (dtype != RTB_F32 && dtype != RTB_F64) return fail(RTB_ERR_DTYPE, "the gated step is defined for f32 and f64 only");
+        if (flags & ~RTB_SCAN_COUPLED) return fail(RTB_ERR_INVALID, "unknown step flags %d", flags);
+        if (rank > RTB_MAX_RANK) return fail(RTB_ERR_DIM, "rank %zu exceeds %d", rank, RTB_MAX_RANK);
+        if (rank && (!shape || !stride_s || !stride_g || !stride_x)) return fail(RTB_ERR_INVALID, "null shape or strides");
+        if (count_of(rank, shape) == 0) return RTB_OK;
+        if (!state || !gate || !x) return fail(RTB_ERR_INVALID, "null argument");
+        for (size_t k = 0; k < rank; ++k)
+            if (stride_s[k] == 0 && shape[k] != 1) return fail(RTB_ERR_SHAPE, "the state's dim %zu is broadcast: it cannot be written", k);
+        Ctx *ctx = C(c);
+        if (int rc = use_device(ctx)) return rc;
+        if (dtype == RTB_F32)
+            return step_any<float>(ctx, flags, (float *)state + off_s, stride_s, (const float *)gate + off_g, stride_g, (const float *)x + off_x,
+                                   stride_x, rank, shape);
+        return step_any<double>(ctx, flags, (double *)state + off_s, stride_s, (const double *)gate + off_g, stride_g, (const double *)x + off_x,
+                                stride_x, rank, shape);
+    });
 }

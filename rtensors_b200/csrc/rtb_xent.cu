@@ -595,7 +595,7 @@ template <typename T> int pick_size(Ctx *ctx, XentArgs<T> &p, bool vec) {
     if (room <= 512 * 128) return run_cta<T, 512>(ctx, p, 1, vec, room);
     for (unsigned cluster = 1; cluster <= kMaxCluster; cluster *= 2)
         if (room <= (size_t)cluster * 1024 * 128) return run_cta<T, 1024>(ctx, p, cluster, vec, room);
-    const size_t grid = std::min<size_t>(p.rows, (size_t)ctx->sm_count * 4);
+    const size_t grid = std::max<size_t>(1, std::min<size_t>(p.rows, (size_t)ctx->sm_count * 4));
     if (vec) return run<T, xent_twice_kernel<T, N>>(ctx, "xent_twice_kernel", p, grid, 512, 0);
     return run<T, xent_twice_kernel<T, 1>>(ctx, "xent_twice_kernel", p, grid, 512, 0);
 }
@@ -618,14 +618,16 @@ using namespace rtb;
 
 RTB_API int rtb_cross_entropy(rtb_ctx *c, int dtype, const void *logits, size_t rows, size_t classes, ptrdiff_t pitch, const int64_t *targets,
                               int reduction, void *loss, void *grad_map) {
-    if (!c || !loss) return fail(RTB_ERR_INVALID, "null argument");
-    if (dtype != RTB_F32 && dtype != RTB_F64) return fail(RTB_ERR_DTYPE, "cross-entropy is defined for f32 and f64 only");
-    if (reduction != 0 && reduction != 1) return fail(RTB_ERR_INVALID, "reduction must be 0 (mean) or 1 (sum)");
-    if (rows && !targets) return fail(RTB_ERR_INVALID, "null targets");
-    if (rows && classes && !logits) return fail(RTB_ERR_INVALID, "null logits");
-    Ctx *ctx = reinterpret_cast<Ctx *>(c);
-    if (int rc = use_device(ctx)) return rc;
-    if (dtype == RTB_F32)
-        return pick<float>(ctx, (const float *)logits, rows, classes, (int64_t)pitch, targets, reduction == 0, (float *)loss, (float *)grad_map);
-    return pick<double>(ctx, (const double *)logits, rows, classes, (int64_t)pitch, targets, reduction == 0, (double *)loss, (double *)grad_map);
+    return guarded([&]() -> int {
+        if (!c || !loss) return fail(RTB_ERR_INVALID, "null argument");
+        if (dtype != RTB_F32 && dtype != RTB_F64) return fail(RTB_ERR_DTYPE, "cross-entropy is defined for f32 and f64 only");
+        if (reduction != 0 && reduction != 1) return fail(RTB_ERR_INVALID, "reduction must be 0 (mean) or 1 (sum)");
+        if (rows && !targets) return fail(RTB_ERR_INVALID, "null targets");
+        if (rows && classes && !logits) return fail(RTB_ERR_INVALID, "null logits");
+        Ctx *ctx = reinterpret_cast<Ctx *>(c);
+        if (int rc = use_device(ctx)) return rc;
+        if (dtype == RTB_F32)
+            return pick<float>(ctx, (const float *)logits, rows, classes, (int64_t)pitch, targets, reduction == 0, (float *)loss, (float *)grad_map);
+        return pick<double>(ctx, (const double *)logits, rows, classes, (int64_t)pitch, targets, reduction == 0, (double *)loss, (double *)grad_map);
+    });
 }

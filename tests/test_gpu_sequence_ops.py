@@ -348,7 +348,8 @@ def _ce_ref(x, t, mean, u):
     hit = np.arange(classes)[None, :] == t[:, None]
     ok = t >= 0
     n = ok.sum() if mean else 1
-    d = np.where(np.isfinite(x), x - m, 0)
+    # an entry 800 below the maximum has an exponential of zero in either type, in the kernel and here: it adds no error
+    d = np.where(np.isfinite(x), np.maximum(x - m, -800), 0)
     # exp: the argument's rounding and a few units in its result; the sum: a chain of classes / 32 terms, each
     # rescaled at most once per term
     chain = 4 * (classes / 32 + 20)
@@ -356,7 +357,7 @@ def _ce_ref(x, t, mean, u):
     p = e / s
     g = np.where(ok[:, None], (p - hit) / n, 0)
     g_tol = np.where(ok[:, None], (p * rel + 4 * u * np.abs(p - hit)) / n, 0)
-    xt = d[np.arange(rows), np.where(ok, t, 0)]
+    xt = (np.where(np.isfinite(x), x - m, 0))[np.arange(rows), np.where(ok, t, 0)]
     per = np.where(ok, np.log(s[:, 0]) - xt, 0)
     per_tol = np.where(ok, rel.max(axis=1) + 4 * u * (np.abs(np.log(s[:, 0])) + np.abs(xt)), 0)
     return per.sum() / n, per_tol.sum() / n + 4 * u * abs(per.sum() / n), g, g_tol
@@ -584,3 +585,121 @@ def test_on_another_stream_and_in_a_graph():
     assert new != want
     for o in outs:
         assert [v.cpu().numpy().tobytes() for v in o] == new
+
+
+# ---- far ends -------------------------------------------------------------------------------------------------
+
+def test_offsets_beyond_32_bits():
+    """Views that reach past 2^31 elements of a 9 GB buffer: the recurrence on the last channels of long rows, the loss of the last
+    rows, the checkpoint of everything."""
+    from rtensors_b200.meta import Meta
+    from rtensors_b200.tensor import Tensor, cross_entropy_loss
+    be, rows, width = _b(), 70001, 32768
+    buf = torch.zeros(rows * width, device="cuda")
+    rng = np.random.default_rng(15)
+    tail = rng.standard_normal((rows, 5)).astype(np.float32)
+    whole = Tensor(be, buf, Meta.contiguous((rows, width)))
+    buf.view(rows, width)[:, -5:] = torch.from_numpy(tail).cuda()
+    gate = np.full((1, 5), 0.75, np.float32)
+    x = whole.slice(1, width - 5, width)
+    got = x.gated_scan_at(0, _t(gate)).cpu()
+    want, tol = _scan_ref(tail[-300:], gate, 0, None, False, False, U[np.float32])
+    # 300 steps back nothing is left of earlier states: 0.75^300 < 1e-37
+    _close(got[-100:], want[-100:], tol[-100:] + 1e-30)
+    t = np.full(rows, -1)
+    t[-2:] = width - 1, 7
+    loss = cross_entropy_loss(whole, _t(t)).item()
+    v = np.zeros((2, width))
+    v[:, -5:] = tail[-2:]
+    assert abs(loss - _ce_ref(v, t[-2:], True, U[np.float32])[0]) <= _ce_ref(v, t[-2:], True, U[np.float32])[1]
+    ck = whole.checkpoint8()
+    last = ck.restore().buf.view(rows, width)[-2:, -128:].cpu().numpy()
+    assert np.array_equal(last[1], _codes_ref(v[1, -128:].astype(np.float32))[2].astype(np.float32)) and not last[0, :-5].any()
+    del whole, x, ck, buf
+    torch.cuda.empty_cache()
+
+
+@DTYPES
+@pytest.mark.parametrize("rows,classes", [(1, 262144), (2, 262149), (3, 140000), (2, 300001), (5, 2048), (40, 1536), (17, 8191)])
+def test_cross_entropy_of_long_rows(dt, rows, classes):
+    """Clusters of every size, and rows beyond them."""
+    from rtensors_b200.tensor import cross_entropy_loss
+    rng = np.random.default_rng(classes)
+    x = (rng.standard_normal((rows, classes)) * 3).astype(dt)
+    t = rng.integers(0, classes, rows)
+    t[-1] = classes - 1
+    if rows > 2:
+        t[1] = -7
+    loss_w, loss_tol, g_w, g_tol = _ce_ref(x, t, True, U[dt])
+    loss, g = cross_entropy_loss(_t(x), _t(t), True)
+    _close(g.cpu(), g_w, g_tol)
+    assert abs(float(loss.item()) - loss_w) <= loss_tol
+
+
+@DTYPES
+@pytest.mark.parametrize("classes", [3, 40, 700, 1030, 20000, 40001])
+def test_cross_entropy_of_extreme_logits(dt, classes):
+    """Masks of the type's lowest value, alone and with others; logits near the type's largest; far from zero."""
+    from rtensors_b200.tensor import cross_entropy_loss
+    low, rng = np.finfo(dt).min, np.random.default_rng(classes)
+    x = rng.standard_normal((7, classes)).astype(dt)
+    t = rng.integers(0, classes, 7)
+    x[0] = low                                  # nothing but masked: every class alike
+    x[1, ::2] = low
+    t[1] = 1
+    x[2] = low
+    x[2, t[2]] = 0                              # one class left
+    x[3] = -low
+    x[4] = np.where(np.arange(classes) == t[4], dt(3e37), dt(-3e37))
+    x[5] += dt(1000)
+    x[6] -= dt(1000)
+    with np.errstate(over="ignore"):
+        loss_w, loss_tol, g_w, g_tol = _ce_ref(x, t, False, U[dt])
+    loss, g = cross_entropy_loss(_t(x), _t(t), True, "sum")
+    # rows 5 and 6: the shift by 1000 has rounded the inputs themselves, exactly as the restatement reads them
+    _close(g.cpu(), g_w, g_tol)
+    assert abs(float(loss.item()) - loss_w) <= loss_tol + 4 * U[dt] * 1000
+
+
+def test_cross_entropy_map_in_the_logits_place():
+    from rtensors_b200._lib import check, lib
+    be, rng = _b(), np.random.default_rng(16)
+    for rows, classes in ((300, 7), (40, 100), (9, 1000), (30, 2049), (20, 5000), (7, 33001), (3, 150001), (2, 300000)):
+        x = rng.standard_normal((rows, classes)).astype(np.float32)
+        t = torch.from_numpy(rng.integers(-1, classes, rows)).cuda()
+        a, loss = torch.from_numpy(x).cuda(), torch.zeros(2, device="cuda")
+        out = torch.empty_like(a)
+        for k, g in enumerate((out, a)):
+            check(lib().rtb_cross_entropy(be._ctx, 10, a.data_ptr(), rows, classes, classes, t.data_ptr(), 0, loss.data_ptr() + 4 * k, g.data_ptr()))
+        assert torch.equal(out, a) and float(loss[0]) == float(loss[1]) or bool((t < 0).all())
+
+
+def test_two_contexts_at_once():
+    """Two contexts on two streams, their calls interleaved: the same bits as one after the other."""
+    from rtensors_b200.backend import CudaB200
+    from rtensors_b200.meta import Meta
+    from rtensors_b200.tensor import Tensor, cross_entropy_loss, gated_scan_backward
+    rng = np.random.default_rng(17)
+    x, a = rng.standard_normal((2, 3000, 96)).astype(np.float32), rng.uniform(0, 1, (2, 3000, 96)).astype(np.float32)
+    t = rng.integers(0, 96, (2, 3000))
+
+    def run(be):
+        tx, ta, tt = (Tensor(be, torch.from_numpy(v).cuda().view(-1), Meta.contiguous(v.shape)) for v in (x, a, t))
+        outs = []
+        for _ in range(4):
+            h = tx.gated_scan_at(1, ta)
+            loss, g = cross_entropy_loss(h, tt, True)
+            outs += [h.buf, loss.buf, g.buf, *(v.buf for v in gated_scan_backward(g, 1, ta, h.checkpoint8())[:2])]
+        return outs
+    want = [v.cpu().numpy().tobytes() for v in run(_b())]
+    streams, backends, outs = [torch.cuda.Stream() for _ in range(2)], [], []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            backends.append(CudaB200(0))
+            outs.append(run(backends[-1]))
+    torch.cuda.synchronize()
+    for o in outs:
+        assert [v.cpu().numpy().tobytes() for v in o] == want
+    for b in backends:
+        b.close()
