@@ -412,8 +412,9 @@ class CudaB200:
                 raise L.RtbError(L.ERR_SHAPE, f"views of shapes {shape} and {m.shape}")
             m.check_extent(buf.numel())
 
-    def _first_states(self, h0: Optional[torch.Tensor], meta: Meta, axis: int):
-        if h0 is not None and h0.numel() < _lanes(meta, axis):
+    @staticmethod
+    def _first_states(h0: torch.Tensor, meta: Meta, axis: int):
+        if h0.numel() < _lanes(meta, axis):
             raise L.RtbError(L.ERR_BOUNDS, f"h0 needs {_lanes(meta, axis)} elements, its buffer has {h0.numel()}")
 
     def gated_scan(self, x: torch.Tensor, xm: Meta, gate: torch.Tensor, gm: Meta, axis: int, h0: Optional[torch.Tensor] = None,
@@ -421,10 +422,12 @@ class CudaB200:
         """h_s = gate_s h_{s-1} + x_s along `axis` (rtb_gated_scan); gm carries x's shape, stride 0 on broadcast dims; h0 is
         dense over the shape with `axis` as 1.  -> the states, dense row-major."""
         _axis(axis, xm.rank)
-        self._same(x, gate, h0)
+        if gate.dtype is not x.dtype or h0 is not None or x.get_device() != self._index or gate.get_device() != self._index:
+            self._same(x, gate, h0)
         self._views(xm.shape, (x, xm), (gate, gm))
-        self._first_states(h0, xm, axis)
-        out = self.alloc(max(xm.size, 1), x.dtype)
+        if h0 is not None:
+            self._first_states(h0, xm, axis)
+        out = x.new_empty(max(xm.size, 1))
         flags = (L.SCAN_REVERSE if reverse else 0) | (L.SCAN_COUPLED if coupled else 0)
         check(lib().rtb_gated_scan(self._ctx, dtype_code(x), flags, gate.data_ptr(), gm.c_strides, gm.offset,
                                    x.data_ptr(), xm.c_strides, xm.offset, None if h0 is None else h0.data_ptr(), out.data_ptr(),
@@ -441,7 +444,8 @@ class CudaB200:
         _axis(axis, um.rank)
         self._same(up, gate, h, x, h0)
         self._views(um.shape, (up, um), (gate, gm))
-        self._first_states(h0, um, axis)
+        if h0 is not None:
+            self._first_states(h0, um, axis)
         want_x, want_g, want_h0 = want[0], want[1], want[2] and h0 is not None
         n = um.size
         codes = mags = None
@@ -457,15 +461,15 @@ class CudaB200:
                 if x is None:
                     raise L.RtbError(L.ERR_INVALID, "the coupled gate's gradient needs x")
                 self._views(um.shape, (x, xm))
-        dx = self.alloc(max(n, 1), up.dtype) if want_x else None
+        dx = up.new_empty(max(n, 1)) if want_x else None
         dg = dh0 = None
         if want_g:
             n_gate = 1
             for s, st in zip(gm.shape, gm.strides):
                 n_gate *= s if st else 1
-            dg = self.alloc(max(n_gate, 1), up.dtype)
+            dg = up.new_empty(max(n_gate, 1))
         if want_h0:
-            dh0 = self.alloc(max(_lanes(um, axis), 1), up.dtype)
+            dh0 = up.new_empty(max(_lanes(um, axis), 1))
         x_args = (x.data_ptr(), xm.c_strides, xm.offset) if x is not None and coupled and want_g else (None, None, 0)
         check(lib().rtb_gated_scan_backward(
             self._ctx, dtype_code(up), (L.SCAN_REVERSE if reverse else 0) | (L.SCAN_COUPLED if coupled else 0), up.data_ptr(), um.c_strides, um.offset, gate.data_ptr(),
@@ -489,7 +493,7 @@ class CudaB200:
             raise L.RtbError(L.ERR_BOUNDS, f"range [{offset}, {offset + n}) exceeds a buffer of {src.numel()}")
         self._same(src)
         codes = self.alloc(max(n, 1), torch.int8)
-        mags = self.alloc(max(-(-n // L.CKPT8_BLOCK), 1), src.dtype)
+        mags = src.new_empty(max(-(-n // L.CKPT8_BLOCK), 1))
         check(lib().rtb_ckpt8_store(self._ctx, dtype_code(src), src.data_ptr() + offset * src.element_size(), n, codes.data_ptr(), mags.data_ptr()))
         return codes, mags
 
@@ -501,7 +505,7 @@ class CudaB200:
 
     def ckpt8_restore(self, codes: torch.Tensor, mags: torch.Tensor, n: int) -> torch.Tensor:
         self._check_ckpt(codes, mags, n, mags)
-        out = self.alloc(max(n, 1), mags.dtype)
+        out = mags.new_empty(max(n, 1))
         check(lib().rtb_ckpt8_restore(self._ctx, dtype_code(mags), codes.data_ptr(), mags.data_ptr(), n, out.data_ptr()))
         return out
 
@@ -510,7 +514,7 @@ class CudaB200:
         self._check_ckpt(codes, mags, n, up)
         if offset < 0 or offset + n > up.numel():
             raise L.RtbError(L.ERR_BOUNDS, f"range [{offset}, {offset + n}) exceeds a buffer of {up.numel()}")
-        out = self.alloc(max(n, 1), up.dtype)
+        out = up.new_empty(max(n, 1))
         check(lib().rtb_ckpt8_grad(self._ctx, dtype_code(up), kind, codes.data_ptr(), mags.data_ptr(),
                                    up.data_ptr() + offset * up.element_size(), n, out.data_ptr()))
         return out
@@ -527,8 +531,8 @@ class CudaB200:
             raise L.RtbError(L.ERR_INVALID, f"cross-entropy needs {rows} dense int64 targets")
         self._same(logits)
         self._same(targets)
-        loss = self.alloc(1, logits.dtype)
-        g = self.alloc(max(rows * classes, 1), logits.dtype) if with_grad else None
+        loss = logits.new_empty(1)
+        g = logits.new_empty(max(rows * classes, 1)) if with_grad else None
         check(lib().rtb_cross_entropy(self._ctx, dtype_code(logits), logits.data_ptr() + offset * logits.element_size(), rows, classes, pitch,
                                       targets.data_ptr(), reduction, loss.data_ptr(), None if g is None else g.data_ptr()))
         return loss, g

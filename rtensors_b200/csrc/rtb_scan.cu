@@ -793,30 +793,25 @@ template <typename T> __global__ void __launch_bounds__(kThreads) neighbour_sum_
 // Merges the dims of `shape` other than `axis` (axis >= rank: all of them) as far as the strides (null: unused) of out, gate,
 // b, x and dg allow.  -> false when more than kMaxLaneDims remain.
 bool lane_dims(size_t rank, const size_t *shape, size_t axis, const ptrdiff_t *const in[5], LaneDims *out) {
-    std::vector<uint64_t> n;
-    std::vector<int64_t> s[5];
+    int64_t *const to[5] = {out->so, out->sg, out->sb, out->sx, out->sd};
+    int nd = 0;
     for (size_t k = 0; k < rank; ++k) {
         if (k == axis || shape[k] == 1) continue;
-        bool merge = !n.empty();
+        bool merge = nd > 0;
         for (int q = 0; q < 5 && merge; ++q)
-            if (in[q] && s[q].back() != (int64_t)in[q][k] * (int64_t)shape[k]) merge = false;
+            if (in[q] && to[q][nd - 1] != (int64_t)in[q][k] * (int64_t)shape[k]) merge = false;
         if (!merge) {
-            n.push_back(1);
-            for (int q = 0; q < 5; ++q) s[q].push_back(0);
+            if (nd == kMaxLaneDims) return false;
+            out->n[nd++] = 1;
         }
-        n.back() *= shape[k];
-        for (int q = 0; q < 5; ++q) s[q].back() = in[q] ? (int64_t)in[q][k] : 0;
+        out->n[nd - 1] *= shape[k];
+        for (int q = 0; q < 5; ++q) to[q][nd - 1] = in[q] ? (int64_t)in[q][k] : 0;
     }
-    if (n.empty()) {
-        n.push_back(1);
-        for (int q = 0; q < 5; ++q) s[q].push_back(0);
+    if (!nd) {
+        out->n[nd++] = 1;
+        for (int q = 0; q < 5; ++q) to[q][0] = 0;
     }
-    if (n.size() > (size_t)kMaxLaneDims) return false;
-    out->nd = (int)n.size();
-    for (int k = 0; k < out->nd; ++k) {
-        out->n[k] = n[k];
-        out->so[k] = s[0][k], out->sg[k] = s[1][k], out->sb[k] = s[2][k], out->sx[k] = s[3][k], out->sd[k] = s[4][k];
-    }
+    out->nd = nd;
     return true;
 }
 
@@ -972,14 +967,14 @@ struct View {
 // one as well.  Any other view (a transposed one, a negative step) is first copied row-major: one more
 // pass, where reading it in place would fetch a 32-byte sector per element.
 int in_place_or_copy(rtb_ctx *c, int dtype, size_t rank, const size_t *shape, size_t inner_dim, bool must_copy, size_t total,
-                     const std::vector<ptrdiff_t> &dense, View *v, Temp *tmp) {
+                     const ptrdiff_t *dense, View *v, Temp *tmp) {
     const ptrdiff_t s = inner_dim < rank ? v->strides[inner_dim] : 1;
     if (!must_copy && (s == 0 || s == 1)) return RTB_OK;
     int rc = rtb_alloc(c, total * dtype_size(dtype), &tmp->p);
     if (rc) return rc;
     rc = rtb_copy_view(c, dtype, v->p, rank, shape, v->strides, v->offset, tmp->p);
     if (rc) return rc;
-    v->p = tmp->p, v->strides = dense.data(), v->offset = 0;
+    v->p = tmp->p, v->strides = dense, v->offset = 0;
     return RTB_OK;
 }
 
@@ -1042,13 +1037,13 @@ SharedGate shared_gate(size_t rank, const size_t *shape, const ptrdiff_t *stride
 
 template <typename T> int run_scan(rtb_ctx *c, Ctx *ctx, int dtype, int flags, ScanCall call, size_t rank, const size_t *shape, size_t axis,
                                    size_t total) {
-    std::vector<ptrdiff_t> dense(rank);
-    rtb_meta_contiguous_strides(rank, shape, dense.data());
+    ptrdiff_t dense[RTB_MAX_RANK];
+    rtb_meta_contiguous_strides(rank, shape, dense);
     const bool coupled = flags & RTB_SCAN_COUPLED, need_x = call.back && coupled && call.dg;
     bool shared = false;
     if (call.dg)
         for (size_t k = 0; k < rank; ++k) shared = shared || (call.gate.strides[k] == 0 && shape[k] != 1);
-    const std::vector<ptrdiff_t> gate_strides(call.gate.strides, call.gate.strides + rank);
+    const ptrdiff_t *const gate_strides = call.gate.strides;   // as given: a copy of the gate below is not broadcast any more
     // the innermost dim with more than one element decides: the axis itself, or a lane dim
     size_t inner = rank;
     for (size_t k = rank; k-- > 0;)
@@ -1065,7 +1060,7 @@ template <typename T> int run_scan(rtb_ctx *c, Ctx *ctx, int dtype, int flags, S
         if ((rc = in_place_or_copy(c, dtype, rank, shape, inner, copy && !tg.p, total, dense, &call.gate, &tg))) return rc;
         if ((rc = in_place_or_copy(c, dtype, rank, shape, inner, copy && !tb.p, total, dense, &call.b, &tb))) return rc;
         if (need_x && (rc = in_place_or_copy(c, dtype, rank, shape, inner, copy && !tx.p, total, dense, &call.x, &tx))) return rc;
-        const ptrdiff_t *const in[5] = {dense.data(), call.gate.strides, call.b.strides, need_x ? call.x.strides : nullptr, dense.data()};
+        const ptrdiff_t *const in[5] = {dense, call.gate.strides, call.b.strides, need_x ? call.x.strides : nullptr, dense};
         if (lane_dims(rank, shape, axis, in, &p.dims)) break;
     }
     const int64_t steps = (int64_t)shape[axis];
@@ -1090,10 +1085,10 @@ template <typename T> int run_scan(rtb_ctx *c, Ctx *ctx, int dtype, int flags, S
     if (shared) {
         const int in_dim = p.dims.nd - 1;
         const bool segments = vec && p.dims.sg[in_dim] == 0;
-        share = shared_gate(rank, shape, gate_strides.data(), axis, segments ? p.dims.n[in_dim] : 0, segments ? 16 / sizeof(T) * side_by_side<T, 16 / sizeof(T)>(ctx, p) : 1);
+        share = shared_gate(rank, shape, gate_strides, axis, segments ? p.dims.n[in_dim] : 0, segments ? 16 / sizeof(T) * side_by_side<T, 16 / sizeof(T)>(ctx, p) : 1);
         if (share.seg_shift) {
             p.seg_shift = share.seg_shift;
-            const ptrdiff_t *const in[5] = {dense.data(), call.gate.strides, call.b.strides, need_x ? call.x.strides : nullptr, share.strides.data()};
+            const ptrdiff_t *const in[5] = {dense, call.gate.strides, call.b.strides, need_x ? call.x.strides : nullptr, share.strides.data()};
             if (!lane_dims(rank, shape, axis, in, &p.dims)) return fail(RTB_ERR_TOO_LARGE, "gated scan: more than %d dims", kMaxLaneDims);
             p.td = down ? -(int64_t)share.strides[axis] : (int64_t)share.strides[axis];
             p.d0 = down ? (steps - 1) * (int64_t)share.strides[axis] : 0;
