@@ -1,6 +1,7 @@
 """rtensors_b200 -- the rtensors tensor hot path (scalar elementwise ops, N-d broadcast binary ops
 over strided / permuted / negative-step views, axis and full reductions, mean_l1_loss,
-reduce-to-shape) as hand-written CUDA for sm_100a behind a C ABI.
+reduce-to-shape, and for sequence models a gated linear recurrence, 8-bit activation checkpoints and the
+softmax cross-entropy) as hand-written CUDA for sm_100a behind a C ABI.
 
 The compute library is `librt_b200.so` (C ABI in include/rt_b200.h, built by
 `python -m rtensors_b200.build`).  This package is the thin host side: a ctypes binding, the
@@ -21,7 +22,7 @@ def __getattr__(name):
     if name in ("CudaB200", "backend"):
         mod = importlib.import_module(".backend", __name__)
         return mod if name == "backend" else mod.CudaB200
-    if name in ("Tensor", "tensor", "mean_l1_loss"):
+    if name in ("Tensor", "tensor", "mean_l1_loss", "cross_entropy_loss", "gated_scan_backward", "Checkpoint8"):
         mod = importlib.import_module(".tensor", __name__)
         return mod if name == "tensor" else getattr(mod, name)
     raise AttributeError(name)
