@@ -12,6 +12,8 @@
 //                         their pairs through shared memory
 //   beyond                a CTA reads the row twice (the second time mostly from L2)
 // A CTA copies the rows ahead into shared memory, vector by vector as it takes a row's vectors from there into registers.
+// f32 with the map: 8192 x 32000 344 us (6.1 TB/s), 16384 x 8192 203 us (5.3), 2048 x 131072 403 us (5.3, clusters of four),
+// 65536 x 1024 106 us (5.0), 262144 x 64 39 us (3.4); 4096 x 10 7 us, a chain of latencies.
 //
 // A row with t < 0 does not count (padding): its map is zero and its logits are not read.  t >= classes gives NaN for the row
 // and the loss.  Rows are dealt out statically and every sum has a fixed order: results are deterministic.
