@@ -54,6 +54,17 @@ def _lanes(meta: Meta, axis: int) -> int:
     return n
 
 
+# the handle of torch's current stream; the public way builds a Stream object, which takes 2 us of a 10 us call
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def ckpt8_layout(n: int, element_size: int) -> Tuple[int, int]:
+    """(where the magnitudes of an 8-bit checkpoint of n elements begin, bytes of the whole): codes, padded to 16 bytes, then
+    one magnitude for each block."""
+    at = (n + 15) // 16 * 16
+    return at, at + -(-n // L.CKPT8_BLOCK) * element_size
+
+
 class _DeviceBlock:
     """A raw device address as an object torch can wrap without copying (CUDA array interface)."""
 
@@ -392,7 +403,8 @@ class CudaB200:
 
     # -- gated linear recurrence, 8-bit checkpoints, cross-entropy ---------------------------------
     def _same(self, first: torch.Tensor, *rest: Optional[torch.Tensor]):
-        """One dtype, and every buffer on this backend's device (a foreign address would fault inside a kernel)."""
+        """One dtype, and every buffer on this backend's device (a foreign address would fault inside a kernel).  Binds the
+        context to torch's current stream if that has changed."""
         dt, index = first.dtype, self._index
         if first.get_device() != index:
             raise L.RtbError(L.ERR_INVALID, f"a buffer on {first.device} was given to the backend of cuda:{index}")
@@ -403,6 +415,8 @@ class CudaB200:
                 raise L.RtbError(L.ERR_DTYPE, f"operands of {dt} and {t.dtype}")
             if t.get_device() != index:
                 raise L.RtbError(L.ERR_INVALID, f"a buffer on {t.device} was given to the backend of cuda:{index}")
+        if _current_stream(index) != self._stream:
+            self.sync_stream()
 
     @staticmethod
     def _views(shape, *views: Tuple[torch.Tensor, Meta]):
@@ -422,8 +436,7 @@ class CudaB200:
         """h_s = gate_s h_{s-1} + x_s along `axis` (rtb_gated_scan); gm carries x's shape, stride 0 on broadcast dims; h0 is
         dense over the shape with `axis` as 1.  -> the states, dense row-major."""
         _axis(axis, xm.rank)
-        if gate.dtype is not x.dtype or h0 is not None or x.get_device() != self._index or gate.get_device() != self._index:
-            self._same(x, gate, h0)
+        self._same(x, gate, h0)
         self._views(xm.shape, (x, xm), (gate, gm))
         if h0 is not None:
             self._first_states(h0, xm, axis)
@@ -435,11 +448,11 @@ class CudaB200:
         return out
 
     def gated_scan_backward(self, up: torch.Tensor, um: Meta, gate: torch.Tensor, gm: Meta, axis: int,
-                            h: Optional[torch.Tensor] = None, ckpt: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                            h: Optional[torch.Tensor] = None, ckpt: Optional[torch.Tensor] = None,
                             x: Optional[torch.Tensor] = None, xm: Optional[Meta] = None, h0: Optional[torch.Tensor] = None,
                             reverse: bool = False, coupled: bool = False, want: Tuple[bool, bool, bool] = (True, True, True)):
         """Gradients of gated_scan for the upstream `up` of every state (rtb_gated_scan_backward): h is the forward pass's
-        dense result, or ckpt = (codes, mags) its 8-bit checkpoint; x is needed for the coupled gate's gradient.
+        dense result, or ckpt its 8-bit checkpoint (ckpt8_store); x is needed for the coupled gate's gradient.
         -> (d_x, d_gate with the gate's broadcast dims summed, d_h0), None where not wanted (d_h0: without h0)."""
         _axis(axis, um.rank)
         self._same(up, gate, h, x, h0)
@@ -455,8 +468,8 @@ class CudaB200:
             if h is not None and h.numel() < n:
                 raise L.RtbError(L.ERR_BOUNDS, f"{n} states do not fit a buffer of {h.numel()}")
             if ckpt is not None:
-                codes, mags = ckpt
-                self._check_ckpt(codes, mags, n, up)
+                codes = ckpt.data_ptr()
+                mags = codes + self._check_ckpt(ckpt, n, up)
             if coupled:
                 if x is None:
                     raise L.RtbError(L.ERR_INVALID, "the coupled gate's gradient needs x")
@@ -474,7 +487,7 @@ class CudaB200:
         check(lib().rtb_gated_scan_backward(
             self._ctx, dtype_code(up), (L.SCAN_REVERSE if reverse else 0) | (L.SCAN_COUPLED if coupled else 0), up.data_ptr(), um.c_strides, um.offset, gate.data_ptr(),
             gm.c_strides, gm.offset, *x_args, h.data_ptr() if h is not None and want_g else None,
-            None if codes is None else codes.data_ptr(), None if mags is None else mags.data_ptr(),
+            codes, mags,
             None if h0 is None else h0.data_ptr(), None if dx is None else dx.data_ptr(), None if dg is None else dg.data_ptr(),
             None if dh0 is None else dh0.data_ptr(), um.rank, um.c_shape, axis))
         return dx, dg, dh0
@@ -486,36 +499,41 @@ class CudaB200:
         check(lib().rtb_gated_step(self._ctx, dtype_code(state), L.SCAN_COUPLED if coupled else 0, state.data_ptr(), sm.c_strides, sm.offset,
                                    gate.data_ptr(), gm.c_strides, gm.offset, x.data_ptr(), xm.c_strides, xm.offset, sm.rank, sm.c_shape))
 
-    def ckpt8_store(self, src: torch.Tensor, n: Optional[int] = None, offset: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
-        """8-bit checkpoint of n consecutive elements of a buffer (rtb_ckpt8_store) -> (codes, mags)."""
+    def ckpt8_store(self, src: torch.Tensor, n: Optional[int] = None, offset: int = 0) -> torch.Tensor:
+        """8-bit checkpoint of n consecutive elements of a buffer (rtb_ckpt8_store) -> an int8 buffer laid out as ckpt8_layout says."""
         n = src.numel() - offset if n is None else n
         if offset < 0 or n < 0 or offset + n > src.numel():
             raise L.RtbError(L.ERR_BOUNDS, f"range [{offset}, {offset + n}) exceeds a buffer of {src.numel()}")
         self._same(src)
-        codes = self.alloc(max(n, 1), torch.int8)
-        mags = src.new_empty(max(-(-n // L.CKPT8_BLOCK), 1))
-        check(lib().rtb_ckpt8_store(self._ctx, dtype_code(src), src.data_ptr() + offset * src.element_size(), n, codes.data_ptr(), mags.data_ptr()))
-        return codes, mags
-
-    def _check_ckpt(self, codes, mags, n, like):
-        if codes.dtype is not torch.int8 or codes.numel() < n or mags.numel() * L.CKPT8_BLOCK < n or mags.dtype is not like.dtype:
-            raise L.RtbError(L.ERR_BOUNDS, f"the checkpoint does not hold {n} elements of {like.dtype}")
-        self._same(codes)
-        self._same(mags, like)
-
-    def ckpt8_restore(self, codes: torch.Tensor, mags: torch.Tensor, n: int) -> torch.Tensor:
-        self._check_ckpt(codes, mags, n, mags)
-        out = mags.new_empty(max(n, 1))
-        check(lib().rtb_ckpt8_restore(self._ctx, dtype_code(mags), codes.data_ptr(), mags.data_ptr(), n, out.data_ptr()))
+        es = src.element_size()
+        at, total = ckpt8_layout(n, es)
+        out = torch.empty(total or 1, dtype=torch.int8, device=self._torch_device)
+        p = out.data_ptr()
+        check(lib().rtb_ckpt8_store(self._ctx, dtype_code(src), src.data_ptr() + offset * es, n, p, p + at))
         return out
 
-    def ckpt8_grad(self, kind: int, codes: torch.Tensor, mags: torch.Tensor, up: torch.Tensor, n: int, offset: int = 0) -> torch.Tensor:
+    def _check_ckpt(self, ckpt: torch.Tensor, n: int, like: torch.Tensor) -> int:
+        """-> where the magnitudes begin"""
+        at, total = ckpt8_layout(n, like.element_size())
+        if ckpt.dtype is not torch.int8 or ckpt.numel() != (total or 1) or ckpt.get_device() != self._index:
+            raise L.RtbError(L.ERR_BOUNDS, f"not a checkpoint of {n} elements of {like.dtype} on cuda:{self._index}")
+        return at
+
+    def ckpt8_restore(self, ckpt: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
+        out = torch.empty(n or 1, dtype=dtype, device=self._torch_device)
+        self._same(out)
+        p = ckpt.data_ptr()
+        check(lib().rtb_ckpt8_restore(self._ctx, dtype_code(out), p, p + self._check_ckpt(ckpt, n, out), n, out.data_ptr()))
+        return out
+
+    def ckpt8_grad(self, kind: int, ckpt: torch.Tensor, up: torch.Tensor, n: int, offset: int = 0) -> torch.Tensor:
         """f'(restored) * up without writing the restored tensor (rtb_ckpt8_grad); up: n elements from `offset` on."""
-        self._check_ckpt(codes, mags, n, up)
+        self._same(up)
         if offset < 0 or offset + n > up.numel():
             raise L.RtbError(L.ERR_BOUNDS, f"range [{offset}, {offset + n}) exceeds a buffer of {up.numel()}")
-        out = up.new_empty(max(n, 1))
-        check(lib().rtb_ckpt8_grad(self._ctx, dtype_code(up), kind, codes.data_ptr(), mags.data_ptr(),
+        out = up.new_empty(n or 1)
+        p = ckpt.data_ptr()
+        check(lib().rtb_ckpt8_grad(self._ctx, dtype_code(up), kind, p, p + self._check_ckpt(ckpt, n, up),
                                    up.data_ptr() + offset * up.element_size(), n, out.data_ptr()))
         return out
 
@@ -530,7 +548,8 @@ class CudaB200:
         if targets.dtype != torch.int64 or targets.numel() < rows or not targets.is_contiguous():
             raise L.RtbError(L.ERR_INVALID, f"cross-entropy needs {rows} dense int64 targets")
         self._same(logits)
-        self._same(targets)
+        if targets.get_device() != self._index:
+            raise L.RtbError(L.ERR_INVALID, f"targets on {targets.device} were given to the backend of cuda:{self._index}")
         loss = logits.new_empty(1)
         g = logits.new_empty(max(rows * classes, 1)) if with_grad else None
         check(lib().rtb_cross_entropy(self._ctx, dtype_code(logits), logits.data_ptr() + offset * logits.element_size(), rows, classes, pitch,

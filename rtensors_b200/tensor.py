@@ -15,7 +15,7 @@ import torch
 
 from . import _lib as L
 from . import grad as _grad
-from .backend import CODE_TO_NP, CudaB200, dtype_code
+from .backend import CODE_TO_NP, CudaB200, ckpt8_layout, dtype_code
 from .meta import Meta, broadcast_params
 
 _NP_TO_TORCH = {np.dtype(np.float32): torch.float32, np.dtype(np.float64): torch.float64,
@@ -338,8 +338,7 @@ class Tensor:
     def checkpoint8(self) -> "Checkpoint8":
         """The tensor in 8 bits an element (see Checkpoint8), in row-major order of its shape."""
         c = _dense(self)
-        codes, mags = self.backend.ckpt8_store(c.buf, c.size, c.offset)
-        return Checkpoint8(self.backend, codes, mags, self.meta.shape)
+        return Checkpoint8(self.backend, self.backend.ckpt8_store(c.buf, c.meta.size, c.meta.offset), c.buf.dtype, self.meta.shape)
 
 
 class Checkpoint8:
@@ -349,27 +348,36 @@ class Checkpoint8:
 
     KINDS = {"mul": L.CKPT8_MUL, "sigmoid": L.CKPT8_SIGMOID, "tanh": L.CKPT8_TANH, "square": L.CKPT8_SQUARE}
 
-    def __init__(self, backend: CudaB200, codes: torch.Tensor, mags: torch.Tensor, shape):
-        self.backend, self.codes, self.mags = backend, codes, mags
+    def __init__(self, backend: CudaB200, buf: torch.Tensor, dtype: torch.dtype, shape):
+        self.backend, self.buf, self.dtype = backend, buf, dtype
         self.meta = Meta.contiguous(shape)
 
     @property
     def shape(self): return self.meta.shape
     @property
     def size(self): return self.meta.size
+    @property
+    def codes(self) -> torch.Tensor:
+        return self.buf[: self.size]
+    @property
+    def mags(self) -> torch.Tensor:
+        at, total = ckpt8_layout(self.size, self.dtype.itemsize)
+        return self.buf[at: total].view(self.dtype)
 
     def restore(self) -> Tensor:
-        return Tensor(self.backend, self.backend.ckpt8_restore(self.codes, self.mags, self.size), self.meta)
+        return Tensor(self.backend, self.backend.ckpt8_restore(self.buf, self.meta.size, self.dtype), self.meta)
 
     def grad(self, kind: str, upstream: Tensor) -> Tensor:
         """f'(r) * upstream for the restored r, which is never written out: "mul" r u; "sigmoid" r (1 - r) u and "tanh"
         (1 - r r) u with r the op's result; "square" 2 r u with r its input."""
         if kind not in self.KINDS:
             raise L.RtbError(L.ERR_INVALID, f"unknown checkpoint map {kind!r}")
-        if upstream.shape != self.shape:
+        if upstream.meta.shape != self.meta.shape:
             raise L.RtbError(L.ERR_SHAPE, f"an upstream of shape {upstream.shape} for a checkpoint of shape {self.shape}")
+        if upstream.buf.dtype is not self.dtype:
+            raise L.RtbError(L.ERR_DTYPE, f"a checkpoint of {self.dtype} for an upstream of {upstream.buf.dtype}")
         u = _dense(upstream)
-        return Tensor(self.backend, self.backend.ckpt8_grad(self.KINDS[kind], self.codes, self.mags, u.buf, self.size, u.offset), self.meta)
+        return Tensor(self.backend, self.backend.ckpt8_grad(self.KINDS[kind], self.buf, u.buf, self.meta.size, u.meta.offset), self.meta)
 
 
 @lru_cache(maxsize=4096)
@@ -380,7 +388,8 @@ def _spread(meta: Meta, shape) -> Optional[Meta]:
 
 def _is_dense(m: Meta) -> bool:
     """Row-major without gaps (Meta.is_contiguous also takes reversed dims)."""
-    return m.strides == Meta.contiguous(m.shape).strides or m.size == 0
+    c = Meta.contiguous(m.shape)
+    return m is c or m.strides == c.strides or m.size == 0
 
 
 def _dense(t: Tensor, force: bool = False) -> Tensor:
@@ -421,7 +430,9 @@ def gated_scan_backward(upstream: Tensor, axis: int, gate: Tensor, h, x: Optiona
         if h is None or h.shape != upstream.shape:
             raise L.RtbError(L.ERR_SHAPE, f"states of shape {None if h is None else h.shape} for an upstream of shape {upstream.shape}")
         if isinstance(h, Checkpoint8):
-            kept["ckpt"] = (h.codes, h.mags)
+            if h.dtype != upstream.buf.dtype:
+                raise L.RtbError(L.ERR_DTYPE, f"a checkpoint of {h.dtype} for an upstream of {upstream.buf.dtype}")
+            kept["ckpt"] = h.buf
         else:
             h = h if h.offset == 0 and _is_dense(h.meta) else h.contiguous()
             kept["h"] = h.buf

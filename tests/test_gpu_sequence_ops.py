@@ -703,3 +703,27 @@ def test_two_contexts_at_once():
         assert [v.cpu().numpy().tobytes() for v in o] == want
     for b in backends:
         b.close()
+
+
+def test_calls_follow_the_current_stream():
+    """Without sync_stream: a call made under another stream is enqueued there, behind what that stream holds."""
+    from rtensors_b200.backend import CudaB200
+    from rtensors_b200.meta import Meta
+    from rtensors_b200.tensor import Tensor, cross_entropy_loss
+    rng = np.random.default_rng(18)
+    be = CudaB200(0)
+    x, a = rng.standard_normal((4, 500, 64)).astype(np.float32), rng.uniform(0, 1, (4, 500, 64)).astype(np.float32)
+    tx, ta = (Tensor(be, torch.from_numpy(v).cuda().view(-1), Meta.contiguous(v.shape)) for v in (x, a))
+    want = tx.gated_scan_at(1, ta).buf.clone() * 2      # linear: twice the input, twice the states
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)                   # some ten milliseconds
+        tx.buf.mul_(2.0)
+        got = tx.gated_scan_at(1, ta)
+        ck = got.checkpoint8()
+        loss = cross_entropy_loss(got, Tensor(be, torch.zeros(2000, dtype=torch.int64, device="cuda"), Meta.contiguous((4, 500))))
+    side.synchronize()
+    assert torch.equal(got.buf, want) and bool(torch.isfinite(loss.buf).all()) and bool((ck.codes != 0).any())
+    torch.cuda.synchronize()
+    be.close()
