@@ -435,16 +435,20 @@ class CudaB200:
                    reverse: bool = False, coupled: bool = False) -> torch.Tensor:
         """h_s = gate_s h_{s-1} + x_s along `axis` (rtb_gated_scan); gm carries x's shape, stride 0 on broadcast dims; h0 is
         dense over the shape with `axis` as 1.  -> the states, dense row-major."""
-        _axis(axis, xm.rank)
-        self._same(x, gate, h0)
-        self._views(xm.shape, (x, xm), (gate, gm))
-        if h0 is not None:
-            self._first_states(h0, xm, axis)
+        i, rank = self._index, len(xm.shape)
+        _axis(axis, rank)
+        if gate.dtype is not x.dtype or h0 is not None or x.get_device() != i or gate.get_device() != i or _current_stream(i) != self._stream:
+            self._same(x, gate, h0)
+            if h0 is not None:
+                self._first_states(h0, xm, axis)
+        if gm.shape != xm.shape:
+            self._views(xm.shape, (gate, gm))
+        xm.check_extent(x.numel()); gm.check_extent(gate.numel())
         out = x.new_empty(max(xm.size, 1))
         flags = (L.SCAN_REVERSE if reverse else 0) | (L.SCAN_COUPLED if coupled else 0)
         check(lib().rtb_gated_scan(self._ctx, dtype_code(x), flags, gate.data_ptr(), gm.c_strides, gm.offset,
                                    x.data_ptr(), xm.c_strides, xm.offset, None if h0 is None else h0.data_ptr(), out.data_ptr(),
-                                   xm.rank, xm.c_shape, axis))
+                                   rank, xm.c_shape, axis))
         return out
 
     def gated_scan_backward(self, up: torch.Tensor, um: Meta, gate: torch.Tensor, gm: Meta, axis: int,
@@ -494,8 +498,13 @@ class CudaB200:
 
     def gated_step(self, state: torch.Tensor, sm: Meta, gate: torch.Tensor, gm: Meta, x: torch.Tensor, xm: Meta, coupled: bool = False):
         """One step of the recurrence in place: state = gate state + x over views of one shape (rtb_gated_step)."""
-        self._same(state, gate, x)
-        self._views(sm.shape, (state, sm), (gate, gm), (x, xm))
+        i, dt = self._index, state.dtype
+        if gate.dtype is not dt or x.dtype is not dt or state.get_device() != i or gate.get_device() != i or x.get_device() != i or \
+                _current_stream(i) != self._stream:
+            self._same(state, gate, x)
+        if gm.shape != sm.shape or xm.shape != sm.shape:
+            self._views(sm.shape, (gate, gm), (x, xm))
+        sm.check_extent(state.numel()); gm.check_extent(gate.numel()); xm.check_extent(x.numel())
         check(lib().rtb_gated_step(self._ctx, dtype_code(state), L.SCAN_COUPLED if coupled else 0, state.data_ptr(), sm.c_strides, sm.offset,
                                    gate.data_ptr(), gm.c_strides, gm.offset, x.data_ptr(), xm.c_strides, xm.offset, sm.rank, sm.c_shape))
 

@@ -322,9 +322,11 @@ class Tensor:
         """The gated linear recurrence h_s = gate_s h_{s-1} + x_s along `axis`, x being this tensor: descending with
         `reverse`, h_s = gate_s h_{s-1} + (1 - gate_s) x_s with `coupled`.  gate broadcasts to x's shape; h0 is the state
         in front of the first step, x's shape with `axis` as 1 (zero without it).  -> every state."""
-        gate, gm, h0 = _scan_operands(self, axis, gate, h0)
-        out = Tensor(self.backend, self.backend.gated_scan(self.buf, self.meta, gate.buf, gm, axis, None if h0 is None else h0.buf,
-                                                           reverse, coupled), Meta.contiguous(self.shape))
+        m, gm = self.meta, gate.meta
+        if h0 is not None or gm.shape != m.shape or 0 in gm.strides:
+            gate, gm, h0 = _scan_operands(self, axis, gate, h0)
+        out = Tensor(self.backend, self.backend.gated_scan(self.buf, m, gate.buf, gm, axis, None if h0 is None else h0.buf, reverse, coupled),
+                     Meta.contiguous(m.shape))
         if _grad.is_enabled():
             _grad.attach_scan(out, self, gate, h0, axis, reverse, coupled)
         return out
