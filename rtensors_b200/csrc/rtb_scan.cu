@@ -457,6 +457,118 @@ __global__ void __launch_bounds__(kThreads, 2) scan_lanes_kernel(const __grid_co
     if (nc > 1) cluster_barrier();   // no CTA leaves while another may still write to it
 }
 
+// ---- lanes contiguous, and so many of them that a thread for each V fills the device; or only a few steps ------------
+// A thread walks its V lanes from end to end, kAhead steps loaded before they are needed: nothing is exchanged.  The gate of a step
+// serves the next one of the backward pass too, so it is read once.  HBM-bound, and more steps ahead open more DRAM pages at
+// once than they hide latency: 1000 x 64 x 1024 f32 forward 134 us with 2 (5.9 TB/s), 164 with 3, 193 with 4; backward 206 us with 1
+// (6.4 TB/s), 231 with 2, 261 with 4.
+template <typename T, int V, int MODE, bool COUPLED, bool GVEC>
+__global__ void __launch_bounds__(kThreads) scan_walk_kernel(const __grid_constant__ ScanArgs<T> p) {
+    constexpr bool kBack = MODE != kForward;
+    constexpr int kAhead = kBack ? 1 : V > 1 ? 2 : 3, VA = GVEC ? V : 1;
+    using P = Pack<T, V>;
+    using PA = Pack<T, VA>;
+    grid_dep_sync();
+    const uint64_t first_lane = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) * V;
+    const bool active = first_lane < p.lanes;
+    const LaneAt at = locate(p.dims, active ? first_lane : 0, p.seg_shift);
+    const int steps = (int)p.steps;
+    const bool need_h = kBack && p.dg;
+    const bool writes_sum = ((threadIdx.x * V) & ((1 << p.seg_shift) - 1)) == 0;
+    const T *in_g = p.g + at.g, *in_b = p.b + at.b, *in_h = kBack && MODE == kBackDense ? p.h + p.o0 + at.o + p.to : nullptr;
+    const T *in_x = kBack && COUPLED ? p.x + at.x : nullptr;
+    int64_t in_c = p.o0 + at.o + p.to;
+    T *to_o = p.out + p.o0 + at.o, *to_d = p.dg + p.d0 + at.d;
+    PA gate[kAhead], before;
+    P b[kAhead], hp[kBack ? kAhead : 1], x[kBack && COUPLED ? kAhead : 1];
+    auto load = [&](int k, int s) {   // step s, into place k
+        if (!active || s >= steps) return;
+        if constexpr (GVEC) gate[k] = ld<T, VA>(in_g);
+        else gate[k].e[0] = *in_g;
+        b[k] = ld<T, V>(in_b);
+        in_g += p.tg, in_b += p.tb;
+        if constexpr (kBack) {
+            if (need_h) {
+                if (s + 1 < steps) {
+                    if constexpr (MODE == kBackDense) hp[k] = ld<T, V>(in_h);
+                    else Ckpt8Scale<T>(p.mags[in_c >> kCkpt8Shift]).template restore<V>(codes_at<V>(p.codes + in_c), hp[k].e);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) hp[k].e[j] = p.h0 ? p.h0[first_lane + j] : (T)0;
+                }
+                if constexpr (MODE == kBackDense) in_h += p.to;
+                else in_c += p.to;
+                if constexpr (COUPLED) x[k] = ld<T, V>(in_x), in_x += p.tx;
+            }
+        }
+    };
+    auto of = [](const PA &v, int j) { return v.e[GVEC ? j : 0]; };
+    P c;
+#pragma unroll
+    for (int j = 0; j < V; ++j) c.e[j] = !kBack && p.h0 && active ? p.h0[first_lane + j] : (T)0;
+#pragma unroll
+    for (int j = 0; j < VA; ++j) before.e[j] = (T)0;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) load(k, k);
+    for (int s0 = 0; s0 < steps; s0 += kAhead) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int s = s0 + k;
+            if (s >= steps) break;   // the same in all threads
+            const PA a = gate[k];
+            const P in = b[k];
+            P d;
+            if constexpr (kBack) {
+                if (need_h) {
+                    d = hp[k];
+                    if constexpr (COUPLED) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) d.e[j] = d.e[j] - x[k].e[j];
+                    }
+                }
+            }
+            load(k, s + kAhead);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                if constexpr (kBack) c.e[j] = fma_(of(before, j), c.e[j], in.e[j]);
+                else c.e[j] = fma_(of(a, j), c.e[j], COUPLED ? ((T)1 - of(a, j)) * in.e[j] : in.e[j]);
+            }
+            if constexpr (!kBack) {
+                if (active) st<T, V>(to_o, c);
+            } else {
+                before = a;
+                if (active && p.out) {
+                    P o = c;
+                    if constexpr (COUPLED) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) o.e[j] = ((T)1 - of(a, j)) * c.e[j];
+                    }
+                    st<T, V>(to_o, o);
+                }
+                if (need_h) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) d.e[j] = active ? c.e[j] * d.e[j] : (T)0;
+                    if (p.seg_shift == 0) {
+                        if (active) st<T, V>(to_d, d);
+                    } else {
+                        T sum = d.e[0];
+#pragma unroll
+                        for (int j = 1; j < V; ++j) sum += d.e[j];
+                        for (int m = 1; m < (1 << p.seg_shift) / V; m <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+                        if (active && writes_sum) *to_d = sum;
+                    }
+                    to_d += p.td;
+                }
+                if (active && p.dh0 && s + 1 == steps) {
+#pragma unroll
+                    for (int j = 0; j < V; ++j) p.dh0[first_lane + j] = of(a, j) * c.e[j];
+                }
+            }
+            to_o += p.to;
+        }
+    }
+}
+
 // ---- the axis itself contiguous ---------------------------------------------------------------------------
 // A warp takes K runs of 32 V consecutive steps of one lane; within a run a thread holds V steps, and the threads' maps
 // are scanned across the warp by shuffles.  TEAM warps share a lane: one walks it alone (many lanes, no barrier at all), or a
@@ -872,6 +984,14 @@ template <typename T, int V> int side_by_side(const Ctx *ctx, const ScanArgs<T> 
     return groups * kMaxCluster * 2 <= (uint64_t)ctx->sm_count ? 4 : 8;
 }
 
+// A thread for each V lanes where rounds would leave most rows of a CTA idle (few steps), or where there are threads enough to
+// fill the device: f32, rounds / walk: (244, 61, 2048) with 16 heads, forward 150 / 54 us, backward 211 / 70 us; (100, 20, 1024)
+// 24 / 9 us; (300, 200, 1024) forward 150 / 164 us, backward 392 / 227 us; (150, 200, 1024) forward 79 / 142 us.
+template <typename T, int V> bool walks(const Ctx *ctx, const ScanArgs<T> &p, bool back) {
+    const uint64_t threads = p.lanes / V / (uint64_t)ctx->sm_count;   // on each SM
+    return p.steps <= 16 || (threads >= 64 && p.steps <= 64) || (threads >= 512 && (back || p.steps <= 128));
+}
+
 // Steps of a thread, with two stages of the ring.  More steps make fewer rounds, each of which costs the same exchange, and take
 // more registers and shared memory (beyond 104 KB one CTA fits an SM, not two).  us at 65536 x 1024 and, behind the slash,
 // 8 x 8192 x 1024, f32, per channel or with one gate for 64 or 128 channels:
@@ -882,6 +1002,12 @@ template <typename T, int V> int side_by_side(const Ctx *ctx, const ScanArgs<T> 
 // By elements, at 8 x 8192 x 1023: forward 8: 186, 12: 192, 16: 191 (shared 16: 171, 8: 218); backward 8: 344, 12: 359, 16: 482.
 template <typename T, int V, int MODE, bool COUPLED, bool GVEC> int run_lanes(Ctx *ctx, ScanArgs<T> &p) {
     constexpr bool back = MODE != kForward;
+    if (walks<T, V>(ctx, p, back)) {
+        const uint64_t grid = (p.lanes + (uint64_t)kThreads * V - 1) / ((uint64_t)kThreads * V);
+        if (grid > kMaxGrid) return fail(RTB_ERR_TOO_LARGE, "gated scan: %zu sequences are beyond one launch", (size_t)p.lanes);
+        launch_dep(ctx, (unsigned)grid, kThreads, scan_walk_kernel<T, V, MODE, COUPLED, GVEC>, p);
+        return check_launch(ctx, "scan_walk_kernel");
+    }
     if constexpr (V == 1) {
         constexpr int R = sizeof(T) == 4 ? (back || GVEC ? 8 : 16) : (back ? 4 : GVEC ? 6 : 8);
         if (side_by_side<T, 1>(ctx, p) == 8) return run_width<T, 1, 8, R, 2, MODE, COUPLED, GVEC>(ctx, p);
@@ -1090,7 +1216,7 @@ template <typename T> int run_scan(rtb_ctx *c, Ctx *ctx, int dtype, int flags, S
     if (shared) {
         const int in_dim = p.dims.nd - 1;
         const bool segments = vec && p.dims.sg[in_dim] == 0;
-        share = shared_gate(rank, shape, gate_strides, axis, segments ? p.dims.n[in_dim] : 0, segments ? 16 / sizeof(T) * side_by_side<T, 16 / sizeof(T)>(ctx, p) : 1);
+        share = shared_gate(rank, shape, gate_strides, axis, segments ? p.dims.n[in_dim] : 0, !segments ? 1 : 16 / sizeof(T) * (walks<T, 16 / sizeof(T)>(ctx, p, true) ? 32 : side_by_side<T, 16 / sizeof(T)>(ctx, p)));
         if (share.seg_shift) {
             p.seg_shift = share.seg_shift;
             const ptrdiff_t *const in[5] = {dense, call.gate.strides, call.b.strides, need_x ? call.x.strides : nullptr, share.strides.data()};

@@ -727,3 +727,48 @@ def test_calls_follow_the_current_stream():
     assert torch.equal(got.buf, want) and bool(torch.isfinite(loss.buf).all()) and bool((ck.codes != 0).any())
     torch.cuda.synchronize()
     be.close()
+
+
+@DTYPES
+@pytest.mark.parametrize("coupled,reverse,heads", [(False, False, 0), (True, True, 0), (False, True, 4), (True, False, 4)])
+@pytest.mark.parametrize("shape", [(700, 16, 64), (257, 17, 132), (160, 61, 256), (400, 3, 1000), (40, 9, 31 * 4)])
+def test_many_lanes_and_few_steps(dt, coupled, reverse, heads, shape):
+    """Sizes where a thread walks its lanes alone, at whole vectors and odd ends; heads share a gate."""
+    from rtensors_b200.tensor import gated_scan_backward
+    b, n, d = shape
+    full = (b, n, heads, d // heads) if heads else shape
+    gate = (b, n, heads, 1) if heads else shape
+    rng, x, a, first = _data(dt, full, gate, 1, True, seed=3)
+    tx, ta, t0 = _t(x), _t(a), _t(first)
+    _close(tx.gated_scan_at(1, ta, t0, reverse=reverse, coupled=coupled).cpu(), *_scan_ref(x, a, 1, first, reverse, coupled, U[dt]))
+    up, h = rng.standard_normal(full).astype(dt), rng.standard_normal(full).astype(dt)
+    ck = _t(h).checkpoint8()
+    for kept, values in ((_t(h), h), (ck, ck.restore().cpu())):
+        want = _scan_back_ref(up, a, 1, values, x, first, reverse, coupled, U[dt])
+        got = gated_scan_backward(_t(up), 1, ta, kept, tx if coupled else None, t0, reverse, coupled)
+        for g, w in zip(got, want):
+            _close(g.cpu(), *w)
+
+
+@pytest.mark.parametrize("d", [256, 255])
+def test_very_many_lanes_agree_with_a_few_at_a_time(d):
+    """Enough lanes that a thread walks each; the same lanes in parts go by rounds.  With gates of at most 0.9 and |values| <= 1 a
+    state's A is 10 at most and E 2 u A / (1 - 0.9), so each way is within (20 + 24) u 10 of the exact states, twice that apart."""
+    from rtensors_b200.meta import Meta
+    from rtensors_b200.tensor import Tensor, gated_scan_backward
+    be, b, n = _b(), 1250 if d == 256 else 320, 70
+    g = torch.Generator(device="cuda")
+    g.manual_seed(d)
+    x, a, up, h = (torch.rand(b, n, d, device="cuda", generator=g) * 2 - 1 for _ in range(4))
+    a = (a + 1) * 0.45
+
+    def run(lo, hi):
+        t = [Tensor(be, v[lo:hi].contiguous().view(-1), Meta.contiguous((hi - lo, n, d))) for v in (x, a, up, h)]
+        states = t[0].gated_scan_at(1, t[1], coupled=True)
+        dx, da, _ = gated_scan_backward(t[2], 1, t[1], t[3], t[0], coupled=True)
+        return [v.buf.view(hi - lo, n, d) for v in (states, dx, da)]
+    whole = run(0, b)
+    for lo in range(0, b, 50):
+        for got, part in zip(whole, run(lo, min(lo + 50, b))):
+            # da multiplies by two values of at most 1 each
+            assert float((got[lo: lo + 50] - part).abs().max()) <= 2 * 2 * 44 * 2.0 ** -24 * 10
