@@ -98,7 +98,7 @@ template <typename A, void (*kernel)(A)> int allow_smem(Ctx *ctx, size_t smem) {
     return RTB_OK;
 }
 
-// How many clusters of `cluster` CTAs (1, 2, 4 or 8) of a kernel an idle device runs at once.  Asked once per device and size.
+// How many clusters of `cluster` CTAs (1 to 8) of a kernel an idle device runs at once.  Asked once per device and size.
 template <typename A, void (*kernel)(A)> int clusters_at_once(Ctx *ctx, unsigned threads, unsigned cluster, size_t smem, unsigned *out) {
     static std::atomic<unsigned> known[64][9];
     std::atomic<unsigned> &mark = known[ctx->device & 63][cluster];

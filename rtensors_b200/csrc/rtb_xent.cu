@@ -571,7 +571,7 @@ template <typename T, int THREADS, int NV, int AHEAD, bool ALIGNED> int run_rows
 // Rows that need six vectors of a thread at most leave room to copy two rows ahead.
 template <typename T, int THREADS> int run_cta(Ctx *ctx, XentArgs<T> &p, unsigned cluster, bool vec, size_t room) {
     p.cluster = cluster;
-    if (cluster == 1 && room <= (size_t)THREADS * 6 * 16)
+    if (room <= (size_t)cluster * THREADS * 6 * 16)
         return vec ? run_rows<T, THREADS, 6, 2, true>(ctx, p) : run_rows<T, THREADS, 6, 2, false>(ctx, p);
     return vec ? run_rows<T, THREADS, 8, 1, true>(ctx, p) : run_rows<T, THREADS, 8, 1, false>(ctx, p);
 }
@@ -595,7 +595,7 @@ template <typename T> int pick_size(Ctx *ctx, XentArgs<T> &p, bool vec) {
     if (room <= 128 * 128) return run_cta<T, 128>(ctx, p, 1, vec, room);
     if (room <= 256 * 128) return run_cta<T, 256>(ctx, p, 1, vec, room);
     if (room <= 512 * 128) return run_cta<T, 512>(ctx, p, 1, vec, room);
-    for (unsigned cluster = 1; cluster <= kMaxCluster; cluster *= 2)
+    for (unsigned cluster = 1; cluster <= kMaxCluster; ++cluster)
         if (room <= (size_t)cluster * 1024 * 128) return run_cta<T, 1024>(ctx, p, cluster, vec, room);
     const size_t grid = std::max<size_t>(1, std::min<size_t>(p.rows, (size_t)ctx->sm_count * 4));
     if (vec) return run<T, xent_twice_kernel<T, N>>(ctx, "xent_twice_kernel", p, grid, 512, 0);
