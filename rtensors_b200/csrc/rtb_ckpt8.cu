@@ -1,8 +1,8 @@
 // 8-bit activation checkpoints (format: rtb_ckpt8.cuh): store, restore, and the backward maps of the tape's nodes
 // fed from codes, so that the restored tensor never exists in memory.  All HBM-bound: f32 moves 5 bytes per
-// element to store or restore, 9 to apply a map.  A warp holds a block (four elements a lane), four blocks at a time so that
-// their loads are in flight together; a block's magnitude is one warp-wide maximum of bit patterns.  67M f32: store 64 us
-// (5.2 TB/s; its chain from load over maximum and reciprocal to code is the longest), restore 52 us (6.4), a map 90 us (6.7).
+// element to store or restore, 9 to apply a map.  A warp holds a block (four elements a lane), several blocks at a time so that
+// their loads are in flight together; a block's magnitude is one warp-wide maximum of bit patterns.  67M f32: store 54 us
+// (6.2 TB/s), restore 52 us (6.4), a map 90 us (6.7); 34M f64: 49, 48 and 86 us.
 #include "rtb_internal.h"
 #include "rtb_ckpt8.cuh"
 
@@ -11,8 +11,13 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kUnroll = 4;                                  // blocks of a warp, loads of all in flight at once
-constexpr int kTileBlocks = kWarps * kUnroll;
+constexpr int kUnroll = 4;   // blocks of a warp, loads of all in flight at once
+
+// The store's chain from load over maximum and reciprocal to code is long, so warps in flight count for more than registers:
+// blocks of a warp, CTAs of an SM.  67M f32: 54 us at 7 or 8 CTAs, 58 at 6, 64 as the compiler chooses; 34M f64: 49 at 8, 51 at 6.
+template <typename T> struct StoreShape;
+template <> struct StoreShape<float> { static constexpr int unroll = 4, ctas = 7; };
+template <> struct StoreShape<double> { static constexpr int unroll = 2, ctas = 8; };
 
 // max |x| of a block.  A NaN wins (max.NaN), and as bits NaN > inf > every finite magnitude, so one comparison tells.
 template <typename T> struct Bits;
@@ -37,13 +42,10 @@ template <> struct Bits<double> {
     }
     static __device__ __forceinline__ U bits(double x) { return (U)__double_as_longlong(x) & 0x7fffffffffffffffull; }
     static __device__ __forceinline__ double value(U u) { return __longlong_as_double((long long)u); }
-    static __device__ __forceinline__ U warp_max(U u) {
-#pragma unroll
-        for (int d = 16; d; d >>= 1) {
-            const U v = __shfl_xor_sync(0xffffffffu, u, d);
-            u = v > u ? v : u;
-        }
-        return u;
+    static __device__ __forceinline__ U warp_max(U u) {   // the high words' maximum, then the low words' among the lanes that hold it
+        const uint32_t hi = (uint32_t)(u >> 32), top_hi = __reduce_max_sync(0xffffffffu, hi);
+        const uint32_t top_lo = __reduce_max_sync(0xffffffffu, hi == top_hi ? (uint32_t)u : 0u);
+        return ((U)top_hi << 32) | top_lo;
     }
 };
 
@@ -75,11 +77,15 @@ struct Quantise32 {
         return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     }
 };
-// f64: the quotient as IEEE arithmetic gives it; the product with the reciprocal decides all but the values within 1e-9 of a tie.
+// f64: the quotient as IEEE arithmetic gives it; the product with a reciprocal decides all but the values within 1e-8 of a tie.  An
+// approximate reciprocal within 2^-18, refined once by Newton's step, is within 2^-36, and 127 times that is below 2e-9.
 struct Quantise64 {
     double m, inv, down;
     bool wide;
-    __device__ __forceinline__ explicit Quantise64(double mag) : m(mag), inv(127.0 / mag), down(1.0), wide(!(mag > 1e-280 && mag < 1e300)) {
+    __device__ __forceinline__ explicit Quantise64(double mag) : m(mag), down(1.0), wide(!(mag > 1e-280 && mag < 1e300)) {
+        double r;
+        asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(r) : "d"(mag));
+        inv = 127.0 * fma(r, fma(-mag, r, 1.0), r);
         if (mag > 1e300) m = mag * 0x1p-20, down = 0x1p-20;   // 127 x stays finite
     }
     __device__ __forceinline__ uint32_t codes(const double x[4]) const {
@@ -92,7 +98,7 @@ struct Quantise64 {
             c[k] = (uint32_t)__double2loint(t);
             off = fmax(off, fabs(fma(x[k], inv, magic - t)));
         }
-        if (wide || off > 0.499999999) {
+        if (wide || off > 0.49999999) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) c[k] = m > 0.0 ? (uint32_t)(int)rint(127.0 * (x[k] * down) / m) : 0u;
         }
@@ -151,15 +157,16 @@ __device__ __forceinline__ void store_codes(int8_t *p, size_t i, size_t n, uint3
 }
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) ckpt8_store_kernel(const T *src, size_t n, int8_t *codes, T *mags) {
+__global__ void __launch_bounds__(kThreads, StoreShape<T>::ctas) ckpt8_store_kernel(const T *src, size_t n, int8_t *codes, T *mags) {
+    constexpr int U = StoreShape<T>::unroll;
     const int lane = threadIdx.x & 31;
-    const size_t block0 = ((size_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * kUnroll;
+    const size_t block0 = ((size_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * U;
     grid_dep_sync();
-    T v[kUnroll][4];
+    T v[U][4];
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) load4<T, VEC>(src, (block0 + u) * kCkpt8Block + lane * 4, n, v[u]);
+    for (int u = 0; u < U; ++u) load4<T, VEC>(src, (block0 + u) * kCkpt8Block + lane * 4, n, v[u]);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
+    for (int u = 0; u < U; ++u) {
         using B = Bits<T>;
         const size_t i = (block0 + u) * kCkpt8Block + lane * 4;
         const typename B::U top = B::warp_max(B::bits(B::top(B::top(v[u][0], v[u][1]), B::top(v[u][2], v[u][3]))));
@@ -211,8 +218,8 @@ __global__ void __launch_bounds__(kThreads) ckpt8_read_kernel(const int8_t *code
     }
 }
 
-int tiles(size_t n, unsigned *grid) {
-    const size_t blocks = (n + kCkpt8Block - 1) / kCkpt8Block, g = (blocks + kTileBlocks - 1) / kTileBlocks;
+int tiles(size_t n, int unroll, unsigned *grid) {
+    const size_t blocks = (n + kCkpt8Block - 1) / kCkpt8Block, tile = (size_t)kWarps * unroll, g = (blocks + tile - 1) / tile;
     if (g > 0x7fffffffu) return fail(RTB_ERR_TOO_LARGE, "checkpoint of %zu elements is beyond one launch", n);
     *grid = (unsigned)g;
     return RTB_OK;
@@ -222,7 +229,7 @@ template <typename T> bool aligned4(const T *p) { return ((uintptr_t)p & (4 * si
 
 template <typename T> int store_typed(Ctx *ctx, const T *src, size_t n, int8_t *codes, T *mags) {
     unsigned grid = 0;
-    if (int rc = tiles(n, &grid)) return rc;
+    if (int rc = tiles(n, StoreShape<T>::unroll, &grid)) return rc;
     if (aligned4(src)) launch_dep(ctx, grid, kThreads, ckpt8_store_kernel<T, true>, src, n, codes, mags);
     else launch_dep(ctx, grid, kThreads, ckpt8_store_kernel<T, false>, src, n, codes, mags);
     return check_launch(ctx, "ckpt8_store_kernel");
@@ -230,7 +237,7 @@ template <typename T> int store_typed(Ctx *ctx, const T *src, size_t n, int8_t *
 
 template <typename T, int KIND> int read_typed(Ctx *ctx, const int8_t *codes, const T *mags, const T *up, size_t n, T *dst) {
     unsigned grid = 0;
-    if (int rc = tiles(n, &grid)) return rc;
+    if (int rc = tiles(n, kUnroll, &grid)) return rc;
     if (aligned4(up) && aligned4(dst)) launch_dep(ctx, grid, kThreads, ckpt8_read_kernel<T, KIND, true>, codes, mags, up, n, dst);
     else launch_dep(ctx, grid, kThreads, ckpt8_read_kernel<T, KIND, false>, codes, mags, up, n, dst);
     return check_launch(ctx, "ckpt8_read_kernel");
