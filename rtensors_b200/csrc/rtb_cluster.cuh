@@ -6,6 +6,7 @@
 namespace rtb {
 
 constexpr unsigned kMaxCluster = 8;                     // the portable size
+constexpr unsigned kWideCluster = 16;                   // what a kernel may opt in to; a device need not be able to place it
 constexpr unsigned long long kWaitNs = 2000000000ull;   // limit of a wait for another CTA's values
 constexpr uint64_t kMaxGrid = 0x7fffffffull;
 
@@ -98,13 +99,15 @@ template <typename A, void (*kernel)(A)> int allow_smem(Ctx *ctx, size_t smem) {
     return RTB_OK;
 }
 
-// How many clusters of `cluster` CTAs (1 to 8) of a kernel an idle device runs at once.  Asked once per device and size.
+// How many clusters of `cluster` CTAs (1 to 16) of a kernel an idle device runs at once; above 8 it may be none, and a size must
+// have been asked for before it is launched.  Asked once per device and size.
 template <typename A, void (*kernel)(A)> int clusters_at_once(Ctx *ctx, unsigned threads, unsigned cluster, size_t smem, unsigned *out) {
-    static std::atomic<unsigned> known[64][9];
+    static std::atomic<unsigned> known[64][kWideCluster + 1];   // one more than the answer
     std::atomic<unsigned> &mark = known[ctx->device & 63][cluster];
     unsigned n = mark.load(std::memory_order_relaxed);
     if (!n) {
         if (int rc = allow_smem<A, kernel>(ctx, smem)) return rc;
+        if (cluster > kMaxCluster) RTB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
         int got = 0;
         if (cluster == 1) {
             RTB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&got, kernel, (int)threads, smem));
@@ -121,10 +124,10 @@ template <typename A, void (*kernel)(A)> int clusters_at_once(Ctx *ctx, unsigned
             cfg.numAttrs = 1;
             RTB_CUDA(cudaOccupancyMaxActiveClusters(&got, kernel, &cfg));
         }
-        n = got > 0 ? (unsigned)got : 1;
+        n = got > 0 ? (unsigned)got + 1 : cluster > kMaxCluster ? 1 : 2;
         mark.store(n, std::memory_order_relaxed);
     }
-    *out = n;
+    *out = n - 1;
     return RTB_OK;
 }
 

@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(kThreads, 2) scan_axis_kernel(const __grid_con
     constexpr bool kBack = MODE != kForward;
     extern __shared__ __align__(16) unsigned char ring[];
     __shared__ T warp_a[2][kWarps], warp_h[2][kWarps];
-    __shared__ alignas(16) Pack<T, 2> cta_maps[2][kMaxCluster];
+    __shared__ alignas(16) Pack<T, 2> cta_maps[2][kWideCluster];
     __shared__ unsigned long long arrived[2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const unsigned nc = TEAM > 1 ? p.cluster : 1, rank = nc > 1 ? cluster_rank() : 0;
@@ -945,13 +945,16 @@ template <int V> bool strides_whole(const LaneDims &d, const int64_t *s, int64_t
 constexpr uint64_t kShortElements = 1u << 24;   // launches of some 30 us gain more from an early start than they lose
 
 // How many CTAs share a group: as many as run at once, as long as each has a part of its own.  `smem` says what a size needs.
+// f32, up to 8 in powers of two / any number up to 16: forward (1, 65536, 64) 56 / 34 us, (1, 32768, 768) 79 / 69 us,
+// (1, 16384, 512) 39 / 33 us, backward 81 / 47, 126 / 105 and 65 / 48 us; one lane of 1000000 55 / 31 and 102 / 55 us;
+// (1, 65536, 1024), 8 either way.
 template <typename T, void (*kernel)(ScanArgs<T>), typename F> int cluster_for(Ctx *ctx, uint64_t groups, uint64_t steps, uint64_t part, F smem, unsigned *out) {
     unsigned n = 1;
-    while (n < kMaxCluster && steps > (uint64_t)n * part) {
+    while (n < kWideCluster && steps > (uint64_t)n * part) {
         unsigned fit = 0;
-        if (int rc = clusters_at_once<ScanArgs<T>, kernel>(ctx, kThreads, n * 2, smem(n * 2), &fit)) return rc;
+        if (int rc = clusters_at_once<ScanArgs<T>, kernel>(ctx, kThreads, n + 1, smem(n + 1), &fit)) return rc;
         if (groups > fit) break;
-        n *= 2;
+        ++n;
     }
     *out = n;
     return RTB_OK;
@@ -974,7 +977,7 @@ template <typename T, int V, int LX, int R, int STAGES, int MODE, bool COUPLED, 
 
 // Threads side by side in a group.  With vectors, 8 give rows of 128 bytes, a full line, and the most steps a round can have with
 // them; 4 double the steps again where groups of 8, in clusters of the largest size, would leave most SMs without work.  Measured,
-// f32: (1, 65536, 128) 112 us with 8, 76 with 4; (8, 8192, 1024) 142 us with 8, 171 with 4, 152 with 16, 155 with 32.
+// f32, at up to 8 CTAs: (1, 65536, 128) 112 us with 8, 76 with 4; (8, 8192, 1024) 142 us with 8, 171 with 4, 152 with 16, 155 with 32.
 // By elements (V = 1), 32 give the full line, and 8 serve few lanes: (8, 8192, 1023) 186 us with 32, 212 with 8; (1, 40000, 75)
 // 90 us with 32, 34 with 8.
 template <typename T, int V> int side_by_side(const Ctx *ctx, const ScanArgs<T> &p) {

@@ -772,3 +772,22 @@ def test_very_many_lanes_agree_with_a_few_at_a_time(d):
         for got, part in zip(whole, run(lo, min(lo + 50, b))):
             # da multiplies by two values of at most 1 each
             assert float((got[lo: lo + 50] - part).abs().max()) <= 2 * 2 * 44 * 2.0 ** -24 * 10
+
+
+@DTYPES
+@pytest.mark.parametrize("coupled,reverse", [(False, False), (True, True)])
+@pytest.mark.parametrize("shape,gate_shape,axis", [((1, 24001, 20), None, 1), ((1, 5000, 300), None, 1), ((1, 13001, 33), None, 1), ((2, 9000, 8, 16), (2, 9000, 8, 1), 1),
+                                                   ((3, 1, 70003), None, 2), ((1, 1, 65536), None, 2), ((2, 4100, 640), (2, 4100, 1), 1)])
+def test_few_lanes_and_many_steps(dt, coupled, reverse, shape, gate_shape, axis):
+    """Sizes where clusters of every size up to the widest share a group of lanes."""
+    from rtensors_b200.tensor import gated_scan_backward
+    rng, x, a, first = _data(dt, shape, gate_shape or shape, axis, True, seed=5)
+    tx, ta, t0 = _t(x), _t(a), _t(first)
+    _close(tx.gated_scan_at(axis, ta, t0, reverse=reverse, coupled=coupled).cpu(), *_scan_ref(x, a, axis, first, reverse, coupled, U[dt]))
+    up, h = rng.standard_normal(shape).astype(dt), rng.standard_normal(shape).astype(dt)
+    ck = _t(h).checkpoint8()
+    for kept, values in ((_t(h), h), (ck, ck.restore().cpu())):
+        want = _scan_back_ref(up, a, axis, values, x, first, reverse, coupled, U[dt])
+        got = gated_scan_backward(_t(up), axis, ta, kept, tx if coupled else None, t0, reverse, coupled)
+        for g, w in zip(got, want):
+            _close(g.cpu(), *w)
