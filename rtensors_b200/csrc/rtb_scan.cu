@@ -942,7 +942,11 @@ template <int V> bool strides_whole(const LaneDims &d, const int64_t *s, int64_t
     return true;
 }
 
-constexpr uint64_t kShortElements = 1u << 24;   // launches of some 30 us gain more from an early start than they lose
+// A grid that starts beside its predecessor's last CTAs (programmatic dependent launch) saves up to 3 us, but takes whatever SMs are free and
+// keeps them: more than a few rounds long, it loses more.  Backward, early / not: f32 (1, 65536, 256) with 4 heads, 11 rounds,
+// 126 / 78 us; f64 (1, 32768, 128) with 2 heads, 6 rounds, 74 / 48 us; f32 (16, 256, 512), 2 rounds, 14.6 / 16.7 us.  Warps that
+// walk a lane alone wait for nobody: early up to some 30 us, (4, 512, 8192) along the contiguous axis 35 / 38 us.
+constexpr uint64_t kEarlyRounds = 4, kEarlyElements = 1u << 24;
 
 // How many CTAs share a group: as many as run at once, as long as each has a part of its own.  `smem` says what a size needs.
 // f32, up to 8 in powers of two / any number up to 16: forward (1, 65536, 64) 56 / 34 us, (1, 32768, 768) 79 / 69 us,
@@ -972,19 +976,22 @@ template <typename T, int V, int LX, int R, int STAGES, int MODE, bool COUPLED, 
     p.bytes = {p.tg * es, p.tb * es, p.tx * es, p.to * es, p.td * es};
     p.round_bytes = {p.tg * n, p.tb * n, p.tx * n, p.to * n, p.td * n};
     return launch_cluster<ScanArgs<T>, kernel>(ctx, "scan_lanes_kernel", groups * p.cluster, kThreads, p.cluster, smem(p.cluster),
-                                               p.lanes * p.steps <= kShortElements, p);
+                                               p.steps <= kEarlyRounds * p.cluster * part, p);
 }
 
 // Threads side by side in a group.  With vectors, 8 give rows of 128 bytes, a full line, and the most steps a round can have with
-// them; 4 double the steps again where groups of 8, in clusters of the largest size, would leave most SMs without work.  Measured,
-// f32, at up to 8 CTAs: (1, 65536, 128) 112 us with 8, 76 with 4; (8, 8192, 1024) 142 us with 8, 171 with 4, 152 with 16, 155 with 32.
-// By elements (V = 1), 32 give the full line, and 8 serve few lanes: (8, 8192, 1023) 186 us with 32, 212 with 8; (1, 40000, 75)
-// 90 us with 32, 34 with 8.
-template <typename T, int V> int side_by_side(const Ctx *ctx, const ScanArgs<T> &p) {
+// them; 4 double the steps again where groups of 8 in the widest clusters would leave SMs without work or get too few CTAs each.
+// 4 / 8, f32: (1, 65536, D) forward D = 64 35 / 57 us, 256 71 / 90, 512 97 / 108, 640 119 / 113; backward 512 153 / 171, 576 197 / 171;
+// (8, 8192, 1024) forward 171 / 142.  Where neighbours' sums are formed, 4 add fewer of them in the kernel: backward 256, 4 heads 78 / 90,
+// 384, 6 heads 95 / 94, 512, 32 heads 134 / 123.
+// By elements (V = 1), 32 give the full line, and 8 serve few lanes: (8, 8192, 1023) 186 us with 32, 212 with 8; (1, 40000, D) forward
+// D = 75 55 us with 32, 25 with 8; 301 74 and 54; backward 601 167 and 182.
+template <typename T, int V> int side_by_side(const Ctx *ctx, const ScanArgs<T> &p, bool back) {
     constexpr int wide = V == 1 ? 32 : 8;
-    const uint64_t groups = (p.lanes + wide * V - 1) / (wide * V);
-    if (V == 1) return groups * kMaxCluster < (uint64_t)ctx->sm_count ? 8 : 32;
-    return groups * kMaxCluster * 2 <= (uint64_t)ctx->sm_count ? 4 : 8;
+    const uint64_t groups = (p.lanes + wide * V - 1) / (wide * V), sms = (uint64_t)ctx->sm_count;
+    if (V == 1) return groups * kMaxCluster < sms ? 8 : 32;
+    const bool sums = back && p.dims.sg[p.dims.nd - 1] == 0;   // whether or not they are wanted: dx has the same bits
+    return groups * (sums ? 12 : 9) <= sms ? 4 : 8;
 }
 
 // A thread for each V lanes where rounds would leave most rows of a CTA idle (few steps), or where there are threads enough to
@@ -1013,11 +1020,11 @@ template <typename T, int V, int MODE, bool COUPLED, bool GVEC> int run_lanes(Ct
     }
     if constexpr (V == 1) {
         constexpr int R = sizeof(T) == 4 ? (back || GVEC ? 8 : 16) : (back ? 4 : GVEC ? 6 : 8);
-        if (side_by_side<T, 1>(ctx, p) == 8) return run_width<T, 1, 8, R, 2, MODE, COUPLED, GVEC>(ctx, p);
+        if (side_by_side<T, 1>(ctx, p, back) == 8) return run_width<T, 1, 8, R, 2, MODE, COUPLED, GVEC>(ctx, p);
         return run_width<T, 1, 32, R, 2, MODE, COUPLED, GVEC>(ctx, p);
     } else {
         constexpr int R = GVEC ? (back ? (COUPLED ? 3 : MODE == kBackDense ? 6 : 4) : 6) : (back ? (COUPLED ? 4 : 6) : 8);
-        if (side_by_side<T, V>(ctx, p) == 4) return run_width<T, V, 4, R, 2, MODE, COUPLED, GVEC>(ctx, p);
+        if (side_by_side<T, V>(ctx, p, back) == 4) return run_width<T, V, 4, R, 2, MODE, COUPLED, GVEC>(ctx, p);
         if constexpr (!back && GVEC)   // many lanes: no clusters, the exchange is cheap
             if (p.lanes >= (uint64_t)ctx->sm_count * 8 * V) return run_width<T, V, 8, 4, 2, MODE, COUPLED, GVEC>(ctx, p);
         return run_width<T, V, 8, R, 2, MODE, COUPLED, GVEC>(ctx, p);
@@ -1053,10 +1060,11 @@ template <typename T, int MODE, bool COUPLED, bool VEC> int run_axis(Ctx *ctx, S
     p.cluster = 1;
     // A warp for each lane wherever that gives every SM eight, or one part is all there is; else a CTA or a cluster.
     if (p.lanes >= (uint64_t)ctx->sm_count * kWarps || p.steps <= Ring::kTile)
-        return launch_cluster<ScanArgs<T>, scan_axis_kernel<T, V, K, S, 1, MODE, COUPLED, VEC>>(ctx, "scan_axis_kernel", (p.lanes + kWarps - 1) / kWarps, kThreads, 1, smem, p.lanes * p.steps <= kShortElements, p);
+        return launch_cluster<ScanArgs<T>, scan_axis_kernel<T, V, K, S, 1, MODE, COUPLED, VEC>>(ctx, "scan_axis_kernel", (p.lanes + kWarps - 1) / kWarps, kThreads, 1, smem, p.lanes * p.steps <= kEarlyElements, p);
     constexpr auto team = scan_axis_kernel<T, V, K, S, kWarps, MODE, COUPLED, VEC>;
-    if (int rc = cluster_for<T, team>(ctx, p.lanes, p.steps, (uint64_t)kWarps * Ring::kTile, [](unsigned) { return smem; }, &p.cluster)) return rc;
-    return launch_cluster<ScanArgs<T>, team>(ctx, "scan_axis_kernel", p.lanes * p.cluster, kThreads, p.cluster, smem, p.lanes * p.steps <= kShortElements, p);
+    constexpr uint64_t part = (uint64_t)kWarps * Ring::kTile;
+    if (int rc = cluster_for<T, team>(ctx, p.lanes, p.steps, part, [](unsigned) { return smem; }, &p.cluster)) return rc;
+    return launch_cluster<ScanArgs<T>, team>(ctx, "scan_axis_kernel", p.lanes * p.cluster, kThreads, p.cluster, smem, p.steps <= kEarlyRounds * p.cluster * part, p);
 }
 
 template <typename T, int MODE, bool COUPLED> int pick_axis(Ctx *ctx, ScanArgs<T> &p) {
@@ -1219,7 +1227,7 @@ template <typename T> int run_scan(rtb_ctx *c, Ctx *ctx, int dtype, int flags, S
     if (shared) {
         const int in_dim = p.dims.nd - 1;
         const bool segments = vec && p.dims.sg[in_dim] == 0;
-        share = shared_gate(rank, shape, gate_strides, axis, segments ? p.dims.n[in_dim] : 0, !segments ? 1 : 16 / sizeof(T) * (walks<T, 16 / sizeof(T)>(ctx, p, true) ? 32 : side_by_side<T, 16 / sizeof(T)>(ctx, p)));
+        share = shared_gate(rank, shape, gate_strides, axis, segments ? p.dims.n[in_dim] : 0, !segments ? 1 : 16 / sizeof(T) * (walks<T, 16 / sizeof(T)>(ctx, p, true) ? 32 : side_by_side<T, 16 / sizeof(T)>(ctx, p, true)));
         if (share.seg_shift) {
             p.seg_shift = share.seg_shift;
             const ptrdiff_t *const in[5] = {dense, call.gate.strides, call.b.strides, need_x ? call.x.strides : nullptr, share.strides.data()};
