@@ -53,19 +53,20 @@ __device__ __forceinline__ double warp_max(double v) {
     return v;
 }
 
-// Sums of exponentials are kept relative to a shift c: s = sum of exp(x) / e^c.  f64: c is a maximum of the logits.  f32: powers of
-// two, c = rint(m log2 e) and s = sum of 2^(x log2 e - c): one fused multiply-add rounds each exponent once, and bringing
-// sums to a common shift is exact.  Logits beyond 1e37, whose product with log2 e may overflow, are first taken
-// relative to m itself; their shifts stay apart from each other and in order.  c = -inf: no logit above -inf yet.
-// A NaN is skipped by the maximum and kept by the sum.
-constexpr float kLog2e = 1.4426950408889634f, kFar = 1e37f;
+// Sums of exponentials are kept relative to a shift c that depends on a maximum m of the logits alone.  f64: c = m, s = sum of
+// exp(x - m).  f32, |m| <= kNear: powers of two, 2c = rint(m log2 e) and s = sum of 2^(x log2 e - 2c): one fused multiply-add rounds each
+// exponent once, and bringing sums to a common shift is exact.  That needs m log2 e below 2^23: its own rounding, which stays in every
+// exponent, is then a quarter at most (from 2^31 on it would be 128 and more, an overflow).  f32 beyond kNear, masks of
+// -1e9 and the like: c = m and s = sum of exp(x - m), as in f64.  The near shifts are halved so that |c| <= 0.73 kNear: a shift tells of
+// which kind it is, shifts have the order of their maxima, and those of different far maxima differ.
+// c = -inf: no logit above -inf yet.  A NaN is skipped by the maximum and kept by the sum.
+constexpr float kLog2e = 1.4426950408889634f, kNear = 4194304.0f;   // 2^22
 template <typename T> struct alignas(2 * sizeof(T)) Lse {
     T c, s;
 };
-__device__ __forceinline__ float shift_of(float m) {
-    if (m == -INFINITY) return m;
-    return fabsf(m) <= kFar ? rintf(m * kLog2e) : m * 0.9f + copysignf(kFar, m);
-}
+__device__ __forceinline__ bool is_far(float c) { return fabsf(c) > kNear; }   // of a maximum or of its shift
+__device__ __forceinline__ bool is_far(double) { return false; }
+__device__ __forceinline__ float shift_of(float m) { return is_far(m) ? m : 0.5f * rintf(m * kLog2e); }
 __device__ __forceinline__ double shift_of(double m) { return m; }
 __device__ __forceinline__ float exp2_(float x) {
     float y;
@@ -74,40 +75,45 @@ __device__ __forceinline__ float exp2_(float x) {
 }
 // what a sum of shift c is multiplied by to have the shift `top` >= c
 __device__ __forceinline__ float rescale(float c, float top) {
-    if (c == -INFINITY) return 1.0f;
-    const float d = c - top;   // a whole number
-    return d >= -126.0f ? __int_as_float(((int)d + 127) << 23) : (d == d ? 0.0f : d);
+    if (fmaxf(fabsf(c), fabsf(top)) > kNear) {   // log2 of e^c / e^top, whichever way either is written
+        const bool fc = is_far(c), ft = is_far(top);
+        const float d = fmaf(fc ? (ft ? c - top : c) : -top, kLog2e, fc ? (ft ? 0.0f : -2.0f * top) : 2.0f * c);
+        return c == -INFINITY ? 1.0f : exp2_(d);
+    }
+    const float d = 2.0f * (c - top);   // a whole number
+    return d >= -126.0f ? __int_as_float(((int)d + 127) << 23) : 0.0f;
 }
 __device__ __forceinline__ double rescale(double c, double top) { return c == -(double)INFINITY ? 1.0 : exp(c - top); }
-__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar && m != -INFINITY; }
-__device__ __forceinline__ bool is_far(double) { return false; }
-// exponential of x relative to the shift c, or, far out, to the maximum itself
-__device__ __forceinline__ float exp_near(float x, float c) { return exp2_(fmaf(x, kLog2e, -c)); }
+// exponential of x relative to a near shift, given as 2c, or to the maximum itself
+__device__ __forceinline__ float exp_near(float x, float c2) { return exp2_(fmaf(x, kLog2e, -c2)); }
 __device__ __forceinline__ float exp_far(float x, float m) { return exp2_((x - m) * kLog2e); }
-__device__ __forceinline__ double exp_near(double x, double c) { return exp(x - c); }
+__device__ __forceinline__ double exp_near(double x, double m) { return exp(x - m); }
 __device__ __forceinline__ double exp_far(double x, double m) { return exp(x - m); }
+__device__ __forceinline__ float near_base(float shift) { return 2.0f * shift; }
+__device__ __forceinline__ double near_base(double shift) { return shift; }
 // x becomes the exponentials of N values
 template <typename T, int N> __device__ __forceinline__ Lse<T> lse_of(T (&x)[N]) {
     T m[4] = {lowest<T>(), lowest<T>(), lowest<T>(), lowest<T>()}, s[4] = {};
 #pragma unroll
     for (int k = 0; k < N; ++k) m[k % 4] = max_(m[k % 4], x[k]);
     const T top = max_(max_(m[0], m[1]), max_(m[2], m[3]));
-    if (is_far(top)) {
+    const T shift = shift_of(top);
+    if (is_far(top) && top != lowest<T>()) {
 #pragma unroll
         for (int k = 0; k < N; ++k) x[k] = exp_far(x[k], top);
     } else {
-        const T c = top == lowest<T>() ? (T)0 : shift_of(top);
+        const T base = top == lowest<T>() ? (T)0 : near_base(shift);
 #pragma unroll
-        for (int k = 0; k < N; ++k) x[k] = exp_near(x[k], c);
+        for (int k = 0; k < N; ++k) x[k] = exp_near(x[k], base);
     }
 #pragma unroll
     for (int k = 0; k < N; ++k) s[k % 4] += x[k];
-    return Lse<T>{shift_of(top), (s[0] + s[1]) + (s[2] + s[3])};
+    return Lse<T>{shift, (s[0] + s[1]) + (s[2] + s[3])};
 }
 // log(sum of exponentials) - target: without cancellation where the target is near the maximum.  p: its softmax
 __device__ __forceinline__ float minus_log(const Lse<float> &l, float target, float p) {
-    if (fabsf(l.c) > kFar) return -logf(p);
-    return 0.6931471805599453f * (log2f(l.s) - fmaf(target, kLog2e, -l.c));
+    if (is_far(l.c)) return -logf(p);
+    return 0.6931471805599453f * (log2f(l.s) - fmaf(target, kLog2e, -2.0f * l.c));
 }
 __device__ __forceinline__ double minus_log(const Lse<double> &l, double target, double) { return log(l.s) - (target - l.c); }
 

@@ -1,0 +1,79 @@
+"""The softmax cross-entropy over the whole range of the type: masks of any common value over all classes of a thread, maxima far
+from zero, maxima that differ by the type's last bit.
+
+Tolerances are those of the general test, roundings counted per exponential and per sum.  Far from zero x - m, its product with
+log2 e and that constant round once each, 2.3 u |x - m| in all, within the 2 u |x - m| + 88 u counted there as long as the exponential is
+not zero.  Exponentials below the smallest normal number count as zero: `tiny` more in the map."""
+import numpy as np
+import pytest
+
+from test_gpu_sequence_ops import DTYPES, U, _ce_ref, _close, _t
+
+pytestmark = pytest.mark.gpu
+
+# a class count for each way a row is dealt out: a thread, some threads of a warp (whole vectors and not), a CTA of every kind, clusters, a
+# CTA that reads the row twice
+CLASSES = [10, 20, 63, 250, 700, 701, 1023, 1500, 5000, 8191, 20000, 40000, 40001, 140000, 262149, 300000]
+
+
+def _check(x, t, reduction="sum"):
+    from rtensors_b200.tensor import cross_entropy_loss
+    dt = x.dtype.type
+    with np.errstate(over="ignore"):
+        loss_w, loss_tol, g_w, g_tol = _ce_ref(x, t, reduction == "mean", U[dt])
+    loss, g = cross_entropy_loss(_t(x), _t(t), True, reduction)
+    _close(g.cpu(), g_w, g_tol + 2 * float(np.finfo(dt).tiny))
+    assert abs(float(loss.item()) - loss_w) <= loss_tol
+    assert cross_entropy_loss(_t(x), _t(t), reduction=reduction).cpu().tobytes() == loss.cpu().tobytes()
+
+
+@DTYPES
+@pytest.mark.parametrize("classes", CLASSES)
+def test_masks_over_whole_threads(dt, classes):
+    """An ordinary row with all but a few classes masked, whatever the mask's value."""
+    rng = np.random.default_rng(classes)
+    fills = [-1e4, -1e7, -1e9, -3e9, -1e10, -1e12, -1e18, -1e20, -1e30, -1e36]
+    x = rng.standard_normal((len(fills), classes)).astype(dt)
+    t = np.zeros(len(fills), np.int64)
+    for r, fill in enumerate(fills):
+        left = rng.choice(classes, 3, replace=False)
+        masked = np.ones(classes, bool)
+        masked[left] = False
+        x[r, masked] = fill
+        t[r] = left[0]
+    _check(x, t)
+    _check(x, t, "mean")
+
+
+@DTYPES
+@pytest.mark.parametrize("classes", CLASSES)
+@pytest.mark.parametrize("sign", [1, -1])
+def test_maxima_far_from_zero(dt, classes, sign):
+    """Rows around +-1e6 ... +-1e37, next to each other in steps of the type, and on both sides of a power of two."""
+    rng = np.random.default_rng(classes + 1)
+    around = [1e6, 2.0 ** 22, 6e6, 3e7, 1e9, 2.0 ** 30, 3e9, 1e10, 1e12, 1e20, 1e30, 9e36, 1.2e38]
+    x = np.empty((len(around), classes), dt)
+    t = np.empty(len(around), np.int64)
+    for r, v in enumerate(around):
+        step = max(float(np.spacing(dt(v))), 1.0)
+        # a few steps above and below, most of them equal: ties of the maximum in different threads
+        x[r] = sign * v + step * np.minimum(rng.integers(-6, 4, classes), 1)
+        t[r] = int(np.argmax(x[r]))
+    _check(x, t)
+
+
+@pytest.mark.parametrize("classes", [20, 700, 5000, 40000, 140000, 300000])
+@pytest.mark.parametrize("base", [1.2e38, -1.2e38, 1.5e37, -2.5e37, 3.4e38, 5e9])
+def test_maxima_one_step_apart_stay_apart(classes, base):
+    """Beyond 2^30 one step is 64 and more: only the larger of two neighbouring floats counts, in whichever thread it is."""
+    base, rng = np.float32(base), np.random.default_rng(classes + 2)
+    x = np.empty((20, classes), np.float32)
+    t = np.empty(20, np.int64)
+    for r in range(20):
+        above = np.nextafter(base, np.float32(np.inf))
+        assert float(above) - float(base) >= 64
+        x[r] = base
+        t[r] = rng.integers(0, classes)
+        x[r, t[r]] = above
+        base = above if base < 0 or r < 10 else base
+    _check(x, t)
