@@ -110,12 +110,14 @@ template <typename T, int N> __device__ __forceinline__ Lse<T> lse_of(T (&x)[N])
     for (int k = 0; k < N; ++k) s[k % 4] += x[k];
     return Lse<T>{shift, (s[0] + s[1]) + (s[2] + s[3])};
 }
-// log(sum of exponentials) - target: without cancellation where the target is near the maximum.  p: its softmax
-__device__ __forceinline__ float minus_log(const Lse<float> &l, float target, float p) {
-    if (is_far(l.c)) return -logf(p);
+// log(sum of exponentials) - target, without cancellation where the target is near the maximum.  Far from zero in 64 bits: in f32 the
+// distance of a masked target times log2 e, or the sum of such losses, would overflow though the loss or the mean fits.
+__device__ __forceinline__ double minus_log(const Lse<float> &l, float target) {
+    if (is_far(l.c)) return (double)logf(l.s) + ((double)l.c - (double)target);
+    if (is_far(target)) return 0.6931471805599453 * ((double)log2f(l.s) + (2.0 * (double)l.c - (double)target * (double)kLog2e));
     return 0.6931471805599453f * (log2f(l.s) - fmaf(target, kLog2e, -2.0f * l.c));
 }
-__device__ __forceinline__ double minus_log(const Lse<double> &l, double target, double) { return log(l.s) - (target - l.c); }
+__device__ __forceinline__ double minus_log(const Lse<double> &l, double target) { return log(l.s) - (target - l.c); }
 
 // number of rows that count, as kCountCtas partial counts
 __global__ void __launch_bounds__(256) xent_count_kernel(const int64_t *targets, size_t rows, unsigned long long *counts) {
@@ -247,19 +249,15 @@ __global__ void __launch_bounds__(256) xent_warp_kernel(const __grid_constant__ 
                 } else {
                     e[k] = x[j];
                 }
-#pragma unroll
-                for (int i = 0; i < N; ++i)
-                    if ((int)j + i == tt) xt = e[k * N + i], mine_t = true;
             } else {
 #pragma unroll
                 for (int i = 0; i < N; ++i) e[k * N + i] = lowest<T>();
             }
         }
-        const Lse<T> own = lse_of(e);
-        T et = (T)0;
 #pragma unroll
         for (int k = 0; k < NV * N; ++k)
-            if ((k / N * TPR + in_row) * N + k % N == tt) et = e[k];
+            if ((k / N * TPR + in_row) * N + k % N == tt) xt = e[k], mine_t = counted;
+        const Lse<T> own = lse_of(e);
         // the row's shift first: one rescaling, then a plain sum
         T top = own.c;
 #pragma unroll
@@ -269,7 +267,7 @@ __global__ void __launch_bounds__(256) xent_warp_kernel(const __grid_constant__ 
 #pragma unroll
         for (int d = TPR / 2; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (counted) {
-            if (mine_t) mine.loss += (double)minus_log(Lse<T>{top, sum}, xt, et * f / sum);
+            if (mine_t) mine.loss += minus_log(Lse<T>{top, sum}, xt);
             if (bad && in_row == 0) mine.loss = NAN;
             if (in_row == 0) mine.rows += 1;
         }
@@ -444,7 +442,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) xent_cta_kernel(const
 #pragma unroll
                 for (int k = 0; k < NV * N; ++k)
                     if (k / N * kStep + k % N == tt) et = e[k];
-                mine.loss += (double)minus_log(Lse<T>{c, sum}, xt, et * to_p);
+                mine.loss += minus_log(Lse<T>{c, sum}, xt);
             }
             if (p.map) {
                 T *g = p.map + r * p.classes;
@@ -523,7 +521,7 @@ __global__ void __launch_bounds__(512) xent_twice_kernel(const __grid_constant__
         for (int w = 0; w < kWarps; ++w) sum += pairs[w].c == lowest<T>() ? pairs[w].s : pairs[w].s * exp_(pairs[w].c - m);
         const bool bad = (uint64_t)t >= p.classes;
         if (threadIdx.x == 0) {
-            mine.loss += bad ? (double)NAN : (double)(log_(sum) - (x[t] - m));
+            mine.loss += bad ? (double)NAN : (double)log_(sum) - ((double)x[t] - (double)m);
             mine.rows += 1;
         }
         __syncthreads();   // the pairs are written again for the next row, x[t] may be overwritten below

@@ -77,3 +77,34 @@ def test_maxima_one_step_apart_stay_apart(classes, base):
         x[r, t[r]] = above
         base = above if base < 0 or r < 10 else base
     _check(x, t)
+
+
+@DTYPES
+@pytest.mark.parametrize("classes", CLASSES)
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_targets_far_below_the_maximum(dt, classes, reduction):
+    """A masked target has a loss as large as its distance from the maximum: finite as long as the type can hold it."""
+    rng = np.random.default_rng(classes + 3)
+    low = float(np.finfo(dt).min)
+    rows = [(0.0, -200.0), (1.0, -1e6), (3.0, -5e6), (-4.1e6, -4.3e6), (0.0, -1e10), (5e9, -5e9), (0.0, -2.4e38), (1.0, low), (3e37, -3e37),
+            (2.0 ** 22, -2.0 ** 22), (1e37, -1e37), (low / 4, low)]
+    for top, target in rows:
+        # one row at a time: a sum of all would only show the largest
+        x = np.full((2, classes), target, dt)
+        x[0] = (rng.standard_normal(classes) + top).astype(dt)
+        t = np.array([rng.integers(0, classes), -1])
+        x[0, t[0]] = target
+        _check(x, t, reduction)
+
+
+def test_a_loss_that_only_the_mean_can_hold():
+    """Two rows' losses of 0.65 times the largest float each: their sum is beyond f32, their mean is not."""
+    from rtensors_b200.tensor import cross_entropy_loss
+    for classes in CLASSES:
+        x = np.full((2, classes), -2.0 ** 126, np.float32)
+        x[:, 0] = 2.0 ** 127 * 0.8
+        t = np.array([1, classes - 1])
+        want = 2.0 ** 126 + float(np.float32(2.0 ** 127 * 0.8))
+        # log2 e as a float is off by half a rounding, its product with the difference is the loss
+        assert abs(float(cross_entropy_loss(_t(x), _t(t)).item()) - want) <= 4 * U[np.float32] * want
+        assert cross_entropy_loss(_t(x), _t(t), reduction="sum").item() == np.inf
