@@ -69,6 +69,15 @@ def lib() -> C.CDLL:
         # declared, so that calls pass plain ints: a tiny call costs the host less
         i, n, p = C.c_int, C.c_size_t, C.c_void_p
         view = [p, p, n]
+        layout = [n, p, p, n]      # rank, shape, strides, offset
+        l.rtb_scalar_op.argtypes = [p, i, i, p, p, *layout]
+        l.rtb_unary_op.argtypes = [p, i, i, p, *layout]
+        l.rtb_fill.argtypes = [p, i, p, p, *layout]
+        l.rtb_copy_view.argtypes = [p, i, p, *layout, p]
+        l.rtb_broadcast.argtypes = [p, i, i, *view, *view, *view, n, p]
+        l.rtb_reduce_flat.argtypes = [p, i, i, p, n, n, p]
+        l.rtb_reduce_axis.argtypes = [p, i, i, p, n, n, n, n, p]
+        l.rtb_reduce_view.argtypes = [p, i, i, p, *layout, C.c_ssize_t, p]
         l.rtb_gated_scan.argtypes = [p, i, i, *view, *view, p, p, n, p, n]
         l.rtb_gated_scan_backward.argtypes = [p, i, i, *view, *view, *view, p, p, p, p, p, p, p, n, p, n]
         l.rtb_gated_step.argtypes = [p, i, i, *view, *view, *view, n, p]

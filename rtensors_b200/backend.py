@@ -6,6 +6,7 @@ into librt_b200.so.  Method names and argument meaning follow the trait: `scalar
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from typing import Optional, Sequence, Tuple
 
 import numpy as np
@@ -74,8 +75,8 @@ class _DeviceBlock:
 
 class CudaB200:
     """One instance per device (`Cuda` of the reference, src/backend/cuda.rs:38-186): owns the
-    library context (stream, workspace, allocator).  Calls are enqueued on torch's current
-    stream of that device."""
+    library context (stream, workspace, allocator).  Every call is enqueued on the stream that is torch's current
+    one of that device in the calling thread; calls on different streams keep one total order (rtb_ctx_set_stream)."""
 
     def __init__(self, device: int = 0):
         if not torch.cuda.is_available():
@@ -83,9 +84,9 @@ class CudaB200:
         self.device = self._index = int(device)
         self._torch_device = torch.device("cuda", self.device)
         torch.cuda.set_device(self.device)
-        self._ctx = C.c_void_p()
+        self._lib, self._ctx = lib(), C.c_void_p()
         check(lib().rtb_ctx_create(C.c_int(self.device), C.byref(self._ctx)))
-        self._stream = None
+        self._stream, self._lock = None, threading.RLock()   # the lock: from binding a stream until the call on it is enqueued
         self.mg_world, self.mg_rank, self.mg_peer_mapped = 1, 0, False
         self.sync_stream()
 
@@ -103,13 +104,26 @@ class CudaB200:
 
     # -- plumbing ---------------------------------------------------------------------------
     def sync_stream(self):
-        """Binds the context to torch's current stream (call after switching streams)."""
-        s = torch.cuda.current_stream(self.device).cuda_stream
-        if s != self._stream:
-            check(lib().rtb_ctx_set_stream(self._ctx, C.c_void_p(s)))
-            self._stream = s
+        """Binds the context to torch's current stream.  Every call does so by itself; for code that hands the context to the
+        C ABI directly."""
+        with self._lock:
+            s = _current_stream(self._index)
+            if s != self._stream:
+                check(lib().rtb_ctx_set_stream(self._ctx, C.c_void_p(s)))
+                self._stream = s
+
+    def _call(self, fn, *args):
+        """A call of the C ABI on torch's current stream.  Another thread may have another current stream: it waits until
+        this call is enqueued."""
+        with self._lock:
+            if _current_stream(self._index) != self._stream:
+                self.sync_stream()
+            rc = fn(self._ctx, *args)
+        if rc:
+            check(rc)
 
     def sync(self):
+        self.sync_stream()
         check(lib().rtb_ctx_sync(self._ctx))
 
     @property
@@ -137,7 +151,7 @@ class CudaB200:
     def copy(self, buf: torch.Tensor) -> torch.Tensor:
         out = self.alloc(max(buf.numel(), 1), buf.dtype)
         if buf.numel():
-            check(lib().rtb_d2d(self._ctx, self._p(out), self._p(buf), C.c_size_t(buf.numel() * buf.element_size())))
+            self._call(self._lib.rtb_d2d, self._p(out), self._p(buf), C.c_size_t(buf.numel() * buf.element_size()))
         return out[: buf.numel()]
 
     def copy_from_slice(self, dst: torch.Tensor, src: np.ndarray):
@@ -145,7 +159,7 @@ class CudaB200:
         if dst.numel() != src.size:
             raise L.RtbError(L.ERR_SHAPE, f"Buffer size mismatch in copy_from_slice: dst size {dst.numel()}, src size {src.size}")
         if src.size:
-            check(lib().rtb_h2d(self._ctx, self._p(dst), src.ctypes.data_as(C.c_void_p), C.c_size_t(src.nbytes)))
+            self._call(self._lib.rtb_h2d, self._p(dst), src.ctypes.data_as(C.c_void_p), C.c_size_t(src.nbytes))
             self.sync()  # the host array may go away
 
     def copy_range_within(self, dst: torch.Tensor, src: torch.Tensor, dst_offset: int, src_offset: int, n: int):
@@ -153,23 +167,23 @@ class CudaB200:
             raise L.RtbError(L.ERR_BOUNDS, "Index out of bounds in copy_range_within")
         if n:
             es = dst.element_size()
-            check(lib().rtb_d2d(self._ctx, C.c_void_p(dst.data_ptr() + dst_offset * es),
-                                C.c_void_p(src.data_ptr() + src_offset * es), C.c_size_t(n * es)))
+            self._call(self._lib.rtb_d2d, C.c_void_p(dst.data_ptr() + dst_offset * es),
+                       C.c_void_p(src.data_ptr() + src_offset * es), C.c_size_t(n * es))
 
     def read(self, buf: torch.Tensor, offset: int):
         if not 0 <= offset < buf.numel():
             raise L.RtbError(L.ERR_BOUNDS, f"Index {offset} out of bounds for buffer of length {buf.numel()}")
         host = np.empty(1, dtype=CODE_TO_NP[dtype_code(buf)])
-        check(lib().rtb_d2h(self._ctx, host.ctypes.data_as(C.c_void_p),
-                            C.c_void_p(buf.data_ptr() + offset * buf.element_size()), C.c_size_t(host.nbytes)))
+        self._call(self._lib.rtb_d2h, host.ctypes.data_as(C.c_void_p),
+                   C.c_void_p(buf.data_ptr() + offset * buf.element_size()), C.c_size_t(host.nbytes))
         return host[0]
 
     def write(self, buf: torch.Tensor, offset: int, value):
         if not 0 <= offset < buf.numel():
             raise L.RtbError(L.ERR_BOUNDS, f"Index {offset} out of bounds for buffer of length {buf.numel()}")
         host = np.array([value], dtype=CODE_TO_NP[dtype_code(buf)])
-        check(lib().rtb_h2d(self._ctx, C.c_void_p(buf.data_ptr() + offset * buf.element_size()),
-                            host.ctypes.data_as(C.c_void_p), C.c_size_t(host.nbytes)))
+        self._call(self._lib.rtb_h2d, C.c_void_p(buf.data_ptr() + offset * buf.element_size()),
+                   host.ctypes.data_as(C.c_void_p), C.c_size_t(host.nbytes))
         self.sync()
 
     @staticmethod
@@ -181,9 +195,7 @@ class CudaB200:
         code = dtype_code(buf) if dtype is None else dtype
         v = _scalar_bytes(code, value)
         meta.check_extent(buf.numel())
-        check(lib().rtb_scalar_op(self._ctx, C.c_int(code), C.c_int(op), self._p(buf), v,
-                                  C.c_size_t(meta.rank), meta.c_shape, meta.c_strides,
-                                  C.c_size_t(meta.offset)))
+        self._call(self._lib.rtb_scalar_op, code, op, buf.data_ptr(), v, meta.rank, meta.c_shape, meta.c_strides, meta.offset)
 
     def scalar_apply_add(self, buf, value, meta): self.scalar_apply(buf, L.ADD, value, meta)
     def scalar_apply_sub(self, buf, value, meta): self.scalar_apply(buf, L.SUB, value, meta)
@@ -192,8 +204,7 @@ class CudaB200:
 
     def apply_unary(self, buf: torch.Tensor, op: int, meta: Meta):
         meta.check_extent(buf.numel())
-        check(lib().rtb_unary_op(self._ctx, C.c_int(dtype_code(buf)), C.c_int(op), self._p(buf), C.c_size_t(meta.rank),
-                                 meta.c_shape, meta.c_strides, C.c_size_t(meta.offset)))
+        self._call(self._lib.rtb_unary_op, dtype_code(buf), op, buf.data_ptr(), meta.rank, meta.c_shape, meta.c_strides, meta.offset)
 
     def scalar_apply_log(self, buf, value, meta): self.scalar_apply(buf, L.LOG, value, meta)
     def scalar_apply_log1p(self, buf, value, meta): self.scalar_apply(buf, L.LOG1P, value, meta)
@@ -216,16 +227,15 @@ class CudaB200:
         code = dtype_code(buf)
         v = _scalar_bytes(code, value)
         meta.check_extent(buf.numel())
-        check(lib().rtb_fill(self._ctx, C.c_int(code), self._p(buf), v,
-                             C.c_size_t(meta.rank), meta.c_shape, meta.c_strides, C.c_size_t(meta.offset)))
+        self._call(self._lib.rtb_fill, code, buf.data_ptr(), v, meta.rank, meta.c_shape, meta.c_strides, meta.offset)
 
     def contiguous(self, buf: torch.Tensor, meta: Meta) -> torch.Tensor:
         """Row-major copy of a view (view_to_contiguous, src/core/tensor.rs:299-325)."""
         out = self.alloc(max(meta.size, 1), buf.dtype)
         if meta.size:
             meta.check_extent(buf.numel())
-            check(lib().rtb_copy_view(self._ctx, C.c_int(dtype_code(buf)), self._p(buf), C.c_size_t(meta.rank),
-                                      meta.c_shape, meta.c_strides, C.c_size_t(meta.offset), self._p(out)))
+            self._call(self._lib.rtb_copy_view, dtype_code(buf), buf.data_ptr(), meta.rank,
+                       meta.c_shape, meta.c_strides, meta.offset, out.data_ptr())
         return out
 
     def grad_mask(self, buf: torch.Tensor, meta: Meta, kind: int, value=None) -> torch.Tensor:
@@ -237,8 +247,8 @@ class CudaB200:
             meta.check_extent(buf.numel())
             code = dtype_code(buf)
             v = None if value is None else _scalar_bytes(code, value)
-            check(lib().rtb_grad_mask(self._ctx, C.c_int(code), C.c_int(kind), v, self._p(buf), C.c_size_t(meta.rank),
-                                      meta.c_shape, meta.c_strides, C.c_size_t(meta.offset), self._p(out)))
+            self._call(self._lib.rtb_grad_mask, C.c_int(code), C.c_int(kind), v, self._p(buf), C.c_size_t(meta.rank),
+                       meta.c_shape, meta.c_strides, C.c_size_t(meta.offset), self._p(out))
         return out
 
     # -- broadcast ----------------------------------------------------------------------------
@@ -248,10 +258,8 @@ class CudaB200:
         (lb, lm), (rb, rm), (db, dm) = left, right, dst
         assert lm.shape == rm.shape == dm.shape
         lm.check_extent(lb.numel()); rm.check_extent(rb.numel()); dm.check_extent(db.numel())
-        check(lib().rtb_broadcast(self._ctx, C.c_int(dtype_code(db)), C.c_int(op), self._p(lb), lm.c_strides,
-                                  C.c_size_t(lm.offset), self._p(rb), rm.c_strides, C.c_size_t(rm.offset),
-                                  self._p(db), dm.c_strides, C.c_size_t(dm.offset), C.c_size_t(dm.rank),
-                                  dm.c_shape))
+        self._call(self._lib.rtb_broadcast, dtype_code(db), op, lb.data_ptr(), lm.c_strides, lm.offset, rb.data_ptr(), rm.c_strides,
+                   rm.offset, db.data_ptr(), dm.c_strides, dm.offset, dm.rank, dm.c_shape)
 
     def binary(self, a: torch.Tensor, am: Meta, b: torch.Tensor, bm: Meta, op: int):
         """`a op b` as the operator impls do it (src/ops/broadcast/add.rs:441-477), except that the
@@ -274,8 +282,7 @@ class CudaB200:
     def apply_reduce_contiguous_flat(self, src: torch.Tensor, dst: torch.Tensor, start: int, length: int, op: int):
         if start + length > src.numel():
             raise L.RtbError(-4, "flat reduction range exceeds the buffer")
-        check(lib().rtb_reduce_flat(self._ctx, C.c_int(dtype_code(src)), C.c_int(op), self._p(src), C.c_size_t(start),
-                                    C.c_size_t(length), self._p(dst)))
+        self._call(self._lib.rtb_reduce_flat, dtype_code(src), op, src.data_ptr(), start, length, dst.data_ptr())
 
     def apply_reduce(self, src: Tuple[torch.Tensor, Meta], dst: torch.Tensor, dim: int, op: int):
         """Backend::apply_reduce (src/backend/mod.rs:375-409): contiguous input; rank 1 -> flat."""
@@ -289,9 +296,7 @@ class CudaB200:
         r = sm.shape[dim]
         if sm.offset + outer * r * inner > sb.numel():
             raise L.RtbError(-4, "axis reduction range exceeds the buffer")
-        check(lib().rtb_reduce_axis(self._ctx, C.c_int(dtype_code(sb)), C.c_int(op), self._p(sb),
-                                    C.c_size_t(sm.offset), C.c_size_t(outer), C.c_size_t(r), C.c_size_t(inner),
-                                    self._p(dst)))
+        self._call(self._lib.rtb_reduce_axis, dtype_code(sb), op, sb.data_ptr(), sm.offset, outer, r, inner, dst.data_ptr())
 
     def reduce_view(self, src: torch.Tensor, meta: Meta, axis: Optional[int], op: int,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -308,9 +313,9 @@ class CudaB200:
             out = self.alloc(max(n_out, 1), src.dtype)
         elif out.numel() < n_out or out.dtype != src.dtype:
             raise ValueError("reduce_view: the output buffer is too small or of another dtype")
-        check(lib().rtb_reduce_view(self._ctx, C.c_int(dtype_code(src)), C.c_int(op), self._p(src), C.c_size_t(meta.rank),
-                                    meta.c_shape, meta.c_strides, C.c_size_t(meta.offset),
-                                    C.c_ssize_t(-1 if axis is None else axis), self._p(out)))
+        self._call(self._lib.rtb_reduce_view, dtype_code(src), op, src.data_ptr(), meta.rank,
+                   meta.c_shape, meta.c_strides, meta.offset,
+                   -1 if axis is None else axis, out.data_ptr())
         return out
 
     def reduce_view_ex(self, src: torch.Tensor, meta: Meta, axis: Optional[int], op: int, unbiased: bool = True,
@@ -324,9 +329,9 @@ class CudaB200:
                 n_out *= 1 if k == axis else s_
         out = self.alloc(max(n_out, 1), torch.int64 if op in (L.ARGMAX, L.ARGMIN) else src.dtype)
         st = L.ReduceSettings(bool(unbiased), bool(is_std), int(norm_type))
-        check(lib().rtb_reduce_view_ex(self._ctx, C.c_int(dtype_code(src)), C.c_int(op), C.byref(st), self._p(src),
-                                       C.c_size_t(meta.rank), meta.c_shape, meta.c_strides, C.c_size_t(meta.offset),
-                                       C.c_ssize_t(-1 if axis is None else axis), self._p(out)))
+        self._call(self._lib.rtb_reduce_view_ex, C.c_int(dtype_code(src)), C.c_int(op), C.byref(st), self._p(src),
+                   C.c_size_t(meta.rank), meta.c_shape, meta.c_strides, C.c_size_t(meta.offset),
+                   C.c_ssize_t(-1 if axis is None else axis), self._p(out))
         return out
 
     def apply_reduce_ex(self, src: Tuple[torch.Tensor, Meta], dst: torch.Tensor, dim: int, op: int, unbiased: bool = True,
@@ -340,16 +345,16 @@ class CudaB200:
         if sm.rank == 1:
             if sm.offset + sm.size > sb.numel():
                 raise L.RtbError(-4, "flat reduction range exceeds the buffer")
-            return check(lib().rtb_reduce_flat_ex(self._ctx, C.c_int(dtype_code(sb)), C.c_int(op), C.byref(st), self._p(sb),
-                                                  C.c_size_t(sm.offset), C.c_size_t(sm.size), self._p(dst)))
+            return self._call(self._lib.rtb_reduce_flat_ex, C.c_int(dtype_code(sb)), C.c_int(op), C.byref(st), self._p(sb),
+                              C.c_size_t(sm.offset), C.c_size_t(sm.size), self._p(dst))
         outer = int(np.prod(sm.shape[:dim], dtype=np.int64)) if dim > 0 else 1
         inner = max(int(np.prod(sm.shape[dim + 1:], dtype=np.int64)), 1)
         r = sm.shape[dim]
         if sm.offset + outer * r * inner > sb.numel():
             raise L.RtbError(-4, "axis reduction range exceeds the buffer")
-        check(lib().rtb_reduce_axis_ex(self._ctx, C.c_int(dtype_code(sb)), C.c_int(op), C.byref(st), self._p(sb),
-                                       C.c_size_t(sm.offset), C.c_size_t(outer), C.c_size_t(r), C.c_size_t(inner),
-                                       self._p(dst)))
+        self._call(self._lib.rtb_reduce_axis_ex, C.c_int(dtype_code(sb)), C.c_int(op), C.byref(st), self._p(sb),
+                   C.c_size_t(sm.offset), C.c_size_t(outer), C.c_size_t(r), C.c_size_t(inner),
+                   self._p(dst))
 
     def broadcast_reduce(self, a: torch.Tensor, am: Meta, b: torch.Tensor, bm: Meta, binop: int, axis: int, redop: int):
         """`(a binop b).<redop>_at(axis)` in one kernel: the broadcast result is never written.
@@ -358,15 +363,14 @@ class CudaB200:
         Meta(shape, sa, am.offset).check_extent(a.numel()); Meta(shape, sb, bm.offset).check_extent(b.numel())
         om = Meta.contiguous(tuple(1 if k == axis else s_ for k, s_ in enumerate(shape)))
         out = self.alloc(max(om.size, 1), a.dtype)
-        check(lib().rtb_broadcast_reduce(self._ctx, C.c_int(dtype_code(a)), C.c_int(binop), C.c_int(redop), self._p(a),
-                                         diffs(sa), C.c_size_t(am.offset), self._p(b), diffs(sb), C.c_size_t(bm.offset),
-                                         C.c_size_t(len(shape)), sizes(shape), C.c_size_t(axis), self._p(out)))
+        self._call(self._lib.rtb_broadcast_reduce, C.c_int(dtype_code(a)), C.c_int(binop), C.c_int(redop), self._p(a),
+                   diffs(sa), C.c_size_t(am.offset), self._p(b), diffs(sb), C.c_size_t(bm.offset),
+                   C.c_size_t(len(shape)), sizes(shape), C.c_size_t(axis), self._p(out))
         return out, om
 
     def reduce_axis_ori(self, src: torch.Tensor, offset: int, outer: int, r: int, inner: int, op: int):
         out = self.alloc(max(outer * inner, 1), src.dtype)
-        check(lib().rtb_reduce_axis(self._ctx, C.c_int(dtype_code(src)), C.c_int(op), self._p(src), C.c_size_t(offset),
-                                    C.c_size_t(outer), C.c_size_t(r), C.c_size_t(inner), self._p(out)))
+        self._call(self._lib.rtb_reduce_axis, dtype_code(src), op, src.data_ptr(), offset, outer, r, inner, out.data_ptr())
         return out
 
     def reduce_ext_ori(self, src: torch.Tensor, offset: int, outer: int, r: int, inner: int, op: int, unbiased: bool = True,
@@ -374,16 +378,16 @@ class CudaB200:
         """Codes 6..10 over a contiguous (outer, r, inner) block (rtb_reduce_axis_ex); int64 output for positions."""
         out = self.alloc(max(outer * inner, 1), torch.int64 if op in (L.ARGMAX, L.ARGMIN) else src.dtype)
         st = L.ReduceSettings(bool(unbiased), bool(is_std), int(norm_type))
-        check(lib().rtb_reduce_axis_ex(self._ctx, C.c_int(dtype_code(src)), C.c_int(op), C.byref(st), self._p(src),
-                                       C.c_size_t(offset), C.c_size_t(outer), C.c_size_t(r), C.c_size_t(inner), self._p(out)))
+        self._call(self._lib.rtb_reduce_axis_ex, C.c_int(dtype_code(src)), C.c_int(op), C.byref(st), self._p(src),
+                   C.c_size_t(offset), C.c_size_t(outer), C.c_size_t(r), C.c_size_t(inner), self._p(out))
         return out
 
     def l1_loss(self, a: torch.Tensor, b: torch.Tensor, reduction: int = 0, with_grad: bool = False):
         assert a.numel() == b.numel() and a.dtype == b.dtype
         loss = self.alloc(1, a.dtype)
         g = self.alloc(a.numel(), a.dtype) if with_grad else None
-        check(lib().rtb_l1_loss(self._ctx, C.c_int(dtype_code(a)), self._p(a), self._p(b), C.c_size_t(a.numel()),
-                                C.c_int(reduction), self._p(loss), self._p(g)))
+        self._call(self._lib.rtb_l1_loss, C.c_int(dtype_code(a)), self._p(a), self._p(b), C.c_size_t(a.numel()),
+                   C.c_int(reduction), self._p(loss), self._p(g))
         return loss, g
 
     def reduce_to_shape(self, upstream: torch.Tensor, shape: Sequence[int], operand_strides: Sequence[int],
@@ -396,15 +400,14 @@ class CudaB200:
         elif out.numel() < n_out or out.dtype != upstream.dtype:
             raise ValueError("reduce_to_shape: the output buffer is too small or of another dtype")
         osh = (C.c_size_t * max(r, 1))()
-        check(lib().rtb_reduce_to_shape(self._ctx, C.c_int(dtype_code(upstream)), self._p(upstream), C.c_size_t(r),
-                                        sizes(shape), diffs(operand_strides), self._p(out), osh))
+        self._call(self._lib.rtb_reduce_to_shape, C.c_int(dtype_code(upstream)), self._p(upstream), C.c_size_t(r),
+                   sizes(shape), diffs(operand_strides), self._p(out), osh)
         assert tuple(osh[:r]) == oshape
         return out, oshape
 
     # -- gated linear recurrence, 8-bit checkpoints, cross-entropy ---------------------------------
     def _same(self, first: torch.Tensor, *rest: Optional[torch.Tensor]):
-        """One dtype, and every buffer on this backend's device (a foreign address would fault inside a kernel).  Binds the
-        context to torch's current stream if that has changed."""
+        """One dtype, and every buffer on this backend's device (a foreign address would fault inside a kernel)."""
         dt, index = first.dtype, self._index
         if first.get_device() != index:
             raise L.RtbError(L.ERR_INVALID, f"a buffer on {first.device} was given to the backend of cuda:{index}")
@@ -415,8 +418,6 @@ class CudaB200:
                 raise L.RtbError(L.ERR_DTYPE, f"operands of {dt} and {t.dtype}")
             if t.get_device() != index:
                 raise L.RtbError(L.ERR_INVALID, f"a buffer on {t.device} was given to the backend of cuda:{index}")
-        if _current_stream(index) != self._stream:
-            self.sync_stream()
 
     @staticmethod
     def _views(shape, *views: Tuple[torch.Tensor, Meta]):
@@ -437,7 +438,7 @@ class CudaB200:
         dense over the shape with `axis` as 1.  -> the states, dense row-major."""
         i, rank = self._index, len(xm.shape)
         _axis(axis, rank)
-        if gate.dtype is not x.dtype or h0 is not None or x.get_device() != i or gate.get_device() != i or _current_stream(i) != self._stream:
+        if gate.dtype is not x.dtype or h0 is not None or x.get_device() != i or gate.get_device() != i:
             self._same(x, gate, h0)
             if h0 is not None:
                 self._first_states(h0, xm, axis)
@@ -446,9 +447,9 @@ class CudaB200:
         xm.check_extent(x.numel()); gm.check_extent(gate.numel())
         out = x.new_empty(max(xm.size, 1))
         flags = (L.SCAN_REVERSE if reverse else 0) | (L.SCAN_COUPLED if coupled else 0)
-        check(lib().rtb_gated_scan(self._ctx, dtype_code(x), flags, gate.data_ptr(), gm.c_strides, gm.offset,
-                                   x.data_ptr(), xm.c_strides, xm.offset, None if h0 is None else h0.data_ptr(), out.data_ptr(),
-                                   rank, xm.c_shape, axis))
+        self._call(self._lib.rtb_gated_scan, dtype_code(x), flags, gate.data_ptr(), gm.c_strides, gm.offset,
+                   x.data_ptr(), xm.c_strides, xm.offset, None if h0 is None else h0.data_ptr(), out.data_ptr(),
+                   rank, xm.c_shape, axis)
         return out
 
     def gated_scan_backward(self, up: torch.Tensor, um: Meta, gate: torch.Tensor, gm: Meta, axis: int,
@@ -488,25 +489,23 @@ class CudaB200:
         if want_h0:
             dh0 = up.new_empty(max(_lanes(um, axis), 1))
         x_args = (x.data_ptr(), xm.c_strides, xm.offset) if x is not None and coupled and want_g else (None, None, 0)
-        check(lib().rtb_gated_scan_backward(
-            self._ctx, dtype_code(up), (L.SCAN_REVERSE if reverse else 0) | (L.SCAN_COUPLED if coupled else 0), up.data_ptr(), um.c_strides, um.offset, gate.data_ptr(),
-            gm.c_strides, gm.offset, *x_args, h.data_ptr() if h is not None and want_g else None,
-            codes, mags,
-            None if h0 is None else h0.data_ptr(), None if dx is None else dx.data_ptr(), None if dg is None else dg.data_ptr(),
-            None if dh0 is None else dh0.data_ptr(), um.rank, um.c_shape, axis))
+        flags = (L.SCAN_REVERSE if reverse else 0) | (L.SCAN_COUPLED if coupled else 0)
+        self._call(self._lib.rtb_gated_scan_backward, dtype_code(up), flags, up.data_ptr(), um.c_strides, um.offset, gate.data_ptr(), gm.c_strides,
+                   gm.offset, *x_args, h.data_ptr() if h is not None and want_g else None, codes, mags,
+                   None if h0 is None else h0.data_ptr(), None if dx is None else dx.data_ptr(), None if dg is None else dg.data_ptr(),
+                   None if dh0 is None else dh0.data_ptr(), um.rank, um.c_shape, axis)
         return dx, dg, dh0
 
     def gated_step(self, state: torch.Tensor, sm: Meta, gate: torch.Tensor, gm: Meta, x: torch.Tensor, xm: Meta, coupled: bool = False):
         """One step of the recurrence in place: state = gate state + x over views of one shape (rtb_gated_step)."""
         i, dt = self._index, state.dtype
-        if gate.dtype is not dt or x.dtype is not dt or state.get_device() != i or gate.get_device() != i or x.get_device() != i or \
-                _current_stream(i) != self._stream:
+        if gate.dtype is not dt or x.dtype is not dt or state.get_device() != i or gate.get_device() != i or x.get_device() != i:
             self._same(state, gate, x)
         if gm.shape != sm.shape or xm.shape != sm.shape:
             self._views(sm.shape, (gate, gm), (x, xm))
         sm.check_extent(state.numel()); gm.check_extent(gate.numel()); xm.check_extent(x.numel())
-        check(lib().rtb_gated_step(self._ctx, dtype_code(state), L.SCAN_COUPLED if coupled else 0, state.data_ptr(), sm.c_strides, sm.offset,
-                                   gate.data_ptr(), gm.c_strides, gm.offset, x.data_ptr(), xm.c_strides, xm.offset, sm.rank, sm.c_shape))
+        self._call(self._lib.rtb_gated_step, dtype_code(state), L.SCAN_COUPLED if coupled else 0, state.data_ptr(), sm.c_strides, sm.offset,
+                   gate.data_ptr(), gm.c_strides, gm.offset, x.data_ptr(), xm.c_strides, xm.offset, sm.rank, sm.c_shape)
 
     def ckpt8_store(self, src: torch.Tensor, n: Optional[int] = None, offset: int = 0) -> torch.Tensor:
         """8-bit checkpoint of n consecutive elements of a buffer (rtb_ckpt8_store) -> an int8 buffer laid out as ckpt8_layout says."""
@@ -518,7 +517,7 @@ class CudaB200:
         at, total = ckpt8_layout(n, es)
         out = torch.empty(total or 1, dtype=torch.int8, device=self._torch_device)
         p = out.data_ptr()
-        check(lib().rtb_ckpt8_store(self._ctx, dtype_code(src), src.data_ptr() + offset * es, n, p, p + at))
+        self._call(self._lib.rtb_ckpt8_store, dtype_code(src), src.data_ptr() + offset * es, n, p, p + at)
         return out
 
     def _check_ckpt(self, ckpt: torch.Tensor, n: int, like: torch.Tensor) -> int:
@@ -532,7 +531,7 @@ class CudaB200:
         out = torch.empty(n or 1, dtype=dtype, device=self._torch_device)
         self._same(out)
         p = ckpt.data_ptr()
-        check(lib().rtb_ckpt8_restore(self._ctx, dtype_code(out), p, p + self._check_ckpt(ckpt, n, out), n, out.data_ptr()))
+        self._call(self._lib.rtb_ckpt8_restore, dtype_code(out), p, p + self._check_ckpt(ckpt, n, out), n, out.data_ptr())
         return out
 
     def ckpt8_grad(self, kind: int, ckpt: torch.Tensor, up: torch.Tensor, n: int, offset: int = 0) -> torch.Tensor:
@@ -542,8 +541,8 @@ class CudaB200:
             raise L.RtbError(L.ERR_BOUNDS, f"range [{offset}, {offset + n}) exceeds a buffer of {up.numel()}")
         out = up.new_empty(n or 1)
         p = ckpt.data_ptr()
-        check(lib().rtb_ckpt8_grad(self._ctx, dtype_code(up), kind, p, p + self._check_ckpt(ckpt, n, up),
-                                   up.data_ptr() + offset * up.element_size(), n, out.data_ptr()))
+        self._call(self._lib.rtb_ckpt8_grad, dtype_code(up), kind, p, p + self._check_ckpt(ckpt, n, up),
+                   up.data_ptr() + offset * up.element_size(), n, out.data_ptr())
         return out
 
     def cross_entropy(self, logits: torch.Tensor, rows: int, classes: int, targets: torch.Tensor, reduction: int = 0, with_grad: bool = False,
@@ -561,29 +560,29 @@ class CudaB200:
             raise L.RtbError(L.ERR_INVALID, f"targets on {targets.device} were given to the backend of cuda:{self._index}")
         loss = logits.new_empty(1)
         g = logits.new_empty(max(rows * classes, 1)) if with_grad else None
-        check(lib().rtb_cross_entropy(self._ctx, dtype_code(logits), logits.data_ptr() + offset * logits.element_size(), rows, classes, pitch,
-                                      targets.data_ptr(), reduction, loss.data_ptr(), None if g is None else g.data_ptr()))
+        self._call(self._lib.rtb_cross_entropy, dtype_code(logits), logits.data_ptr() + offset * logits.element_size(), rows, classes, pitch,
+                   targets.data_ptr(), reduction, loss.data_ptr(), None if g is None else g.data_ptr())
         return loss, g
 
     # -- fused MLP pieces ---------------------------------------------------------------------
     def relu_mask(self, x: torch.Tensor) -> torch.Tensor:
         mask = torch.empty_like(x)
         fn = lib().rtb_relu_mask_f64 if x.dtype == torch.float64 else lib().rtb_relu_mask_f32
-        check(fn(self._ctx, self._p(x), self._p(mask), C.c_size_t(x.numel())))
+        self._call(fn, self._p(x), self._p(mask), C.c_size_t(x.numel()))
         return mask
 
     def bias_relu_mask(self, z: torch.Tensor, bias: torch.Tensor, rows: int, cols: int) -> torch.Tensor:
         """z = relu(z + bias) in place over a dense (rows, cols) activation; returns the gradient mask."""
         mask = torch.empty_like(z)
-        check(lib().rtb_bias_relu_mask(self._ctx, C.c_int(dtype_code(z)), self._p(z), self._p(bias), self._p(mask),
-                                       C.c_size_t(rows), C.c_size_t(cols)))
+        self._call(self._lib.rtb_bias_relu_mask, C.c_int(dtype_code(z)), self._p(z), self._p(bias), self._p(mask),
+                   C.c_size_t(rows), C.c_size_t(cols))
         return mask
 
     def sgd_update(self, p: torch.Tensor, g: torch.Tensor, lr: float):
         if p.dtype == torch.float64:
-            check(lib().rtb_sgd_update_f64(self._ctx, self._p(p), self._p(g), C.c_double(lr), C.c_size_t(p.numel())))
+            self._call(self._lib.rtb_sgd_update_f64, self._p(p), self._p(g), C.c_double(lr), C.c_size_t(p.numel()))
         else:
-            check(lib().rtb_sgd_update_f32(self._ctx, self._p(p), self._p(g), C.c_float(lr), C.c_size_t(p.numel())))
+            self._call(self._lib.rtb_sgd_update_f32, self._p(p), self._p(g), C.c_float(lr), C.c_size_t(p.numel()))
 
     def convert(self, src: torch.Tensor, dst_dtype: torch.dtype, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """`convert::<T, N>` (src/backend/mod.rs:234) into `out`, or into a fresh buffer: every element
@@ -592,21 +591,21 @@ class CudaB200:
             out = self.alloc(max(src.numel(), 1), dst_dtype)
         elif out.dtype != dst_dtype or out.numel() < src.numel():
             raise ValueError("Buffer size mismatch in convert")
-        check(lib().rtb_convert(self._ctx, C.c_int(dtype_code(src)), C.c_int(TORCH_TO_CODE[dst_dtype]), self._p(src),
-                                self._p(out), C.c_size_t(src.numel())))
+        self._call(self._lib.rtb_convert, C.c_int(dtype_code(src)), C.c_int(TORCH_TO_CODE[dst_dtype]), self._p(src),
+                   self._p(out), C.c_size_t(src.numel()))
         return out
 
     def convert_raw(self, src: torch.Tensor, src_code: int, dst_code: int) -> torch.Tensor:
         """convert over raw byte buffers (torch.uint8), for the 128-bit integer types torch lacks."""
         n = src.numel() // L.DTYPE_SIZE[src_code]
         out = self.alloc(max(n, 1) * L.DTYPE_SIZE[dst_code], torch.uint8)
-        check(lib().rtb_convert(self._ctx, C.c_int(src_code), C.c_int(dst_code), self._p(src), self._p(out), C.c_size_t(n)))
+        self._call(self._lib.rtb_convert, C.c_int(src_code), C.c_int(dst_code), self._p(src), self._p(out), C.c_size_t(n))
         return out
 
     def u8_to_f32_div(self, src: torch.Tensor, divisor: float = 255.0) -> torch.Tensor:
         out = self.alloc(src.numel(), torch.float32)
-        check(lib().rtb_u8_to_f32_div(self._ctx, self._p(src), self._p(out), C.c_float(divisor),
-                                      C.c_size_t(src.numel())))
+        self._call(self._lib.rtb_u8_to_f32_div, self._p(src), self._p(out), C.c_float(divisor),
+                   C.c_size_t(src.numel()))
         return out
 
     # -- multi-GPU (rtb_mg_*): one rank per GPU, the communicator lives in the library context -----
@@ -618,13 +617,13 @@ class CudaB200:
 
     def mg_init(self, nranks: int, rank: int, unique_id: bytes):
         """Collective: every rank passes the id made by rank 0's mg_unique_id()."""
-        check(lib().rtb_mg_init(self._ctx, C.c_int(nranks), C.c_int(rank), C.c_char_p(unique_id)))
+        self._call(self._lib.rtb_mg_init, C.c_int(nranks), C.c_int(rank), C.c_char_p(unique_id))
         n, r, m = C.c_int(), C.c_int(), C.c_int()
         check(lib().rtb_mg_info(self._ctx, C.byref(n), C.byref(r), C.byref(m)))
         self.mg_world, self.mg_rank, self.mg_peer_mapped = n.value, r.value, bool(m.value)
 
     def mg_finalize(self):
-        check(lib().rtb_mg_finalize(self._ctx))
+        self._call(self._lib.rtb_mg_finalize)
         self.mg_world, self.mg_rank, self.mg_peer_mapped = 1, 0, False
 
     def mg_set_wait_ns(self, ns: int):
@@ -632,19 +631,19 @@ class CudaB200:
 
     def mg_status(self) -> int:
         bits = C.c_uint()
-        check(lib().rtb_mg_status(self._ctx, C.byref(bits)))
+        self._call(self._lib.rtb_mg_status, C.byref(bits))
         return bits.value
 
     def mg_realign(self):
-        check(lib().rtb_mg_realign(self._ctx))
+        self._call(self._lib.rtb_mg_realign)
 
     def mg_allreduce(self, buf: torch.Tensor, op: int = L.SUM, mean_count: int = 0, overlap: bool = False):
         fn = lib().rtb_mg_allreduce_begin if overlap else lib().rtb_mg_allreduce
-        check(fn(self._ctx, C.c_int(dtype_code(buf)), C.c_int(op), self._p(buf), C.c_size_t(buf.numel()),
-                 C.c_size_t(mean_count)))
+        self._call(fn, C.c_int(dtype_code(buf)), C.c_int(op), self._p(buf), C.c_size_t(buf.numel()),
+                   C.c_size_t(mean_count))
 
     def mg_allreduce_join(self):
-        check(lib().rtb_mg_allreduce_join(self._ctx))
+        self._call(self._lib.rtb_mg_allreduce_join)
 
     # -- host-buffer operations (rtb_host_*): two transfer lanes and a pool of device blocks inside the library --
     def _pool_tensor(self, ptr: int, n: int, dtype: torch.dtype) -> torch.Tensor:
@@ -654,31 +653,32 @@ class CudaB200:
     def host_stage_in(self, host: torch.Tensor) -> torch.Tensor:
         """Starts the upload of a (pinned) host tensor; the compute stream waits only at host_ready."""
         out = C.c_void_p()
-        check(lib().rtb_host_stage_in(self._ctx, C.c_void_p(host.data_ptr()), C.c_size_t(host.numel() * host.element_size()),
-                                      C.byref(out)))
+        self._call(self._lib.rtb_host_stage_in, C.c_void_p(host.data_ptr()), C.c_size_t(host.numel() * host.element_size()),
+                   C.byref(out))
         return self._pool_tensor(out.value, max(host.numel(), 1), host.dtype)
 
     def host_scratch(self, n: int, dtype: torch.dtype) -> torch.Tensor:
         out = C.c_void_p()
-        check(lib().rtb_host_scratch(self._ctx, C.c_size_t(int(n) * torch.empty(0, dtype=dtype).element_size()), C.byref(out)))
+        self._call(self._lib.rtb_host_scratch, C.c_size_t(int(n) * torch.empty(0, dtype=dtype).element_size()), C.byref(out))
         return self._pool_tensor(out.value, max(int(n), 1), dtype)
 
     def host_ready(self, dev: torch.Tensor):
-        check(lib().rtb_host_ready(self._ctx, self._p(dev)))
+        self._call(self._lib.rtb_host_ready, self._p(dev))
 
     def host_stage_out(self, dev: torch.Tensor, host: torch.Tensor):
         if host.numel() * host.element_size() > dev.numel() * dev.element_size():
             raise L.RtbError(-4, "host_stage_out: the host tensor is larger than the device block")
-        check(lib().rtb_host_stage_out(self._ctx, self._p(dev), C.c_void_p(host.data_ptr()),
-                                       C.c_size_t(host.numel() * host.element_size())))
+        self._call(self._lib.rtb_host_stage_out, self._p(dev), C.c_void_p(host.data_ptr()),
+                   C.c_size_t(host.numel() * host.element_size()))
 
     def host_release(self, dev: torch.Tensor):
-        check(lib().rtb_host_release(self._ctx, self._p(dev)))
+        self._call(self._lib.rtb_host_release, self._p(dev))
 
     def host_join(self):
-        check(lib().rtb_host_join(self._ctx))
+        self._call(self._lib.rtb_host_join)
 
     def host_wait(self):
+        self.sync_stream()
         check(lib().rtb_host_wait(self._ctx))
 
     def host_trim(self):
@@ -691,10 +691,10 @@ class CudaB200:
                          unbiased: bool = True, is_std: bool = False, norm_type: int = 2):
         """Reduction of a tensor whose buffer is in host memory; the result goes to host_out (enqueues only)."""
         st = L.ReduceSettings(bool(unbiased), bool(is_std), int(norm_type))
-        check(lib().rtb_host_reduce_view(self._ctx, C.c_int(dtype_code(host)), C.c_int(op), C.byref(st), C.c_void_p(host.data_ptr()),
-                                         C.c_size_t(host.numel()), C.c_size_t(meta.rank), meta.c_shape, meta.c_strides,
-                                         C.c_size_t(meta.offset), C.c_ssize_t(-1 if axis is None else axis),
-                                         C.c_void_p(host_out.data_ptr())))
+        self._call(self._lib.rtb_host_reduce_view, C.c_int(dtype_code(host)), C.c_int(op), C.byref(st), C.c_void_p(host.data_ptr()),
+                   C.c_size_t(host.numel()), C.c_size_t(meta.rank), meta.c_shape, meta.c_strides,
+                   C.c_size_t(meta.offset), C.c_ssize_t(-1 if axis is None else axis),
+                   C.c_void_p(host_out.data_ptr()))
 
     def host_broadcast(self, a_host: torch.Tensor, am: Meta, b_host: torch.Tensor, bm: Meta, op: int, out_host: torch.Tensor,
                        dim_range: Optional[Tuple[int, int]] = None):
@@ -707,22 +707,22 @@ class CudaB200:
             per *= n
         if out_host.numel() < (hi - lo) * per or out_host.dtype != a_host.dtype:
             raise ValueError("host_broadcast: the output tensor is too small or of another dtype")
-        check(lib().rtb_host_broadcast(self._ctx, C.c_int(dtype_code(a_host)), C.c_int(op), C.c_void_p(a_host.data_ptr()),
-                                       C.c_size_t(a_host.numel()), diffs(sa), C.c_size_t(am.offset), C.c_void_p(b_host.data_ptr()),
-                                       C.c_size_t(b_host.numel()), diffs(sb), C.c_size_t(bm.offset), C.c_void_p(out_host.data_ptr()),
-                                       C.c_size_t(len(shape)), sizes(shape), C.c_size_t(lo), C.c_size_t(hi)))
+        self._call(self._lib.rtb_host_broadcast, C.c_int(dtype_code(a_host)), C.c_int(op), C.c_void_p(a_host.data_ptr()),
+                   C.c_size_t(a_host.numel()), diffs(sa), C.c_size_t(am.offset), C.c_void_p(b_host.data_ptr()),
+                   C.c_size_t(b_host.numel()), diffs(sb), C.c_size_t(bm.offset), C.c_void_p(out_host.data_ptr()),
+                   C.c_size_t(len(shape)), sizes(shape), C.c_size_t(lo), C.c_size_t(hi))
 
     def mg_combine(self, buf: torch.Tensor, op: int = L.SUM, mean_count: int = 0):
-        check(lib().rtb_mg_combine(self._ctx, C.c_int(dtype_code(buf)), C.c_int(op), self._p(buf), C.c_size_t(buf.numel()),
-                                   C.c_size_t(mean_count)))
+        self._call(self._lib.rtb_mg_combine, C.c_int(dtype_code(buf)), C.c_int(op), self._p(buf), C.c_size_t(buf.numel()),
+                   C.c_size_t(mean_count))
 
     def mg_reduce_flat(self, src: torch.Tensor, start: int, local_len: int, global_len: int, op: int,
                        dst: Optional[torch.Tensor] = None) -> torch.Tensor:
         if start + local_len > src.numel():
             raise L.RtbError(-4, "flat reduction range exceeds the buffer")
         dst = self.alloc(1, src.dtype) if dst is None else dst
-        check(lib().rtb_mg_reduce_flat(self._ctx, C.c_int(dtype_code(src)), C.c_int(op), self._p(src), C.c_size_t(start),
-                                       C.c_size_t(local_len), C.c_size_t(global_len), self._p(dst)))
+        self._call(self._lib.rtb_mg_reduce_flat, C.c_int(dtype_code(src)), C.c_int(op), self._p(src), C.c_size_t(start),
+                   C.c_size_t(local_len), C.c_size_t(global_len), self._p(dst))
         return dst
 
     def mg_reduce_axis(self, src: torch.Tensor, offset: int, outer: int, r_local: int, inner: int, global_r: int, op: int,
@@ -731,15 +731,15 @@ class CudaB200:
         dst = self.alloc(max(outer * inner, 1), src.dtype) if dst is None else dst
         so = r_local * inner if outer_stride is None else outer_stride
         sr = inner if row_stride is None else row_stride
-        check(lib().rtb_mg_reduce_axis(self._ctx, C.c_int(dtype_code(src)), C.c_int(op), self._p(src), C.c_size_t(offset),
-                                       C.c_size_t(outer), C.c_size_t(r_local), C.c_size_t(inner), C.c_ssize_t(so),
-                                       C.c_ssize_t(sr), C.c_size_t(global_r), self._p(dst)))
+        self._call(self._lib.rtb_mg_reduce_axis, C.c_int(dtype_code(src)), C.c_int(op), self._p(src), C.c_size_t(offset),
+                   C.c_size_t(outer), C.c_size_t(r_local), C.c_size_t(inner), C.c_ssize_t(so),
+                   C.c_ssize_t(sr), C.c_size_t(global_r), self._p(dst))
         return dst
 
     def mg_l1_loss(self, a: torch.Tensor, b: torch.Tensor, global_n: int, reduction: int = 0, with_grad: bool = False):
         assert a.numel() == b.numel() and a.dtype == b.dtype
         loss = self.alloc(1, a.dtype)
         g = self.alloc(a.numel(), a.dtype) if with_grad else None
-        check(lib().rtb_mg_l1_loss(self._ctx, C.c_int(dtype_code(a)), self._p(a), self._p(b), C.c_size_t(a.numel()),
-                                   C.c_size_t(global_n), C.c_int(reduction), self._p(loss), self._p(g)))
+        self._call(self._lib.rtb_mg_l1_loss, C.c_int(dtype_code(a)), self._p(a), self._p(b), C.c_size_t(a.numel()),
+                   C.c_size_t(global_n), C.c_int(reduction), self._p(loss), self._p(g))
         return loss, g

@@ -134,12 +134,19 @@ RTB_API int rtb_ctx_set_stream(rtb_ctx *c, void *stream) {
     int rc = rtb::use_device(ctx);
     if (rc) return rc;
     if (!ctx->order_event) RTB_CUDA(cudaEventCreateWithFlags(&ctx->order_event, cudaEventDisableTiming));
-    if (!rtb::capturing(ctx) && !rtb::stream_capturing(next)) {
-        // (a stream that is being captured cannot be joined with work outside its graph: whoever set
-        // up the capture has ordered the capturing stream after the earlier work)
-        RTB_CUDA(cudaEventRecord(ctx->order_event, ctx->stream));
+    auto join = [&](cudaStream_t from) -> int {
+        RTB_CUDA(cudaEventRecord(ctx->order_event, from));
         RTB_CUDA(cudaStreamWaitEvent(next, ctx->order_event, 0));
-    }
+        return RTB_OK;
+    };
+    // (a stream that is being captured cannot be joined with work outside its graph: whoever set
+    // up the capture has ordered the capturing stream after the earlier work.  The next stream that is not
+    // being captured is made to wait for the one that was left for the capture.)
+    const bool from_capture = rtb::capturing(ctx), to_capture = rtb::stream_capturing(next);
+    if (!from_capture && to_capture && !ctx->left_open) ctx->left = ctx->stream, ctx->left_open = true;
+    if (!from_capture && !to_capture && (rc = join(ctx->stream))) return rc;
+    if (ctx->left_open && !to_capture && ctx->left != next && !rtb::stream_capturing(ctx->left) && (rc = join(ctx->left))) return rc;
+    if (!to_capture) ctx->left_open = false;
     ctx->stream = next;
     return RTB_OK;
 }

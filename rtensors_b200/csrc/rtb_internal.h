@@ -62,6 +62,8 @@ struct Ctx {
     std::vector<void *> retired;              // superseded workspaces, freed only with the context
     std::atomic<uint64_t> ws_generation{0};   // bumped whenever device memory a captured graph may hold goes away
     cudaEvent_t order_event = nullptr;        // joins the old stream into the new one in rtb_ctx_set_stream
+    cudaStream_t left = nullptr;              // the stream that was left, unjoined, for one that was being captured
+    bool left_open = false;
     Mg *mg = nullptr;                         // set by rtb_mg_init
     HostLanes *host = nullptr;                // created by the first host-buffer operation
     // caching allocator: free blocks by rounded size; live blocks by pointer

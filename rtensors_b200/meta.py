@@ -94,12 +94,13 @@ class Meta:
 
     def check_extent(self, buf_len: int) -> None:
         # a view that fits a buffer of n elements fits every longer one: remember the shortest seen
-        ok = self.__dict__.get("_fits")
-        if ok is not None and buf_len >= ok:
+        if buf_len >= self._fits:
             return
         check(lib().rtb_meta_check_extent(C.c_size_t(self.rank), self.c_shape, self.c_strides,
                                           C.c_size_t(self.offset), C.c_size_t(buf_len)))
-        self.__dict__["_fits"] = buf_len if ok is None else min(ok, buf_len)
+        self.__dict__["_fits"] = buf_len
+
+    _fits = 1 << 63     # no buffer is that long
 
 
 @lru_cache(maxsize=4096)
