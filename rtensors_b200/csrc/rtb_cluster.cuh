@@ -10,6 +10,24 @@ constexpr unsigned kWideCluster = 16;                   // what a kernel may opt
 constexpr unsigned long long kWaitNs = 2000000000ull;   // limit of a wait for another CTA's values
 constexpr uint64_t kMaxGrid = 0x7fffffffull;
 
+// A limit by device that only ever rises, shared by all contexts and threads: `set` is what raises it, never while another raise
+// is under way, so that a smaller one cannot come last.
+class RisingLimit {
+    std::mutex mu;
+    std::atomic<size_t> reached[64] = {};
+
+  public:
+    template <typename F> int raise(int device, size_t to, F set) {
+        std::atomic<size_t> &mark = reached[device & 63];
+        if (mark.load(std::memory_order_acquire) >= to) return RTB_OK;
+        std::lock_guard<std::mutex> lock(mu);
+        if (mark.load(std::memory_order_relaxed) >= to) return RTB_OK;
+        if (int rc = set()) return rc;
+        mark.store(to, std::memory_order_release);
+        return RTB_OK;
+    }
+};
+
 #ifdef __CUDACC__
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack {
     T e[V];
@@ -90,13 +108,11 @@ __device__ __forceinline__ bool mbar_wait(unsigned long long *bar, unsigned pari
 
 // Allows a kernel `smem` bytes of dynamic shared memory (on first use on a device; each kernel instantiates this function).
 template <typename A, void (*kernel)(A)> int allow_smem(Ctx *ctx, size_t smem) {
-    static std::atomic<uint64_t> allowed[64];   // by device
-    std::atomic<uint64_t> &mark = allowed[ctx->device & 63];
-    if (smem && mark.load(std::memory_order_relaxed) < smem) {
+    static RisingLimit limit;
+    return limit.raise(ctx->device, smem, [&]() -> int {
         RTB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-        mark.store(smem, std::memory_order_relaxed);
-    }
-    return RTB_OK;
+        return RTB_OK;
+    });
 }
 
 // How many clusters of `cluster` CTAs (1 to 16) of a kernel an idle device runs at once; above 8 it may be none, and a size must
