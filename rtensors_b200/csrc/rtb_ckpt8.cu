@@ -77,16 +77,26 @@ struct Quantise32 {
         return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     }
 };
-// f64: the quotient as IEEE arithmetic gives it; the product with a reciprocal decides all but the values within 1e-8 of a tie.  An
-// approximate reciprocal within 2^-18, refined once by Newton's step, is within 2^-36, and 127 times that is below 2e-9.
+// f64: the product with a reciprocal decides all but the values within 1e-8 of a tie.  An approximate reciprocal within 2^-18, refined
+// once by Newton's step, is within 2^-36, and 127 times that is below 2e-9.  What is left is decided by the sign of
+// 254 |x| - (2 n + 1) m for the whole number n below the quotient: both products as exact sums of two numbers, compared part by part.
+// Such a decision is made for all four values of a lane, and its warp waits: 34M values of 0, 1/2 and 1, a third of
+// them ties, 240 us instead of 48 (the f32 division: 67M 429 us instead of 53).
 struct Quantise64 {
-    double m, inv, down;
+    double m, inv, scale;
     bool wide;
-    __device__ __forceinline__ explicit Quantise64(double mag) : m(mag), down(1.0), wide(!(mag > 1e-280 && mag < 1e300)) {
+    __device__ __forceinline__ explicit Quantise64(double mag) : m(mag), scale(1.0), wide(!(mag > 1e-280 && mag < 1e300)) {
         double r;
         asm("rcp.approx.ftz.f64 %0, %1;" : "=d"(r) : "d"(mag));
         inv = 127.0 * fma(r, fma(-mag, r, 1.0), r);
-        if (mag > 1e300) m = mag * 0x1p-20, down = 0x1p-20;   // 127 x stays finite
+        if (wide) scale = mag > 1.0 ? 0x1p-20 : 0x1p512, m = mag * scale;   // the products stay finite, their lower parts normal
+    }
+    __device__ __forceinline__ uint32_t exact(double x) const {
+        const double s = fabs(x) * scale, n = floor(127.0 * s / m), odd = 2.0 * n + 1.0;
+        const double left = 254.0 * s, right = odd * m;
+        const double d = (left - right) + (fma(254.0, s, -left) - fma(odd, m, -right));
+        const int c = (int)n + (d > 0.0 || (d == 0.0 && ((int)n & 1)) ? 1 : 0);
+        return (uint32_t)(x < 0.0 ? -c : c);
     }
     __device__ __forceinline__ uint32_t codes(const double x[4]) const {
         const double magic = 6755399441055744.0;   // 1.5 2^52
@@ -100,7 +110,7 @@ struct Quantise64 {
         }
         if (wide || off > 0.49999999) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) c[k] = m > 0.0 ? (uint32_t)(int)rint(127.0 * (x[k] * down) / m) : 0u;
+            for (int k = 0; k < 4; ++k) c[k] = m > 0.0 ? exact(x[k]) : 0u;
         }
         return __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     }
