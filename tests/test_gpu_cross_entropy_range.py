@@ -108,3 +108,25 @@ def test_a_loss_that_only_the_mean_can_hold():
         # log2 e as a float is off by half a rounding, its product with the difference is the loss
         assert abs(float(cross_entropy_loss(_t(x), _t(t)).item()) - want) <= 4 * U[np.float32] * want
         assert cross_entropy_loss(_t(x), _t(t), reduction="sum").item() == np.inf
+
+
+@DTYPES
+@pytest.mark.parametrize("classes", CLASSES)
+def test_infinities_next_to_far_maxima(dt, classes):
+    """Classes masked with -inf in rows far from zero take no part; one +inf, a NaN or nothing but -inf give NaN, in that row alone."""
+    from rtensors_b200.tensor import cross_entropy_loss
+    rng = np.random.default_rng(classes + 4)
+    x = rng.standard_normal((7, classes)).astype(dt)
+    t = np.zeros(7, np.int64)
+    for r, v in enumerate((5e6, -1e10, 1e20, -3e37)):
+        x[r] = -np.inf
+        left = rng.choice(classes, 2, replace=False)
+        x[r, left] = v
+        t[r] = left[0]
+    x[4, classes // 2], x[5, classes // 2], x[6] = np.inf, np.nan, -np.inf
+    x[4:6, 0] = -1e20
+    _check(x[:4].copy(), t[:4])
+    loss, g = cross_entropy_loss(_t(x), _t(t), True)
+    g, (_, _, g_w, g_tol) = g.cpu(), _ce_ref(x[:4], t[:4], False, U[dt])
+    assert np.isnan(loss.item()) and np.isnan(g[4:]).all()
+    _close(g[:4] * 7, g_w, g_tol + 4 * U[dt] * np.abs(g_w))     # a seventh each: the mean's factor rounds, and its product
