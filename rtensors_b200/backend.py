@@ -447,7 +447,7 @@ class CudaB200:
         xm.check_extent(x.numel()); gm.check_extent(gate.numel())
         out = x.new_empty(max(xm.size, 1))
         flags = (L.SCAN_REVERSE if reverse else 0) | (L.SCAN_COUPLED if coupled else 0)
-        self._call(self._lib.rtb_gated_scan, dtype_code(x), flags, gate.data_ptr(), gm.c_strides, gm.offset,
+        self._call(self._lib.rtb_gated_scan, TORCH_TO_CODE[x.dtype], flags, gate.data_ptr(), gm.c_strides, gm.offset,
                    x.data_ptr(), xm.c_strides, xm.offset, None if h0 is None else h0.data_ptr(), out.data_ptr(),
                    rank, xm.c_shape, axis)
         return out
@@ -504,7 +504,7 @@ class CudaB200:
         if gm.shape != sm.shape or xm.shape != sm.shape:
             self._views(sm.shape, (gate, gm), (x, xm))
         sm.check_extent(state.numel()); gm.check_extent(gate.numel()); xm.check_extent(x.numel())
-        self._call(self._lib.rtb_gated_step, dtype_code(state), L.SCAN_COUPLED if coupled else 0, state.data_ptr(), sm.c_strides, sm.offset,
+        self._call(self._lib.rtb_gated_step, TORCH_TO_CODE[dt], L.SCAN_COUPLED if coupled else 0, state.data_ptr(), sm.c_strides, sm.offset,
                    gate.data_ptr(), gm.c_strides, gm.offset, x.data_ptr(), xm.c_strides, xm.offset, sm.rank, sm.c_shape)
 
     def ckpt8_store(self, src: torch.Tensor, n: Optional[int] = None, offset: int = 0) -> torch.Tensor:
@@ -512,7 +512,8 @@ class CudaB200:
         n = src.numel() - offset if n is None else n
         if offset < 0 or n < 0 or offset + n > src.numel():
             raise L.RtbError(L.ERR_BOUNDS, f"range [{offset}, {offset + n}) exceeds a buffer of {src.numel()}")
-        self._same(src)
+        if src.get_device() != self._index:
+            self._same(src)
         es = src.element_size()
         at, total = ckpt8_layout(n, es)
         out = torch.empty(total or 1, dtype=torch.int8, device=self._torch_device)
@@ -529,14 +530,14 @@ class CudaB200:
 
     def ckpt8_restore(self, ckpt: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
         out = torch.empty(n or 1, dtype=dtype, device=self._torch_device)
-        self._same(out)
         p = ckpt.data_ptr()
         self._call(self._lib.rtb_ckpt8_restore, dtype_code(out), p, p + self._check_ckpt(ckpt, n, out), n, out.data_ptr())
         return out
 
     def ckpt8_grad(self, kind: int, ckpt: torch.Tensor, up: torch.Tensor, n: int, offset: int = 0) -> torch.Tensor:
         """f'(restored) * up without writing the restored tensor (rtb_ckpt8_grad); up: n elements from `offset` on."""
-        self._same(up)
+        if up.get_device() != self._index:
+            self._same(up)
         if offset < 0 or offset + n > up.numel():
             raise L.RtbError(L.ERR_BOUNDS, f"range [{offset}, {offset + n}) exceeds a buffer of {up.numel()}")
         out = up.new_empty(n or 1)
@@ -555,7 +556,8 @@ class CudaB200:
             raise L.RtbError(L.ERR_BOUNDS, "the logits' rows exceed their buffer")
         if targets.dtype != torch.int64 or targets.numel() < rows or not targets.is_contiguous():
             raise L.RtbError(L.ERR_INVALID, f"cross-entropy needs {rows} dense int64 targets")
-        self._same(logits)
+        if logits.get_device() != self._index:
+            self._same(logits)
         if targets.get_device() != self._index:
             raise L.RtbError(L.ERR_INVALID, f"targets on {targets.device} were given to the backend of cuda:{self._index}")
         loss = logits.new_empty(1)

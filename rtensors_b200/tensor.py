@@ -333,7 +333,9 @@ class Tensor:
 
     def gated_step_inplace(self, gate: "Tensor", x: "Tensor", coupled: bool = False) -> "Tensor":
         """One step of the recurrence with this tensor as the state: h = gate h + x (or gate h + (1 - gate) x) in place."""
-        self.backend.gated_step(self.buf, self.meta, gate.buf, self._spread(gate.meta, "the gate"), x.buf, self._spread(x.meta, "x"), coupled)
+        m, gm, xm = self.meta, gate.meta, x.meta
+        self.backend.gated_step(self.buf, m, gate.buf, gm if gm.shape == m.shape else self._spread(gm, "the gate"),
+                                x.buf, xm if xm.shape == m.shape else self._spread(xm, "x"), coupled)
         return self
 
     # ---- 8-bit checkpoints --------------------------------------------------------------------
