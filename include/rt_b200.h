@@ -102,7 +102,10 @@ void rtb_ctx_destroy(rtb_ctx *ctx);
  * only, so a change of stream makes the new stream wait (event record + cudaStreamWaitEvent) for
  * everything this context has enqueued on the old one: calls through one context keep one total
  * order on the device whatever streams they were issued on.  Use one context per stream for work
- * that should overlap. */
+ * that should overlap.  A graph captured through the context holds the addresses of that scratch state: order its replays
+ * with each other, with those of other graphs of the context and with calls through it.  A change of stream and the
+ * call meant for it are two calls: host threads that share a context and set streams of their own need a lock
+ * around the pair. */
 int rtb_ctx_set_stream(rtb_ctx *ctx, void *stream);
 void *rtb_ctx_get_stream(rtb_ctx *ctx);
 int rtb_ctx_device(rtb_ctx *ctx);
@@ -425,9 +428,10 @@ int rtb_convert(rtb_ctx *ctx, int src_dtype, int dst_dtype, const void *src, voi
  *      rtb_gated_step: one step in place, state = gate state + x (or (1 - gate) x) over views of one shape; state must not
  *      be broadcast, and may overlap gate or x only where it is the same view.
  *
- *      Long axes are cut into parts that run in parallel; the results do not depend on timing.  Gates in [-1, 1] behave
- *      as the formula; where a PRODUCT of gates within some thousand steps leaves the type's range, the result
- *      may be inf or NaN though every step's is finite.  A view that is not read in place (its innermost dim strided), and
+ *      Long axes are cut into parts that run in parallel; the results do not depend on timing.  Finite states under gates in
+ *      [-1, 1] behave as the formula, up to the smallest number times the largest state.  Where a PRODUCT of gates within one
+ *      part (up to 65536 steps along a contiguous axis, 8192 else) leaves the type's range, the result may be inf or
+ *      NaN though every step's is finite, and an infinite state may go on as NaN.  A view that is not read in place (its innermost dim strided), and
  *      the gradient of a broadcast gate, may take a block of the context allocator. -------------------------- */
 enum { RTB_SCAN_REVERSE = 1, RTB_SCAN_COUPLED = 2 };
 int rtb_gated_scan(rtb_ctx *ctx, int dtype, int flags, const void *gate, const ptrdiff_t *stride_g, size_t off_g, const void *x,
@@ -459,7 +463,7 @@ int rtb_ckpt8_grad(rtb_ctx *ctx, int dtype, int kind, const int8_t *codes, const
  *        grad_map (dense, may be NULL) = softmax(x_r) - [j = t_r], divided likewise
  *      A row with t_r < 0 does not count and gets a zero map (padding); t_r >= classes makes its map and the loss NaN.
  *      The mean of no row is NaN, the sum 0.  An entry of -inf takes no part; a row of -inf only, of +inf or
- *      with a NaN gives NaN.  f32 / f64; the rows' losses are added in 64 bits in a fixed order.  grad_map may be the
+ *      with a NaN gives NaN.  Finite logits may have any value; in f32 a probability below 2^-126 is zero.  f32 / f64; the rows' losses are added in 64 bits in a fixed order.  grad_map may be the
  *      logits' own buffer when pitch == classes. ---------------------------------------------------------------- */
 int rtb_cross_entropy(rtb_ctx *ctx, int dtype, const void *logits, size_t rows, size_t classes, ptrdiff_t pitch, const int64_t *targets,
                       int reduction, void *loss, void *grad_map);

@@ -1,8 +1,8 @@
 // 8-bit activation checkpoints (format: rtb_ckpt8.cuh): store, restore, and the backward maps of the tape's nodes
 // fed from codes, so that the restored tensor never exists in memory.  All HBM-bound: f32 moves 5 bytes per
 // element to store or restore, 9 to apply a map.  A warp holds a block (four elements a lane), several blocks at a time so that
-// their loads are in flight together; a block's magnitude is one warp-wide maximum of bit patterns.  67M f32: store 54 us
-// (6.2 TB/s), restore 52 us (6.4), a map 90 us (6.7); 34M f64: 49, 48 and 86 us.
+// their loads are in flight together; a block's magnitude is one warp-wide maximum of bit patterns.  67M f32: store 53 us
+// (6.4 TB/s), restore 52 us (6.4), a map 90 us (6.7); 34M f64: 48, 48 and 86 us.
 #include "rtb_internal.h"
 #include "rtb_ckpt8.cuh"
 
@@ -15,6 +15,7 @@ constexpr int kUnroll = 4;   // blocks of a warp, loads of all in flight at once
 
 // The store's chain from load over maximum and reciprocal to code is long, so warps in flight count for more than registers:
 // blocks of a warp, CTAs of an SM.  67M f32: 54 us at 7 or 8 CTAs, 58 at 6, 64 as the compiler chooses; 34M f64: 49 at 8, 51 at 6.
+// At 7 CTAs ptxas takes 32 registers and spills some 100 bytes a thread.
 template <typename T> struct StoreShape;
 template <> struct StoreShape<float> { static constexpr int unroll = 4, ctas = 7; };
 template <> struct StoreShape<double> { static constexpr int unroll = 2, ctas = 8; };

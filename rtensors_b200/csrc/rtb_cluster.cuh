@@ -149,7 +149,7 @@ template <typename A, void (*kernel)(A)> int clusters_at_once(Ctx *ctx, unsigned
 
 // Launches `kernel` with `smem` bytes of dynamic shared memory in clusters of `cluster` CTAs.  early: the grid may start beside
 // its predecessor's last CTAs (programmatic dependent launch).  A long-running grid of one wave should not: it lands on
-// the SMs that happen to be free and stays there (a 270 us recurrence behind another kernel: 435 us).
+// the SMs that happen to be free and stays there (f32 (1, 65536, 256) with 4 heads, backward: 126 us early, 78 us not).
 template <typename A, void (*kernel)(A)>
 int launch_cluster(Ctx *ctx, const char *name, uint64_t grid, unsigned threads, unsigned cluster, size_t smem, bool early, const A &args) {
     if (grid > kMaxGrid) return fail(RTB_ERR_TOO_LARGE, "%s: %zu CTAs are beyond one launch", name, (size_t)grid);

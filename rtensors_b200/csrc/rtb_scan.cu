@@ -16,8 +16,9 @@
 // so results are deterministic.  Copies run ahead in a ring of shared-memory stages; a thread (or a warp) copies what it
 // will read itself, so the ring needs no barrier.
 //
-// A product of gates that leaves the type's range inside one round (at most some thousand steps) makes the
-// carry's share inf or NaN where step-by-step evaluation might not; gates in [-1, 1] cannot.
+// A product of gates that leaves the type's range inside one round (at most 8192 steps of neighbouring lanes, 65536 along a contiguous
+// axis) makes the carry's share inf or NaN where step-by-step evaluation might not; gates in [-1, 1] cannot.  Where such a
+// product underflows, a finite carry's share is zero and an infinite one's NaN.
 #include <algorithm>
 #include <vector>
 

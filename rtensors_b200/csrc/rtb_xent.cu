@@ -12,8 +12,10 @@
 //                         their pairs through shared memory
 //   beyond                a CTA reads the row twice (the second time mostly from L2)
 // A CTA copies the rows ahead into shared memory, vector by vector as it takes a row's vectors from there into registers.
-// f32 with the map: 8192 x 32000 344 us (6.1 TB/s), 16384 x 8192 203 us (5.3), 2048 x 131072 403 us (5.3, clusters of four),
-// 65536 x 1024 106 us (5.0), 262144 x 64 39 us (3.4); 4096 x 10 7 us, a chain of latencies.
+// f32 with the map: 8192 x 32000 340 us (6.2 TB/s), 16384 x 8192 202 us (5.3), 2048 x 131072 400 us (5.4, clusters of four),
+// 65536 x 1024 97 us (5.5), 262144 x 64 35 us (3.8), 1000000 x 10 46 us (1.7: single 4-byte loads, two barriers a tile); 4096 x 10
+// 6 us, a chain of latencies; read twice, 2048 x 300000 1842 us.  The loss alone: 8192 x 32000 227 us (4.6 TB/s): half
+// the bytes, two thirds of the time.
 //
 // A row with t < 0 does not count (padding): its map is zero and its logits are not read.  t >= classes gives NaN for the row
 // and the loss.  Rows are dealt out statically and every sum has a fixed order: results are deterministic.
@@ -68,7 +70,7 @@ __device__ __forceinline__ bool is_far(float c) { return fabsf(c) > kNear; }   /
 __device__ __forceinline__ bool is_far(double) { return false; }
 __device__ __forceinline__ float shift_of(float m) { return is_far(m) ? m : 0.5f * rintf(m * kLog2e); }
 __device__ __forceinline__ double shift_of(double m) { return m; }
-__device__ __forceinline__ float exp2_(float x) {
+__device__ __forceinline__ float exp2_(float x) {   // zero below 2^-126
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;

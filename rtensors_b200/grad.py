@@ -16,7 +16,9 @@ rtensors_b200.tensor) instead of in full.  Kept so: operands of `*` and of `matm
 relu and abs (exact: their values are 0 and +-1), the results of sigmoid, tanh and exp, the input of square, the states of
 gated_scan_at (and x of its coupled form).  Kept in full: leaves and untracked inputs (they live anyway), the gate of a
 recurrence (its errors would add up along the axis), and what other nodes divide by or take a pole of.
-The backward kernels read the codes; only `matmul` restores its operand.
+The backward kernels read the codes; restored in full for the time of their node's backward are operands of `matmul`, an operand of `*`
+that was broadcast, and x of the coupled recurrence.  Each node makes a checkpoint of its own: a tensor that several nodes
+keep is stored once for each, and one that a node keeps in full (a recurrence's gate) is stored beside that for others.
 
     with grad.enabled(ref_quirks=False) as ctx:
         w.param(); b.param()
